@@ -423,7 +423,7 @@ def _exact_append(s, case):
         new = x[a:b].permute(1, 2, 0, 3)  # [K|V][head][token][d]
         amax = new.abs().amax((-1, -2))
         half, e = torch.frexp((amax / E4M3_MAX).clamp(min=2.0 ** -100))
-        want = torch.ldexp(torch.ones_like(half), e - (half == 0.5))  # the power of two at or above it
+        want = torch.ldexp(torch.ones_like(half), e - (half == 0.5).to(e.dtype))  # the power of two at or above it
         if off:
             scale = torch.maximum(scales[page], want)
             pages[page, :, :, :off] = _to_e4m3(pages[page, :, :, :off] * (scales[page] / scale)[..., None, None])
