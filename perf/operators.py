@@ -211,7 +211,7 @@ def prepare(case, seed):
         from disk_streaming_moe_engine_b200 import kv8
         s["cache"] = kv8.Kv8Cache(s["pages"], s["scales"])
         if case["op"] == "attn":
-            s["workspace"] = kv8.attention_workspace(s["cache"], case["n"], t, hk * case["group"])
+            s["workspace"] = kv8.attention_workspace(s["cache"])
     return s
 
 
