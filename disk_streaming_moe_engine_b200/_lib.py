@@ -77,8 +77,34 @@ class DmQuantTensorInfo(C.Structure):
                 ("scales_bytes", C.c_uint64), ("weights_bytes", C.c_uint64)]
 
 
+class DmKv8Cache(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("scales", C.c_void_p), ("num_pages", C.c_int32),
+                ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32)]
+
+
+class DmKv8AttnArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n", C.c_int32), ("num_q_heads", C.c_int32), ("max_q_len", C.c_int32),
+                ("rows", C.c_int32), ("table_width", C.c_int32), ("sm_scale", C.c_float), ("reserved", C.c_int32),
+                ("q", C.c_void_p), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("lse", C.c_void_p), ("block_table", C.c_void_p), ("seq_lens", C.c_void_p), ("cu_q", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("err_dev", C.c_void_p)]
+
+
+class DmRopeParams(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("theta", C.c_double), ("factor", C.c_double), ("original_context", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("attention_factor", C.c_double)]
+
+
+class DmRopePlan(C.Structure):
+    _fields_ = [("freq", C.c_double * 128), ("mscale", C.c_float), ("head_dim", C.c_int32),
+                ("rotary_dim", C.c_int32), ("layout", C.c_int32)]
+
+
 P = C.c_void_p
 I32 = C.c_int32
+I64 = C.c_int64
 U64 = C.c_uint64
 F32 = C.c_float
 
@@ -132,6 +158,14 @@ SIGNATURES = {
     "dm_synth_f16_absnormal": (I32, [U64, U64, U64, F32, P]),
     "dm_synth_model_device": (I32, [P, U64]),
     "dm_moe_layer_noalloc": (I32, [I32, I32, I32, I32, F32, P, P, P, P, P, P, P, P, P, C.c_char_p, U64]),
+    "dm_kv8_status": (I32, [P, P, C.c_char_p, U64]),
+    "dm_kv8_plan": (I32, [I32, P, P, P, I32, P, I32, P, P, P, P, I32, P, P, P, P, P, C.c_char_p, U64]),
+    "dm_rope_plan_init": (I32, [C.POINTER(DmRopeParams), C.POINTER(DmRopePlan), C.c_char_p, U64]),
+    "dm_rope": (I32, [P, I32, I32, P, P, I64, I64, P, I64, I64, I32, P, I64, I64, P, I64, I64, I32, P,
+                      C.c_char_p, U64]),
+    "dm_kv8_append": (I32, [P, I32, I32, P, I64, I64, P, I64, I64, P, P, P, C.c_char_p, U64]),
+    "dm_kv8_attention": (I32, [P, P, P, C.c_char_p, U64]),
+    "dm_kv8_attention_workspace": (I32, [P, C.POINTER(U64), C.c_char_p, U64]),
     "dm_batch_capacity": (I32, [P, C.POINTER(I32)]),
     "dm_decode_batch": (I32, [P, P, P, I32, P, P]),
     "dm_generate_batch": (I32, [P, P, P, I32, I32, P]),

@@ -1,0 +1,45 @@
+// dm_kv8.h — shared by the 8-bit paged KV cache operators: host-side argument checks, the
+// device guard and the kernels' argument structs.
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "dismoen_cuda.h"
+#include "dm_internal.h"
+
+namespace dm {
+
+constexpr int kKv8Page = DM_KV8_PAGE_TOKENS;
+constexpr int kKv8MinExp = -100, kKv8MaxExp = 100;  // scales are 2^k, k in this range
+
+// Formats the error object of dm_last_error's shape into buf and returns code.
+int kv8_err(char* buf, uint64_t size, int code, const char* type, const char* stage, const char* fmt, ...);
+
+// Makes the device that holds `p` current for the scope and restores the old one.
+struct Kv8Device {
+    int prev = -1, dev = -1, num_sms = 0;
+    int enter(const void* p, const char* stage, char* eb, uint64_t es);
+    ~Kv8Device();
+};
+
+int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t es);
+
+// Attention over the cache, as the kernels see it.
+struct Kv8AttnArgs {
+    const uint8_t* pages;
+    const float* scales;
+    const void* q;
+    void* out;
+    float* lse;
+    const int* table;
+    const int* seq_lens;
+    const int* cu_q;      // null: one row per request
+    float* part;          // [slots][8][D + 2] partial results (O rows, then max and sum)
+    unsigned* counters;   // [items] arrivals of the splits of an item
+    uint32_t* err;
+    int64_t q_rs, q_hs, o_rs, o_hs;  // strides in elements
+    float scale_log2;     // sm_scale * log2(e)
+    int n, rows, Hq, Hkv, group, num_pages, width, max_q, nsplit, blocks;
+};
+
+}  // namespace dm

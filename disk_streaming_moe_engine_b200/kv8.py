@@ -1,0 +1,263 @@
+"""Python side of the 8-bit paged KV cache operators (dm_kv8_plan, dm_rope, dm_kv8_append,
+dm_kv8_attention of include/dismoen_cuda.h) over torch CUDA tensors.
+
+A host runtime that keeps its own paged cache runs, per step,
+
+    plan = plan_slots(free, state, table, lens, new_lens, max_tokens)      # pages and slots
+    q, k = rope(rope_plan, q, k, plan.positions)
+    append(cache, k, v, plan.slots)
+    out = attention(cache, q, table, plan.seq_lens, plan.cu_new, max_q_len, workspace=ws)
+
+Every call runs on torch's current stream (or `stream`, a cudaStream_t) of the tensors' device
+and returns without waiting, so a step may be captured into a CUDA graph (with the outputs
+given).  Arguments are checked on the host and raise DmError; what only the device can see
+goes into the error word of `error_word()` and is raised by `check()`.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+PAGE_TOKENS = 16
+MAX_REQUESTS = 8192
+LAYOUTS = {"half": 0, "interleaved": 1}
+SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+_DTYPES = {torch.bfloat16: _lib.DM_DTYPE_BF16, torch.float32: _lib.DM_DTYPE_F32}
+_ERR = 512
+
+
+def _raise(rc: int, buf):
+    raise _lib.DmError(rc, buf.value.decode())
+
+
+def _bad(detail: str):
+    raise _lib.DmError(_lib.DM_ERR_INVALID_ARG, '{"error_type":"INVALID_ARG","detail":"%s","stage":"kv8","layer":-1}' % detail)
+
+
+def _stream(t: torch.Tensor, stream) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream if stream is None else stream
+
+
+def _ints(device, **tensors):
+    """int32, contiguous, on the device."""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.device != device):
+            _bad(f"{name} must be a contiguous int32 tensor on {device}")
+
+
+def _rows(name: str, t: torch.Tensor, heads, dim: int, device, dtype):
+    if (t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or t.device != device
+            or t.dtype != dtype or (t.numel() and t.stride(2) != 1)):
+        _bad(f"{name} must be [rows][{'heads' if heads is None else heads}][{dim}] {dtype} on {device}, head elements "
+             f"contiguous (got {tuple(t.shape)} {t.dtype} on {t.device})")
+
+
+def error_word(device="cuda") -> torch.Tensor:
+    """The device error word the operators OR their DM_DEVERR_* bits into."""
+    return torch.zeros(1, dtype=torch.int32, device=device)
+
+
+def check(err: torch.Tensor, stream=None) -> None:
+    """Waits for the stream, clears the error word and raises DmError when a bit was set."""
+    buf = C.create_string_buffer(_ERR)
+    rc = _lib.load().dm_kv8_status(err.data_ptr(), _stream(err, stream), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+
+
+class Kv8Cache:
+    """pages uint8 [num_pages][K|V][kv heads][16][head_dim] e4m3 codes, scales fp32
+    [num_pages][K|V][kv heads] powers of two; value = code * scale."""
+
+    def __init__(self, pages: torch.Tensor, scales: torch.Tensor):
+        if (pages.dim() != 5 or pages.shape[1] != 2 or pages.shape[3] != PAGE_TOKENS or pages.dtype != torch.uint8
+                or not pages.is_contiguous() or not pages.is_cuda):
+            _bad("pages must be a contiguous uint8 CUDA tensor [num_pages][2][kv heads][16][head_dim]")
+        if (scales.shape != pages.shape[:3] or scales.dtype != torch.float32 or not scales.is_contiguous()
+                or scales.device != pages.device):
+            _bad("scales must be a contiguous float32 tensor [num_pages][2][kv heads] beside the pages")
+        self.pages, self.scales = pages, scales
+        self.device = pages.device
+        self.num_pages, _, self.num_kv_heads, _, self.head_dim = pages.shape
+        self._c = _lib.DmKv8Cache(pages.data_ptr(), scales.data_ptr(), self.num_pages, self.num_kv_heads,
+                                  self.head_dim, 0)
+        self._ref = C.addressof(self._c)
+
+    @classmethod
+    def empty(cls, num_pages: int, num_kv_heads: int, head_dim: int, device="cuda") -> "Kv8Cache":
+        return cls(torch.zeros((num_pages, 2, num_kv_heads, PAGE_TOKENS, head_dim), dtype=torch.uint8, device=device),
+                   torch.full((num_pages, 2, num_kv_heads), 2.0 ** -100, dtype=torch.float32, device=device))
+
+    def values(self) -> torch.Tensor:
+        """The whole cache as fp32 (a copy)."""
+        return self.pages.view(torch.float8_e4m3fn).float() * self.scales[..., None, None]
+
+
+def free_list(num_pages: int, device="cuda"):
+    """(free_pages, free_state) with every page free; page 0 is the first to be taken."""
+    pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+    return pages, torch.tensor([num_pages, 0], dtype=torch.int32, device=device)
+
+
+class SlotPlan(NamedTuple):
+    """seq_lens [n], cu_new [n + 1]; slots, positions, requests [max_tokens] (-1 behind the last token)."""
+    seq_lens: torch.Tensor
+    cu_new: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    requests: torch.Tensor
+
+
+def plan_slots(free_pages, free_state, block_table, ctx_lens, new_lens, max_tokens: int, *, state_out=None,
+               out: SlotPlan | None = None, err=None, stream=None) -> SlotPlan:
+    """dm_kv8_plan: pages for the new tokens of every request (new_lens -1 returns a request's
+    pages), written into block_table and taken from the free list (free_state in place, or to
+    state_out).  `out` may hold the results' tensors; its seq_lens may be ctx_lens."""
+    dev = ctx_lens.device
+    n = ctx_lens.numel()
+    if out is None:
+        tok = torch.empty((3, max_tokens), dtype=torch.int32, device=dev)
+        req = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
+        out = SlotPlan(req[:n], req[n:], tok[0], tok[1], tok[2])
+    else:
+        _ints(dev, **out._asdict())
+        if (out.seq_lens.numel() < n or out.cu_new.numel() < n + 1
+                or min(out.slots.numel(), out.positions.numel(), out.requests.numel()) < max_tokens):
+            _bad("an output of the plan is too small")
+    _ints(dev, ctx_lens=ctx_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
+          free_state=free_state, state_out=state_out, err=err)
+    if new_lens.numel() != n or block_table.dim() != 2 or block_table.shape[0] < n or free_state.numel() != 2 or \
+            (state_out is not None and state_out.numel() != 2):
+        _bad("need new_lens [n], block_table [n][width], free_state [2]")
+    buf = C.create_string_buffer(_ERR)
+    rc = _lib.load().dm_kv8_plan(
+        n, ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1],
+        free_pages.data_ptr(), free_pages.numel(), free_state.data_ptr(),
+        (free_state if state_out is None else state_out).data_ptr(), out.seq_lens.data_ptr(), out.cu_new.data_ptr(),
+        max_tokens, out.slots.data_ptr(), out.positions.data_ptr(), out.requests.data_ptr(),
+        None if err is None else err.data_ptr(), _stream(ctx_lens, stream), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+    return out
+
+
+class RopePlan:
+    """Rotary angles of a head: `rotary_dim` of its `head_dim` elements turn (None: all), in
+    "half" or "interleaved" pairs, unscaled or stretched ("linear", "yarn") by `factor` past
+    `original_context`."""
+
+    def __init__(self, head_dim: int, rotary_dim: int | None = None, *, theta: float = 1e4, layout: str = "half",
+                 scaling: str = "none", factor: float = 1.0, original_context: float = 32768, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, attention_factor: float = 0.0):
+        if layout not in LAYOUTS or scaling not in SCALINGS:
+            _bad(f"unknown layout {layout!r} or scaling {scaling!r}".replace('"', "'"))
+        p = _lib.DmRopeParams(head_dim, head_dim if rotary_dim is None else rotary_dim, LAYOUTS[layout],
+                              SCALINGS[scaling], theta, factor, original_context, beta_fast, beta_slow,
+                              attention_factor)
+        self._c = _lib.DmRopePlan()
+        self._ref = C.addressof(self._c)
+        buf = C.create_string_buffer(_ERR)
+        rc = _lib.load().dm_rope_plan_init(C.byref(p), C.byref(self._c), buf, _ERR)
+        if rc != _lib.DM_OK:
+            _raise(rc, buf)
+        self.head_dim, self.rotary_dim, self.layout = self._c.head_dim, self._c.rotary_dim, layout
+        self.mscale = self._c.mscale
+
+    @property
+    def freq(self) -> list[float]:
+        return list(self._c.freq[:self.rotary_dim // 2])
+
+
+def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None):
+    """dm_rope: rotated q [n][Hq][D] and k [n][Hk][D] (k may be None).  q_out / k_out may be
+    q / k themselves; rows at negative positions are skipped."""
+    dev, D = positions.device, plan.head_dim
+    n = positions.numel()
+    _ints(dev, positions=positions)
+    if q.dtype not in _DTYPES:
+        _bad(f"q is bf16 or fp32 (got {q.dtype})")
+    k = q[:, :0] if k is None else k
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
+    for name, t, like in (("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)):
+        _rows(name, t, like.shape[1], D, dev, q.dtype)
+        if t.shape[0] != n:
+            _bad(f"{name} has {t.shape[0]} rows, positions {n}")
+    buf = C.create_string_buffer(_ERR)
+    rc = _lib.load().dm_rope(
+        plan._ref, _DTYPES[q.dtype], n, positions.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
+        q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1], k.data_ptr(), k.stride(0), k.stride(1),
+        k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1], _stream(positions, stream), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+    return q_out, k_out
+
+
+def append(cache: Kv8Cache, k, v, slots, *, err=None, stream=None) -> None:
+    """dm_kv8_append: k, v [n][kv heads][D] quantised into slots [n] of the cache's pages."""
+    n = slots.numel()
+    if k.dtype not in _DTYPES:
+        _bad(f"k is bf16 or fp32 (got {k.dtype})")
+    _rows("k", k, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
+    _rows("v", v, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
+    _ints(cache.device, slots=slots, err=err)
+    if k.shape[0] < n or v.shape[0] < n:
+        _bad(f"{n} slots, k has {k.shape[0]} rows, v {v.shape[0]}")
+    buf = C.create_string_buffer(_ERR)
+    rc = _lib.load().dm_kv8_append(
+        cache._ref, _DTYPES[k.dtype], n, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+        v.stride(1), slots.data_ptr(), None if err is None else err.data_ptr(), _stream(slots, stream), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+
+
+def attention_workspace(cache: Kv8Cache) -> torch.Tensor:
+    """A zeroed workspace for attention() calls on this cache's geometry; calls that may run
+    at the same time need one each."""
+    nbytes = C.c_uint64()
+    buf = C.create_string_buffer(_ERR)
+    with torch.cuda.device(cache.device):
+        rc = _lib.load().dm_kv8_attention_workspace(cache._ref, C.byref(nbytes), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+    return torch.zeros(nbytes.value, dtype=torch.uint8, device=cache.device)
+
+
+def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: int = 1, *, sm_scale=None, out=None,
+              lse=None, workspace, err=None, stream=None) -> torch.Tensor:
+    """dm_kv8_attention: q [rows][Hq][D] against the cached tokens of each request; rows
+    [cu_q[i], cu_q[i + 1]) belong to request i and are its last tokens (cu_q None: one row
+    per request).  Rows from cu_q[n] on are left as they were in `out`."""
+    dev, D = cache.device, cache.head_dim
+    n = seq_lens.numel()
+    if q.dtype not in _DTYPES:
+        _bad(f"q is bf16 or fp32 (got {q.dtype})")
+    _rows("q", q, None, D, dev, q.dtype)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _rows("out", out, q.shape[1], D, dev, q.dtype)
+    _ints(dev, block_table=block_table, seq_lens=seq_lens, cu_q=cu_q, err=err)
+    if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \
+            out.shape[0] < q.shape[0]:
+        _bad("need block_table [n][width], cu_q [n + 1] and out of q's shape")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or
+                            not lse.is_contiguous() or lse.device != dev):
+        _bad("lse must be a contiguous float32 [rows][Hq]")
+    if workspace.device != dev or not workspace.is_contiguous():
+        _bad("the workspace must be a contiguous tensor on the cache's device")
+    a = _lib.DmKv8AttnArgs(
+        _DTYPES[q.dtype], n, q.shape[1], max_q_len, q.shape[0], block_table.shape[1],
+        D ** -0.5 if sm_scale is None else sm_scale, 0, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
+        out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), None if err is None else err.data_ptr())
+    buf = C.create_string_buffer(_ERR)
+    rc = _lib.load().dm_kv8_attention(cache._ref, C.addressof(a), _stream(q, stream), buf, _ERR)
+    if rc != _lib.DM_OK:
+        _raise(rc, buf)
+    return out

@@ -454,6 +454,167 @@ int32_t dm_moe_layer_noalloc(int32_t hidden_size, int32_t moe_intermediate_size,
                              const float* x_mid_dev, float* x_out_dev, int32_t* ids_dev,
                              float* probs_dev, void* stream, char* err_buf, uint64_t err_buf_size);
 
+/* ---- 8-bit paged KV cache: operators over buffers the caller owns -----------------------
+ * No counterpart in the reference (its caches hold bf16 or fp32).  The
+ * serving chain of a host runtime that keeps its own paged cache in half the bytes:
+ *   dm_kv8_plan       block tables and slot maps from request lengths, on the device
+ *   dm_rope           rotary positions of the step's queries and keys
+ *   dm_kv8_append     new K / V rows quantised into the cache's pages
+ *   dm_kv8_attention  attention over the cache, one token or a ragged chunk per request
+ * Every call enqueues on `stream` (a cudaStream_t; NULL = the legacy default stream) and
+ * returns without waiting; it allocates nothing and may be captured into a CUDA graph.
+ * The device is the one that holds the first device pointer; the current device is left
+ * as it was.  All pointers are device memory of that device unless marked _host.
+ * Statuses and err_buf are as in dm_moe_layer_noalloc.  What only the device can see (a
+ * page id out of range, lengths that do not fit) is OR-ed as DM_DEVERR_* bits into
+ * *err_dev (one uint32, may be NULL) and the access is skipped; dm_kv8_status reads it.
+ *
+ * Cache layout (the engine's page layout, one byte per value):
+ *   pages  uint8 [num_pages][K|V][Hkv][16][D]   e4m3 codes
+ *   scales fp32  [num_pages][K|V][Hkv]          powers of two 2^k, k in [-100, 100]
+ *   value = code * scale.  A power-of-two scale makes the scaling exact in both
+ *   directions, so a stored value is off by its one e4m3 rounding alone; e4m3 has the same
+ *   relative step under any scale, so a finer scale would gain nothing.
+ * head_dim in {64, 128, 256}; pages 16-byte aligned. */
+#define DM_KV8_PAGE_TOKENS 16
+#define DM_KV8_MAX_REQUESTS 8192
+#define DM_DEVERR_NONFINITE 0x2u  /* NaN / Inf among the appended values                  */
+#define DM_DEVERR_CAPACITY 0x4u   /* pages, table width or token buffers do not suffice   */
+#define DM_DEVERR_PAGE 0x8u       /* a page id or slot outside the cache                  */
+#define DM_DEVERR_RANGE 0x20u     /* a length, row range or slot order out of contract    */
+typedef struct dm_kv8_cache {
+    uint8_t* pages;
+    float* scales;
+    int32_t num_pages;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t reserved;   /* 0 */
+} dm_kv8_cache;
+
+/* Waits for `stream`, reads and clears *err_dev and returns it as a status (DM_OK,
+ * DM_ERR_CAPACITY, DM_ERR_INVALID_ARG for PAGE and RANGE, DM_ERR_NONFINITE). */
+int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t err_buf_size);
+
+/* Plans one step of n requests (1 <= n <= DM_KV8_MAX_REQUESTS).  Request i holds ctx_lens[i]
+ * tokens and gets new_lens[i] more (0 allowed); new_lens[i] = -1 ends it: its pages go back
+ * to the free list first and its length becomes 0.
+ *   block_table [n][table_width] page ids; row i's first ceil(ctx/16) entries are in use.
+ *     The entries of the pages that the new tokens need are written; the others stay.
+ *   free_pages [free_capacity]: a stack, its first free_state[0] entries are free pages.
+ *     The j-th new page (in request, then page order) is the j-th from the top of
+ *     free_pages[0 .. count) followed by the released pages (same order).
+ *   free_state int32[2] {count, 0}; free_state_out receives {count after, 0} and may be the
+ *     same array (its second word is the library's, zero between calls).
+ *   seq_lens [n] lengths after the step (may be ctx_lens itself), cu_new [n + 1] prefix sums
+ *     of the new tokens, and per new token (request, then position order) slots[t] =
+ *     page * 16 + position % 16, positions[t], requests[t]; entries [total, max_tokens)
+ *     of these three become -1.
+ * All or nothing: when pages, the table's width, max_tokens or free_capacity do not suffice
+ * (DM_DEVERR_CAPACITY) or a length is negative (DM_DEVERR_RANGE), no page moves, the
+ * lengths stay ctx_lens, cu_new is all 0 and the token arrays all -1.
+ * n * table_width <= 2^27, max_tokens <= 2^30. */
+int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table,
+                    int32_t table_width, int32_t* free_pages, int32_t free_capacity, const int32_t* free_state,
+                    int32_t* free_state_out, int32_t* seq_lens, int32_t* cu_new, int32_t max_tokens, int32_t* slots,
+                    int32_t* positions, int32_t* requests, uint32_t* err_dev, void* stream, char* err_buf,
+                    uint64_t err_buf_size);
+
+/* Rotary positions.  A plan (host memory, plain data, never freed) holds the angles per
+ * position of the rotary_dim / 2 pairs in 64 bits:
+ *   f_i = theta^(-2 i / rotary_dim)
+ *   DM_ROPE_LINEAR: f_i / factor
+ *   DM_ROPE_YARN:   f_i (1 - g_i) + (f_i / factor) g_i, g_i the ramp from 0 to 1 between the
+ *     pairs that turn beta_fast and beta_slow times over original_context positions (their
+ *     indices rounded outwards); the rotated values are multiplied by attention_factor
+ *     (<= 0: 0.1 ln(factor) + 1).
+ * layout DM_ROPE_HALF pairs element i with i + rotary_dim / 2, DM_ROPE_INTERLEAVED 2i with
+ * 2i + 1; elements from rotary_dim on pass through. */
+#define DM_ROPE_HALF 0
+#define DM_ROPE_INTERLEAVED 1
+#define DM_ROPE_NONE 0
+#define DM_ROPE_LINEAR 1
+#define DM_ROPE_YARN 2
+typedef struct dm_rope_params {
+    int32_t head_dim;          /* multiple of 8, <= 256                                   */
+    int32_t rotary_dim;        /* multiple of 16, <= head_dim                             */
+    int32_t layout;
+    int32_t scaling;
+    double theta;              /* > 1                                                     */
+    double factor;             /* >= 1 (linear, yarn)                                     */
+    double original_context;   /* > 0 (yarn)                                              */
+    double beta_fast, beta_slow;  /* > 0, fast > slow (yarn; usual 32 and 1)              */
+    double attention_factor;
+} dm_rope_params;
+typedef struct dm_rope_plan {
+    double freq[128];
+    float mscale;
+    int32_t head_dim, rotary_dim, layout;
+} dm_rope_plan;
+int32_t dm_rope_plan_init(const dm_rope_params* params_host, dm_rope_plan* plan_host, char* err_buf,
+                          uint64_t err_buf_size);
+/* Rotates q [n][Hq][D] and k [n][Hk][D] of the tokens at positions[n] (either may have no
+ * heads).  dtype DM_DTYPE_BF16 or DM_DTYPE_F32; strides in elements between tokens and
+ * between heads, elements of a head contiguous.  q_out / k_out may be q / k with the same
+ * strides (then the elements that pass through are not touched); no other overlap.  Angles
+ * are reduced in 64 bits, products in fp32, one rounding to the output type.  A row with a
+ * negative position is skipped: its outputs stay as they were. */
+int32_t dm_rope(const dm_rope_plan* plan_host, int32_t dtype, int32_t n, const int32_t* positions, const void* q,
+                int64_t q_row_stride, int64_t q_head_stride, void* q_out, int64_t q_out_row_stride,
+                int64_t q_out_head_stride, int32_t Hq, const void* k, int64_t k_row_stride, int64_t k_head_stride,
+                void* k_out, int64_t k_out_row_stride, int64_t k_out_head_stride, int32_t Hk, void* stream,
+                char* err_buf, uint64_t err_buf_size);
+
+/* Quantises k, v [n][Hkv][D] (dtype bf16 or fp32, strides in elements) into the slots
+ * slots[n] (page * 16 + offset; -1 skips the row).  The rows of one page must be adjacent
+ * and their offsets ascend by one, as dm_kv8_plan gives them (otherwise DM_DEVERR_RANGE and
+ * the later rows are skipped; a page that comes up again elsewhere in the call is undefined).
+ * Per page, K|V and head, with the page's first new offset o and the largest finite |x|
+ * of its new rows: want = the smallest 2^k >= max / 448 (k in [-100, 100]).  o = 0 starts the
+ * page afresh, scale = want; else scale = max(want, the page's scale), and when it grows the
+ * codes before o are rounded again by the ratio.  Codes are x / scale to nearest even e4m3;
+ * +-Inf become the largest code, NaN the NaN code, both raise DM_DEVERR_NONFINITE. */
+int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, const void* k, int64_t k_row_stride,
+                      int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                      const int32_t* slots, uint32_t* err_dev, void* stream, char* err_buf, uint64_t err_buf_size);
+
+/* Attention over the cache: o = softmax(sm_scale q K^T) V, query head h reading kv head
+ * h / (Hq / Hkv).  Request i has seq_lens[i] tokens in the pages of block_table row i
+ * (its new tokens already appended) and the query rows [cu_q[i], cu_q[i + 1]) of q and out
+ * [rows][Hq][D]; its query j of m sees the keys before seq_lens[i] - m + j + 1.  cu_q NULL:
+ * one query per request, row i.  A query that sees no key gets zeros (lse -inf); rows from
+ * cu_q[n] on stay as they were.  max_q_len >= every request's query count (a request with
+ * more is skipped, DM_DEVERR_RANGE); it also chooses the kernel.  A key on a page id out of
+ * range is left out (DM_DEVERR_PAGE), and so are keys beyond the table's width
+ * (DM_DEVERR_CAPACITY).  NaN codes of keys that a query does not see do not reach it.
+ * dtype (q and out) bf16 or fp32; scores, softmax and sums are fp32.
+ * lse (may be NULL) [rows][Hq] receives ln sum exp of the scaled scores.
+ * workspace: dm_kv8_attention_workspace bytes, 256-byte aligned, zeroed once before its
+ * first use; every call leaves it ready for the next.  Calls that may overlap in time
+ * (other streams, graphs) need workspaces of their own. */
+typedef struct dm_kv8_attn_args {
+    int32_t dtype, n, num_q_heads, max_q_len;
+    int32_t rows;              /* rows of q and out                                       */
+    int32_t table_width;
+    float sm_scale;
+    int32_t reserved;          /* 0 */
+    const void* q;
+    int64_t q_row_stride, q_head_stride;
+    void* out;
+    int64_t out_row_stride, out_head_stride;
+    float* lse;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    const int32_t* cu_q;
+    void* workspace;
+    uint64_t workspace_bytes;
+    uint32_t* err_dev;
+} dm_kv8_attn_args;
+int32_t dm_kv8_attention(const dm_kv8_cache* cache_host, const dm_kv8_attn_args* args_host, void* stream,
+                         char* err_buf, uint64_t err_buf_size);
+/* Bytes for any call with this cache geometry on the current device. */
+int32_t dm_kv8_attention_workspace(const dm_kv8_cache* cache_host, uint64_t* bytes_out, char* err_buf,
+                                   uint64_t err_buf_size);
+
 /* ---- synthetic checkpoint (seeded; host and device generate the same distributions) --
  * Counter-based generator: element i of stream `stream_id` under `seed` is a pure
  * function of (seed, stream_id, i), so any subrange can be produced independently. */
