@@ -1,0 +1,731 @@
+// dm_kv8_keys.cu — attention over the 8-bit paged cache with the keys on the tensor cores' M
+// side: one token (or a few query rows) per request against long caches, any type.
+//
+// Work: an item is RB query rows (a row = one query token and one query head) of one request
+// and kv head; its keys come in tiles of 128 tokens (8 pages).  Per tile, on tcgen05 with
+// e4m3 operands straight from the cache's bytes (no conversion of the cache at all):
+//   S^T [128 tokens x N] = codeK [128 x D] . Qterms^T [D x N]
+//   O^T [D x N]         += codeV^T [D x 128] . Pterms [128 x N]
+// N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
+// scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
+// before it left) and costs only N: 2 terms give bf16's 8 bits, 6 give 24.  The tensor time of
+// a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
+// below the time of the tile's bytes from HBM, which is what bounds the kernel.
+//
+// Softmax in base 2: with a page's scales sK, sV = 2^v,
+//   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
+// M the row's reference for x + v: raised to the running maximum whenever some x + v exceeds
+// it by more than 2 (then O^T and the sums are rescaled), so w <= 4 and 64 w stays in e4m3's
+// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t owns token t of the tile: its scores, its
+// weights, its share of the row sums; nothing else crosses threads but the reference.
+//
+// Split: all items' tiles in one sequence, cut into one contiguous range per CTA (one CTA per
+// SM, persistent), so ragged lengths balance to a tile.  An item cut by a range boundary
+// leaves partial O, M, sum in the workspace, and the last of its CTAs to arrive joins them in
+// range order: the result does not depend on timing.
+//
+// Roles (192 threads): warps 0-3 softmax, epilogue and Q preparation; warp 4 producer (8 lanes,
+// one page each: page id and scales two tiles ahead, TMA boxes of 16 rows; a missing page
+// reads zeros); warp 5 MMA (one thread).  All waits are bounded; after a timeout every role
+// leaves and copies and MMAs in flight are waited for.
+#include <cmath>
+
+#include "dm_kv8_tc.cuh"
+
+namespace dm {
+
+constexpr int kKeyThreads = 192;
+constexpr int kKeyTile = 128;
+constexpr int kKeyPages = kKeyTile / kKv8Page;
+constexpr int kKeySmem = 227 * 1024 - 2048;  // dynamic shared memory (static arrays beside it)
+constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
+constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
+
+template <typename T, int D, int RB>
+struct KeyShape {
+    static constexpr int kTerms = sizeof(T) == 4 ? 6 : 2;
+    static constexpr int kN = RB * kTerms;
+    static constexpr int CW = D >= 128 ? 128 : D;
+    static constexpr int kChunks = D / CW;
+    static constexpr int kTileBytes = kKeyTile * D;   // K or V of a tile
+    static constexpr int kStage = 2 * kTileBytes;
+    static constexpr int kQ = kN * D;
+    static constexpr int kP = kN * kKeyTile;          // one of two buffers
+    static constexpr int kFixed = kQ + 2 * kP + 1024;
+    static constexpr int kFit = (kKeySmem - kFixed) / kStage;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kFixed;
+    static constexpr int kColsUsed = (2 + kChunks) * kN;
+    static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+    static_assert(kStages >= 2 && kN % 16 == 0 && kColsUsed <= 512, "shape");
+    static_assert(kQ % 1024 == 0 && kP % 1024 == 0, "tiles start at the swizzle's 1024 bytes");
+};
+
+struct KeyArgs {
+    CUtensorMap map;
+    Kv8AttnArgs a;
+};
+
+// What a role knows of the request it is at.
+struct KeyReq {
+    int row0, m, len, full, blocks, tiles;
+};
+
+template <int RB>
+DM_DEV KeyReq key_req(const Kv8AttnArgs& a, int i, bool report) {
+    KeyReq r;
+    r.row0 = i;
+    r.m = 1;
+    if (a.cu_q) {
+        r.row0 = a.cu_q[i];
+        const long long m = static_cast<long long>(a.cu_q[i + 1]) - r.row0;
+        if (r.row0 < 0 || m < 0 || m > a.max_q || r.row0 + m > a.rows) {
+            if (report) raise_error(a.err, DM_DEVERR_RANGE);
+            r.m = 0;
+        } else {
+            r.m = static_cast<int>(m);
+        }
+    }
+    r.full = a.seq_lens[i];
+    if (r.full < 0) {
+        if (report) raise_error(a.err, DM_DEVERR_RANGE);
+        r.full = 0;
+    }
+    r.len = r.full;
+    if (r.len > a.width * kKv8Page) {
+        if (report) raise_error(a.err, DM_DEVERR_CAPACITY);
+        r.len = a.width * kKv8Page;
+    }
+    r.blocks = static_cast<int>((static_cast<long long>(r.m) * a.group + RB - 1) / RB);
+    r.tiles = max(1, (r.len + kKeyTile - 1) / kKeyTile);
+    return r;
+}
+
+// keys that a block's rows see: every row those before lo, its last token's rows those before hi
+template <int RB>
+DM_DEV void key_limits(const Kv8AttnArgs& a, const KeyReq& r, int blk, int& lo, int& hi) {
+    const int rows = r.m * a.group;
+    const int first = blk * RB / a.group, last = (min(rows, (blk + 1) * RB) - 1) / a.group;
+    lo = min(r.len, max(0, r.full - r.m + first + 1));
+    hi = min(r.len, max(0, r.full - r.m + last + 1));
+}
+
+// Position in the sequence of all items' tiles: request, then row block, kv head, tile.
+template <int RB>
+struct KeyWalk {
+    const Kv8AttnArgs& a;
+    long long unit, end;  // this CTA's range
+    int req, blk, h, tile;
+    KeyReq r;
+    DM_DEV KeyWalk(const Kv8AttnArgs& args, long long u0, long long u1, int rq, long long rem) : a(args), unit(u0), end(u1) {
+        req = rq;
+        r = key_req<RB>(a, req, false);
+        tile = static_cast<int>(rem % r.tiles);
+        const long long q = rem / r.tiles;
+        h = static_cast<int>(q % a.Hkv);
+        blk = static_cast<int>(q / a.Hkv);
+    }
+    // tiles of the current item in the range: [tile, tile + count) of the sequence
+    DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(r.tiles - tile), end - unit)); }
+    DM_DEV void next(int cnt) {
+        unit += cnt;
+        if (unit >= end) return;
+        tile = 0;
+        if (++h < a.Hkv) return;
+        h = 0;
+        if (++blk < r.blocks) return;
+        blk = 0;
+        do {
+            if (++req >= a.n) {  // only if the lengths changed under the kernel
+                end = unit;
+                return;
+            }
+            r = key_req<RB>(a, req, false);
+        } while (r.blocks == 0);
+    }
+};
+
+template <typename T, int D, int RB>
+__global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
+    using S = KeyShape<T, D, RB>;
+    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages;
+    const Kv8AttnArgs& a = ka.a;
+    extern __shared__ __align__(1024) uint8_t key_raw[];
+    uint8_t* sm = key_raw + ((1024u - (smem_u32(key_raw) & 1023u)) & 1023u);
+    uint8_t* s_q = sm + ST * S::kStage;
+    uint8_t* s_p = s_q + S::kQ;
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
+    __shared__ float2 s_meta[ST][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
+    __shared__ float s_frow[RB];
+    __shared__ int s_lim[RB];
+    __shared__ float s_red[4][RB];
+    __shared__ unsigned long long s_sum[kKeyThreads / 32 + 1];
+    __shared__ long long s_rem;
+    __shared__ unsigned long long s_total;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_req, s_abort;
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* abort_flag = &s_abort;
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_ready[i], 128);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(&q_ready, 128);
+        mbar_init(&done_bar, 1);
+        mbar_fence_init();
+        s_abort = 0;
+    }
+    if (warp == 5) tc_alloc(&s_tmem, S::kCols);
+
+    // this CTA's range of the tile sequence: block-wide sums of the requests' tiles
+    const int per = (a.n + kKeyThreads - 1) / kKeyThreads;
+    const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
+    unsigned long long mine = 0;
+    for (int i = i0; i < i1; ++i) {
+        const KeyReq r = key_req<RB>(a, i, blockIdx.x == 0);
+        mine += static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
+    }
+    unsigned long long pre = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, pre, o);
+        if (lane >= o) pre += y;
+    }
+    if (lane == 31) s_sum[warp] = pre;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    unsigned long long base = 0, total = 0;
+    for (int w = 0; w < kKeyThreads / 32; ++w) {
+        if (w < warp) base += s_sum[w];
+        total += s_sum[w];
+    }
+    pre += base - mine;  // tiles before this thread's requests
+    const unsigned long long grid = min(static_cast<unsigned long long>(gridDim.x), total);
+    const bool active = blockIdx.x < grid;
+    const long long u0 = active ? static_cast<long long>(total * blockIdx.x / grid) : 0;
+    const long long u1 = active ? static_cast<long long>(total * (blockIdx.x + 1) / grid) : 0;
+    if (active && static_cast<unsigned long long>(u0) >= pre && static_cast<unsigned long long>(u0) < pre + mine) {
+        unsigned long long at = pre;
+        for (int i = i0; i < i1; ++i) {
+            const KeyReq r = key_req<RB>(a, i, false);
+            const unsigned long long c = static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
+            if (static_cast<unsigned long long>(u0) < at + c) {
+                s_req = i;
+                s_rem = static_cast<long long>(u0 - at);
+                break;
+            }
+            at += c;
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem = s_tmem;
+
+    if (active && warp == 4) {
+        // ---------------- producer: 8 lanes, one page of a tile each ----------------
+        uint32_t use = 0;  // tiles issued
+        bool ok = true;
+        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        // pipeline over this CTA's tiles: page ids two ahead, scales one ahead
+        KeyWalk<RB> wi = w;      // walks ahead of w
+        int ti = -1, ei = 0;     // next tile of wi's item, end of its tiles
+        auto next_id = [&](int& id, int& h) {  // page id of this lane in the next tile (-1: none)
+            id = -1;
+            h = 0;
+            while (wi.unit < wi.end) {
+                if (ti < 0) {
+                    int lo, hi;
+                    key_limits<RB>(a, wi.r, wi.blk, lo, hi);
+                    ti = wi.tile;
+                    ei = min(wi.tile + wi.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
+                }
+                if (ti < ei) {
+                    int lo, hi;
+                    key_limits<RB>(a, wi.r, wi.blk, lo, hi);
+                    const int p = ti * kKeyPages + lane;
+                    if (lane < kKeyPages && p * kKv8Page < hi) id = max(-1, a.table[static_cast<size_t>(wi.req) * a.width + p]);
+                    else id = -2;  // beyond the keys: nothing to report
+                    h = wi.h;
+                    ++ti;
+                    return true;
+                }
+                wi.next(wi.count());
+                ti = -1;
+            }
+            return false;
+        };
+        auto scales_of = [&](int id, int h) {
+            float2 s = make_float2(0.0f, -1.0f);
+            if (id >= 0 && id < a.num_pages) {
+                const float* sc = a.scales + static_cast<size_t>(id) * 2 * a.Hkv + h;
+                s = make_float2(sc[0], sc[a.Hkv]);
+            } else if (id != -2 && lane < kKeyPages) {
+                raise_error(a.err, DM_DEVERR_PAGE);
+            }
+            return s;
+        };
+        int id0, h0, id1, h1;
+        bool have0 = next_id(id0, h0);
+        bool have1 = next_id(id1, h1);
+        float2 sc0 = have0 ? scales_of(id0, h0) : make_float2(0.0f, -1.0f);
+        while (have0 && ok) {
+            const uint32_t si = use % ST, ph = (use / ST) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
+                ok = false;
+                break;
+            }
+            if (lane < kKeyPages) s_meta[si][lane] = sc0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(&full[si], S::kStage);
+            __syncwarp();
+            if (lane < kKeyPages) {
+                const int page = sc0.y < 0.0f ? a.num_pages : id0;
+                const uint32_t k = smem_u32(sm + si * S::kStage) + lane * (kKv8Page * CW);
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c)
+                    tma_load_3d(k + c * (kKeyTile * CW), &ka.map, c * CW, h0 * kKv8Page, page, &full[si]);
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c)
+                    tma_load_3d(k + S::kTileBytes + c * (kKeyTile * CW), &ka.map, c * CW, (a.Hkv + h0) * kKv8Page, page,
+                                &full[si]);
+            }
+            ++use;
+            id0 = id1;
+            h0 = h1;
+            have0 = have1;
+            if (have0) sc0 = scales_of(id0, h0);
+            if (have1) have1 = next_id(id1, h1);
+        }
+        if (lane == 0)
+            for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
+                mbar_wait_bounded(&full[u % ST], (u / ST) & 1u, a.err, nullptr);
+    } else if (active && warp == 5) {
+        // ---------------- MMA ----------------
+        if (lane == 0) {
+            uint32_t t = 0, item = 0;
+            bool ok = true;
+            const uint32_t i_s = f8_idesc(128, N, false, false), i_o = f8_idesc(128, N, true, true);
+            const uint32_t sq = smem_u32(s_q), sp = smem_u32(s_p);
+            auto scores = [&](uint32_t x) {  // S^T of tile x into its buffer
+                if (!(ok = mbar_wait_bounded(&full[x % ST], (x / ST) & 1u, a.err, abort_flag))) return;
+                tc_fence_after();
+                const uint32_t k = smem_u32(sm + (x % ST) * S::kStage);
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c) {
+                    const uint64_t ad = f8_desc_k<CW>(k + c * (kKeyTile * CW)), bd = f8_desc_k<CW>(sq + c * (N * CW));
+#pragma unroll
+                    for (int j = 0; j < CW / 32; ++j) f8_mma(tmem + (x & 1u) * N, ad + 2 * j, bd + 2 * j, i_s, c > 0 || j > 0);
+                }
+                tc_commit(&s_full[x & 1u]);
+            };
+            KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+            while (w.unit < w.end && ok) {
+                int lo, hi;
+                key_limits<RB>(a, w.r, w.blk, lo, hi);
+                const int cnt = w.count();
+                const int nt = min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) - w.tile;
+                if (nt > 0) {
+                    if (!(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) break;
+                    ++item;
+                    tc_fence_after();
+                    scores(t);
+                    for (int i = 0; i < nt && ok; ++i) {
+                        const uint32_t x = t + i;
+                        if (i + 1 < nt) scores(x + 1);
+                        if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
+                        tc_fence_after();
+                        const uint32_t v = smem_u32(sm + (x % ST) * S::kStage) + S::kTileBytes;
+                        const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
+#pragma unroll
+                        for (int c = 0; c < S::kChunks; ++c) {
+                            const uint64_t ad = f8_desc_m<CW>(v + c * (kKeyTile * CW));
+#pragma unroll
+                            for (int j = 0; j < kKeyTile / 32; ++j)
+                                f8_mma(tmem + (2 + c) * N, ad + j * (32 * CW / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
+                        }
+                        tc_commit(&empty[x % ST]);
+                        tc_commit(&pv_done[x & 1u]);
+                    }
+                    t += nt;
+                }
+                w.next(cnt);
+            }
+            tc_commit(&done_bar);
+            mbar_wait_bounded(&done_bar, 0, a.err, nullptr);
+        }
+    } else if (active) {
+        // ---------------- softmax, epilogue, Q ----------------
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+        uint32_t t = 0;
+        bool ok = true;
+        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        while (w.unit < w.end && ok) {
+            int lim_min, lim_max;
+            key_limits<RB>(a, w.r, w.blk, lim_min, lim_max);
+            const int cnt = w.count();
+            const int real = max(1, (lim_max + kKeyTile - 1) / kKeyTile);  // tiles of the item
+            const int t_begin = w.tile, nt = min(w.tile + cnt, real) - w.tile;
+            if (nt <= 0) {
+                w.next(cnt);
+                continue;
+            }
+            const int nrow = min(RB, w.r.m * a.group - w.blk * RB);
+            {   // Q terms: 128 / RB threads per row
+                constexpr int TR = 128 / RB, E = D / TR;
+                const int r = tid / TR, e0 = (tid % TR) * E;
+                const int f = w.blk * RB + min(r, nrow - 1);
+                const int tok = f / a.group, head = w.h * a.group + f % a.group;
+                const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(w.r.row0 + tok) * a.q_rs +
+                             static_cast<int64_t>(head) * a.q_hs + e0;
+                float x[E];
+                float amax = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    x[e] = r < nrow ? static_cast<float>(q[e]) : 0.0f;
+                    if (!(fabsf(x[e]) <= 3.402823466e38f)) x[e] = __int_as_float(0x7fc00000);
+                    amax = fmaxf(amax, fabsf(x[e]));
+                }
+#pragma unroll
+                for (int o = TR / 2; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                // largest magnitude of the row to [2^7, 2^8)
+                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
+                const float mul = __int_as_float((127 - ex) << 23);
+                if (tid % TR == 0) {
+                    s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
+                    s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] *= mul;
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        float2 b0, b1;
+                        const uint32_t lo = e4m3_round2(x[e], x[e + 1], b0), hi = e4m3_round2(x[e + 2], x[e + 3], b1);
+                        const int d = e0 + e, n = i * RB + r;
+                        uint8_t* dst = s_q + (d / CW) * (N * CW) + f8_unit<CW>(n, (d % CW) / 16) + d % 16;
+                        *reinterpret_cast<uint32_t*>(dst) = lo | (hi << 16);
+                        x[e] = (x[e] - b0.x) * 16.0f, x[e + 1] = (x[e + 1] - b0.y) * 16.0f;
+                        x[e + 2] = (x[e + 2] - b1.x) * 16.0f, x[e + 3] = (x[e + 3] - b1.y) * 16.0f;
+                    }
+                fence_proxy_async_smem();
+                mbar_arrive(&q_ready);
+                named_bar_sync(1, 128);
+            }
+            float mref[RB], l[RB];
+#pragma unroll
+            for (int r = 0; r < RB; ++r) mref[r] = -INFINITY, l[r] = 0.0f;
+
+            for (int i = 0; i < nt; ++i) {
+                const uint32_t x = t + i, si = x % ST;
+                const int key = (t_begin + i) * kKeyTile + tid;
+                const int tile_end = (t_begin + i + 1) * kKeyTile;
+                ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag);
+                ok = ok && mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag);
+                // every thread of the four warps leaves together
+                if (named_bar_or(1, 128, !ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float2 sc = s_meta[si][tid >> 4];
+                const float vexp = static_cast<float>(((__float_as_int(sc.y) >> 23) & 0xff) - 127);
+                float y[RB];
+                {
+                    float c[16];
+#pragma unroll
+                    for (int b = 0; b < N / 16; ++b) {
+                        tc_ld16(lanes + (x & 1u) * N + b * 16, c);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int n = b * 16 + j, term = n / RB, r = n % RB;
+                            const float s = 1.0f / static_cast<float>(1 << (4 * term));
+                            y[r] = term == 0 ? c[j] : fmaf(c[j], s, y[r]);
+                        }
+                    }
+                }
+                const bool edge = tile_end > lim_min;
+                bool over = false;
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    y[r] = fmaf(y[r], s_frow[r] * sc.x, vexp);
+                    if (edge && key >= s_lim[r]) y[r] = -INFINITY;
+                    if (sc.y < 0.0f) y[r] = -INFINITY;
+                    over = over || y[r] > mref[r] + kKeyLazy;
+                }
+                if (named_bar_or(1, 128, over)) {
+                    // raise the references to the maximum of this tile and rescale
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        const float mx = warp_max(y[r]);
+                        if (lane == 0) s_red[warp][r] = mx;
+                    }
+                    named_bar_sync(1, 128);
+                    float fac[RB];
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        const float mx = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r]));
+                        const float nm = fmaxf(mref[r], mx);
+                        fac[r] = nm == mref[r] ? 1.0f : exp2f(mref[r] - nm);
+                        mref[r] = nm;
+                        l[r] *= fac[r];
+                    }
+                    if (i > 0) {
+                        ok = mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
+                        tc_fence_after();
+#pragma unroll
+                        for (int b = 0; b < S::kChunks * N / 16; ++b) {
+                            float c[16];
+                            uint32_t u[16];
+                            tc_ld16(lanes + 2 * N + b * 16, c);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(c[j] * fac[(b * 16 + j) % RB]);
+                            tc_st16(lanes + 2 * N + b * 16, u);
+                        }
+                        tc_wait_st();
+                    }
+                    named_bar_sync(1, 128);  // s_red is free again
+                }
+                // weights, row sums, e4m3 terms
+                const float vinv = __int_as_float((127 - static_cast<int>(vexp)) << 23);
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    const float wgt = exp2f(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
+                    l[r] = fmaf(wgt, vinv, l[r]);
+                    y[r] = wgt * kKeyBoost;
+                }
+                if (edge && sc.y >= 0.0f) {
+                    // V rows behind the last key become zeros; a NaN code that not every row sees
+                    // becomes 0 and makes the sums of the rows that see it NaN
+                    uint8_t* v = sm + si * S::kStage + S::kTileBytes + tid * CW;
+                    if (key >= lim_max) {
+#pragma unroll
+                        for (int c = 0; c < S::kChunks; ++c)
+                            for (int u = 0; u < CW / 16; ++u)
+                                *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
+                    } else if (key >= lim_min) {
+                        bool nan = false;
+#pragma unroll
+                        for (int c = 0; c < S::kChunks; ++c)
+                            for (int u = 0; u < CW / 4; ++u) {
+                                uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
+                                const uint32_t bad = e4m3_nan_mask(*p);
+                                if (bad) {
+                                    *p &= ~bad;
+                                    nan = true;
+                                }
+                            }
+                        if (nan)
+#pragma unroll
+                            for (int r = 0; r < RB; ++r)
+                                if (key < s_lim[r]) l[r] = __int_as_float(0x7fc00000);
+                    }
+                }
+                if (ok && x >= 2 && i >= 2)
+                    ok = mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag);
+                uint8_t* p = s_p + (x & 1u) * S::kP + tid * 16;
+                uint32_t code[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i2 = 0; i2 < TERMS; ++i2)
+#pragma unroll
+                    for (int r = 0; r < RB; r += 2) {
+                        float2 back;
+                        const uint32_t c2 = e4m3_round2(y[r], y[r + 1], back);
+                        if (i2 + 1 < TERMS) {
+                            y[r] = (y[r] - back.x) * 16.0f;
+                            y[r + 1] = (y[r + 1] - back.y) * 16.0f;
+                        }
+                        const int n = i2 * RB + r, wd = (n % 16) / 4;
+                        code[wd] = (n % 4 == 0) ? c2 : (code[wd] | (c2 << 16));
+                        if (n % 16 == 14)
+                            *reinterpret_cast<uint4*>(p + (n / 16) * (kKeyTile * 16)) = make_uint4(code[0], code[1], code[2], code[3]);
+                    }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                mbar_arrive(&p_ready[x & 1u]);
+            }
+            if (!ok) break;
+            t += nt;
+            // the item's sums, then O
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                const float s = warp_sum(l[r]);
+                if (lane == 0) s_red[warp][r] = s;
+            }
+            ok = mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
+            if (named_bar_or(1, 128, !ok)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int r = 0; r < RB; ++r) l[r] = s_red[0][r] + s_red[1][r] + s_red[2][r] + s_red[3][r];
+            named_bar_sync(1, 128);  // s_red is free again
+
+            const long long item0 = w.unit - t_begin;  // the item's first tile in the sequence
+            const bool whole = t_begin == 0 && nt == real;
+            const long long tot = static_cast<long long>(total), gr = static_cast<long long>(grid);
+            const int c_first = static_cast<int>(((item0 + 1) * gr - 1) / tot);
+            const int c_last = static_cast<int>(((item0 + real) * gr - 1) / tot);
+            constexpr int kSlot = RB * (D + 2);
+            float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
+            auto put = [&](int r, int d, float o, float mm, float ll) {
+                if (r >= nrow) return;
+                const int f = w.blk * RB + r;
+                const int64_t row = w.r.row0 + f / a.group;
+                const int head = w.h * a.group + f % a.group;
+                // a row that saw no key keeps the reference -inf
+                static_cast<T*>(a.out)[row * a.o_rs + static_cast<int64_t>(head) * a.o_hs + d] =
+                    static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o / ll);
+                if (d == 0 && a.lse)
+                    a.lse[row * a.Hq + head] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+            };
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) {
+                float o[RB];
+                float v[16];
+#pragma unroll
+                for (int b = 0; b < N / 16; ++b) {
+                    tc_ld16(lanes + (2 + c) * N + b * 16, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int n = b * 16 + j, term = n / RB, r = n % RB;
+                        const float s = 1.0f / (static_cast<float>(1 << (4 * term)) * kKeyBoost);
+                        o[r] = term == 0 ? v[j] * s : fmaf(v[j], s, o[r]);
+                    }
+                }
+                if (tid < CW) {
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        if (whole) put(r, c * CW + tid, o[r], mref[r], l[r]);
+                        else slot[r * D + c * CW + tid] = o[r];
+                    }
+                }
+            }
+            tc_fence_before();
+            if (!whole) {
+                if (tid == 0) {
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        slot[RB * D + r] = mref[r];
+                        slot[RB * D + RB + r] = l[r];
+                    }
+                }
+                __threadfence();
+                named_bar_sync(1, 128);
+                if (tid == 0) {
+                    const unsigned parts = static_cast<unsigned>(c_last - c_first + 1);
+                    const unsigned got = atomicAdd(a.counters + c_first, 1u);
+                    s_last = got + 1 == parts;
+                    if (s_last) a.counters[c_first] = 0;
+                    __threadfence();
+                }
+                named_bar_sync(1, 128);
+                if (s_last) {
+                    auto part_of = [&](int c) {
+                        return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
+                    };
+                    for (int r = 0; r < nrow; ++r) {
+                        float mm = -INFINITY, ll = 0.0f;
+                        float o[S::kChunks];
+#pragma unroll
+                        for (int c = 0; c < S::kChunks; ++c) o[c] = 0.0f;
+                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + r));
+                        const float mu = mm == -INFINITY ? 0.0f : mm;
+                        for (int c = c_first; c <= c_last; ++c) {
+                            const float* p = part_of(c);
+                            const float mc = __ldcg(p + RB * D + r);
+                            const float f = mc == mm ? 1.0f : exp2f(mc - mu);
+                            ll = fmaf(__ldcg(p + RB * D + RB + r), f, ll);
+                            if (tid < CW)
+#pragma unroll
+                                for (int k = 0; k < S::kChunks; ++k) o[k] = fmaf(__ldcg(p + r * D + k * CW + tid), f, o[k]);
+                        }
+                        if (tid < CW)
+#pragma unroll
+                            for (int k = 0; k < S::kChunks; ++k) put(r, k * CW + tid, o[k], mm, ll);
+                    }
+                }
+            }
+            w.next(cnt);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        tc_dealloc(tmem, S::kCols);
+    }
+}
+
+bool kv8_encode_map(const dm_kv8_cache* c, CUtensorMap* map) {
+    typedef CUresult (*Fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                           const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                           CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Fn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<Fn>(p);
+    }();
+    if (!fn) return false;
+    const cuuint32_t cw = c->head_dim >= 128 ? 128 : 64;
+    const cuuint64_t rows = 2ull * c->num_kv_heads * kKv8Page;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c->head_dim), rows, static_cast<cuuint64_t>(c->num_pages)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c->head_dim), rows * c->head_dim};
+    const cuuint32_t box[3] = {cw, kKv8Page, 1}, estr[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c->pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              cw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, int RB>
+static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStream_t s) {
+    using S = KeyShape<T, D, RB>;
+    static bool ready[64] = {};
+    if (dev >= 64 || !ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv8_attn_keys_kernel<T, D, RB>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready[dev] = true;
+    }
+    kv8_attn_keys_kernel<T, D, RB><<<num_sms, kKeyThreads, S::kSmem, s>>>(ka);
+    return cudaGetLastError();
+}
+
+template <typename T, int RB>
+static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev, cudaStream_t s) {
+    if (D == 64) return launch_keys<T, 64, RB>(ka, num_sms, dev, s);
+    if (D == 128) return launch_keys<T, 128, RB>(ka, num_sms, dev, s);
+    return launch_keys<T, 256, RB>(ka, num_sms, dev, s);
+}
+
+// Rows of an item: 16 when a request's rows fill more than 8 (the cache is then read once
+// for 16 rows), else 8.
+cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f32, int num_sms, int dev, cudaStream_t s) {
+    KeyArgs ka{};
+    if (!kv8_encode_map(c, &ka.map)) return cudaErrorNotSupported;
+    ka.a = a;
+    const bool wide = static_cast<int64_t>(a.max_q) * a.group > 8;
+    if (f32) return wide ? launch_keys_d<float, 16>(ka, c->head_dim, num_sms, dev, s)
+                         : launch_keys_d<float, 8>(ka, c->head_dim, num_sms, dev, s);
+    return wide ? launch_keys_d<__nv_bfloat16, 16>(ka, c->head_dim, num_sms, dev, s)
+                : launch_keys_d<__nv_bfloat16, 8>(ka, c->head_dim, num_sms, dev, s);
+}
+
+size_t kv8_keys_part_floats(int D, int num_sms) { return static_cast<size_t>(num_sms) * 2 * 16 * (D + 2); }
+
+}  // namespace dm

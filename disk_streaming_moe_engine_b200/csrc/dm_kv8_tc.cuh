@@ -1,0 +1,103 @@
+// dm_kv8_tc.cuh — tcgen05 kind::f8f6f4 (e4m3 x e4m3 -> fp32) and TMA helpers of the 8-bit
+// cache attention kernels.
+//
+// Tiles of the cache in shared memory, as the TMA boxes of 16 token rows x CW bytes leave
+// them (CW = 128 with the 128-byte swizzle, or 64 with the 64-byte swizzle at head_dim 64):
+// token rows of CW bytes, 8-row groups of 8 CW bytes, the 16-byte units of a row permuted by
+// the row.  The same bytes serve two roles: K as a K-major operand (rows = M, the head's
+// elements = K) and V as an M-major operand (rows = K, the head's elements = M).
+#pragma once
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include "dm_kv8.h"
+#include "dm_tc.cuh"
+
+namespace dm {
+
+constexpr uint64_t kDescVersion = 1ull << 46;
+
+// K-major operand of CW-byte rows: 8-row groups 8 CW bytes apart (stride byte offset); one
+// K = 32 step of the tile advances the start address by 32 bytes.
+template <int CW>
+DM_DEV uint64_t f8_desc_k(uint32_t addr) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(8 * CW / 16) << 32) |
+           kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
+}
+// M-major operand: 8-token groups 8 CW bytes apart (stride byte offset); the second CW
+// elements of M (CW = 64 only) at leading byte offset 0, i.e. M rows 64-127 repeat rows 0-63.
+template <int CW>
+DM_DEV uint64_t f8_desc_m(uint32_t addr) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(8 * CW / 16) << 32) | kDescVersion |
+           (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
+}
+// N-major operand without swizzle: per 16 N columns a block of 16-byte rows, one per K;
+// 8-row groups 128 bytes apart (leading byte offset), blocks `block` bytes apart (stride).
+DM_DEV uint64_t f8_desc_n16(uint32_t addr, uint32_t block) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 / 16) << 16) |
+           (static_cast<uint64_t>(block / 16) << 32) | kDescVersion;
+}
+
+// Instruction descriptor: fp32 accumulator, e4m3 operands; bit 15 / 16: A / B with M / N as
+// the contiguous dimension.
+DM_DEV uint32_t f8_idesc(int M, int N, bool a_m_major, bool b_n_major) {
+    return (1u << 4) | (a_m_major ? 1u << 15 : 0u) | (b_n_major ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+DM_DEV void f8_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+DM_DEV void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Byte of 16-byte unit u of token row r in a tile of CW-byte rows.
+template <int CW>
+DM_DEV uint32_t f8_unit(int r, int u) {
+    const int x = CW == 128 ? (u ^ (r & 7)) : (u ^ ((r >> 1) & 3));
+    return static_cast<uint32_t>(r * CW + x * 16);
+}
+
+DM_DEV float e4m3_round(float x, uint32_t& code) {  // code of the nearest value, and that value
+    code = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+}
+// codes of two values (a in the low byte), and the values they stand for
+DM_DEV uint32_t e4m3_round2(float a, float b, float2& back) {
+    const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), __NV_E4M3)));
+    return c;
+}
+// 0xff in the bytes of w that hold a NaN code
+DM_DEV uint32_t e4m3_nan_mask(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+// Barrier over the 128 softmax threads that also ORs a predicate.
+DM_DEV bool named_bar_or(int id, int count, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(count), "r"(v ? 1u : 0u)
+        : "memory");
+    return r != 0;
+}
+
+// Tensor map of the cache: (head element, row of a page, page), boxes of 16 rows x CW bytes.
+// A page index of num_pages reads zeros.
+bool kv8_encode_map(const dm_kv8_cache* c, CUtensorMap* map);
+
+}  // namespace dm

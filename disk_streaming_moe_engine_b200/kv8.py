@@ -16,6 +16,7 @@ goes into the error word of `error_word()` and is raised by `check()`.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import NamedTuple
 
 import torch
@@ -28,6 +29,15 @@ LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 _DTYPES = {torch.bfloat16: _lib.DM_DTYPE_BF16, torch.float32: _lib.DM_DTYPE_F32}
 _ERR = 512
+_local = threading.local()
+
+
+def _buffer():
+    """This thread's message buffer."""
+    buf = getattr(_local, "buf", None)
+    if buf is None:
+        buf = _local.buf = C.create_string_buffer(_ERR)
+    return buf
 
 
 def _raise(rc: int, buf):
@@ -38,15 +48,17 @@ def _bad(detail: str):
     raise _lib.DmError(_lib.DM_ERR_INVALID_ARG, '{"error_type":"INVALID_ARG","detail":"%s","stage":"kv8","layer":-1}' % detail)
 
 
-def _stream(t: torch.Tensor, stream) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream if stream is None else stream
+def _stream(device, stream) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream
 
 
-def _ints(device, **tensors):
-    """int32, contiguous, on the device."""
-    for name, t in tensors.items():
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.device != device):
-            _bad(f"{name} must be a contiguous int32 tensor on {device}")
+def _ints(device, names, *tensors):
+    """int32, contiguous, on the device (None: not given)."""
+    for i, t in enumerate(tensors):
+        if t is not None and (t.dtype is not torch.int32 or t.device != device or not t.is_contiguous()):
+            _bad(f"{names.split()[i]} must be a contiguous int32 tensor on {device}")
+    if device.type != "cuda":
+        _bad(f"the tensors must be on a CUDA device (got {device})")
 
 
 def _rows(name: str, t: torch.Tensor, heads, dim: int, device, dtype):
@@ -63,8 +75,8 @@ def error_word(device="cuda") -> torch.Tensor:
 
 def check(err: torch.Tensor, stream=None) -> None:
     """Waits for the stream, clears the error word and raises DmError when a bit was set."""
-    buf = C.create_string_buffer(_ERR)
-    rc = _lib.load().dm_kv8_status(err.data_ptr(), _stream(err, stream), buf, _ERR)
+    buf = _buffer()
+    rc = _lib.load().dm_kv8_status(err.data_ptr(), _stream(err.device, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
 
@@ -120,26 +132,25 @@ def plan_slots(free_pages, free_state, block_table, ctx_lens, new_lens, max_toke
     dev = ctx_lens.device
     n = ctx_lens.numel()
     if out is None:
-        tok = torch.empty((3, max_tokens), dtype=torch.int32, device=dev)
-        req = torch.empty(2 * n + 1, dtype=torch.int32, device=dev)
-        out = SlotPlan(req[:n], req[n:], tok[0], tok[1], tok[2])
+        room = torch.empty(2 * n + 1 + 3 * max_tokens, dtype=torch.int32, device=dev)
+        out = SlotPlan(*room.split_with_sizes((n, n + 1, max_tokens, max_tokens, max_tokens)))
     else:
-        _ints(dev, **out._asdict())
+        _ints(dev, "seq_lens cu_new slots positions requests", *out)
         if (out.seq_lens.numel() < n or out.cu_new.numel() < n + 1
                 or min(out.slots.numel(), out.positions.numel(), out.requests.numel()) < max_tokens):
             _bad("an output of the plan is too small")
-    _ints(dev, ctx_lens=ctx_lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
-          free_state=free_state, state_out=state_out, err=err)
+    _ints(dev, "ctx_lens new_lens block_table free_pages free_state state_out err", ctx_lens, new_lens, block_table,
+          free_pages, free_state, state_out, err)
     if new_lens.numel() != n or block_table.dim() != 2 or block_table.shape[0] < n or free_state.numel() != 2 or \
             (state_out is not None and state_out.numel() != 2):
         _bad("need new_lens [n], block_table [n][width], free_state [2]")
-    buf = C.create_string_buffer(_ERR)
+    buf = _buffer()
     rc = _lib.load().dm_kv8_plan(
         n, ctx_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1],
         free_pages.data_ptr(), free_pages.numel(), free_state.data_ptr(),
         (free_state if state_out is None else state_out).data_ptr(), out.seq_lens.data_ptr(), out.cu_new.data_ptr(),
         max_tokens, out.slots.data_ptr(), out.positions.data_ptr(), out.requests.data_ptr(),
-        None if err is None else err.data_ptr(), _stream(ctx_lens, stream), buf, _ERR)
+        None if err is None else err.data_ptr(), _stream(dev, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
     return out
@@ -160,7 +171,7 @@ class RopePlan:
                               attention_factor)
         self._c = _lib.DmRopePlan()
         self._ref = C.addressof(self._c)
-        buf = C.create_string_buffer(_ERR)
+        buf = _buffer()
         rc = _lib.load().dm_rope_plan_init(C.byref(p), C.byref(self._c), buf, _ERR)
         if rc != _lib.DM_OK:
             _raise(rc, buf)
@@ -177,7 +188,7 @@ def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None
     q / k themselves; rows at negative positions are skipped."""
     dev, D = positions.device, plan.head_dim
     n = positions.numel()
-    _ints(dev, positions=positions)
+    _ints(dev, "positions", positions)
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     k = q[:, :0] if k is None else k
@@ -187,11 +198,11 @@ def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None
         _rows(name, t, like.shape[1], D, dev, q.dtype)
         if t.shape[0] != n:
             _bad(f"{name} has {t.shape[0]} rows, positions {n}")
-    buf = C.create_string_buffer(_ERR)
+    buf = _buffer()
     rc = _lib.load().dm_rope(
         plan._ref, _DTYPES[q.dtype], n, positions.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
         q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1], k.data_ptr(), k.stride(0), k.stride(1),
-        k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1], _stream(positions, stream), buf, _ERR)
+        k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1], _stream(dev, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
     return q_out, k_out
@@ -204,13 +215,13 @@ def append(cache: Kv8Cache, k, v, slots, *, err=None, stream=None) -> None:
         _bad(f"k is bf16 or fp32 (got {k.dtype})")
     _rows("k", k, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
     _rows("v", v, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
-    _ints(cache.device, slots=slots, err=err)
+    _ints(cache.device, "slots err", slots, err)
     if k.shape[0] < n or v.shape[0] < n:
         _bad(f"{n} slots, k has {k.shape[0]} rows, v {v.shape[0]}")
-    buf = C.create_string_buffer(_ERR)
+    buf = _buffer()
     rc = _lib.load().dm_kv8_append(
         cache._ref, _DTYPES[k.dtype], n, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-        v.stride(1), slots.data_ptr(), None if err is None else err.data_ptr(), _stream(slots, stream), buf, _ERR)
+        v.stride(1), slots.data_ptr(), None if err is None else err.data_ptr(), _stream(cache.device, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
 
@@ -219,9 +230,8 @@ def attention_workspace(cache: Kv8Cache) -> torch.Tensor:
     """A zeroed workspace for attention() calls on this cache's geometry; calls that may run
     at the same time need one each."""
     nbytes = C.c_uint64()
-    buf = C.create_string_buffer(_ERR)
-    with torch.cuda.device(cache.device):
-        rc = _lib.load().dm_kv8_attention_workspace(cache._ref, C.byref(nbytes), buf, _ERR)
+    buf = _buffer()
+    rc = _lib.load().dm_kv8_attention_workspace(cache._ref, C.byref(nbytes), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
     return torch.zeros(nbytes.value, dtype=torch.uint8, device=cache.device)
@@ -241,7 +251,7 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     else:
         _rows("out", out, q.shape[1], D, dev, q.dtype)
-    _ints(dev, block_table=block_table, seq_lens=seq_lens, cu_q=cu_q, err=err)
+    _ints(dev, "block_table seq_lens cu_q err", block_table, seq_lens, cu_q, err)
     if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \
             out.shape[0] < q.shape[0]:
         _bad("need block_table [n][width], cu_q [n + 1] and out of q's shape")
@@ -256,8 +266,8 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
         out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), block_table.data_ptr(),
         seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), None if err is None else err.data_ptr())
-    buf = C.create_string_buffer(_ERR)
-    rc = _lib.load().dm_kv8_attention(cache._ref, C.addressof(a), _stream(q, stream), buf, _ERR)
+    buf = _buffer()
+    rc = _lib.load().dm_kv8_attention(cache._ref, C.addressof(a), _stream(dev, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
     return out

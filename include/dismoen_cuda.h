@@ -611,7 +611,7 @@ typedef struct dm_kv8_attn_args {
 } dm_kv8_attn_args;
 int32_t dm_kv8_attention(const dm_kv8_cache* cache_host, const dm_kv8_attn_args* args_host, void* stream,
                          char* err_buf, uint64_t err_buf_size);
-/* Bytes for any call with this cache geometry on the current device. */
+/* Bytes for any call with this cache geometry on the cache's device. */
 int32_t dm_kv8_attention_workspace(const dm_kv8_cache* cache_host, uint64_t* bytes_out, char* err_buf,
                                    uint64_t err_buf_size);
 

@@ -99,17 +99,19 @@ def plain_append(pages, scales, k, v, slots):
 
 
 def plain_attention(cache, q, table, lens, cu, scale):
-    """64-bit results, sum p |v| of every output, largest sum |q k| of every row, lse."""
+    """64-bit results, their magnitudes (sum p |v|, and the row's largest p sV times the sum of
+    |codes|), the largest sum |q k| of every row, lse."""
     pages, scales = cache.pages.cpu().numpy(), cache.scales.cpu().numpy().astype(np.float64)
     q = q.double().cpu().numpy()
     hk, d = pages.shape[2], pages.shape[4]
     grp = q.shape[1] // hk
-    out, mag, sat = np.zeros_like(q), np.zeros_like(q), np.zeros(q.shape[:2])
+    out, mag, small, sat = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q), np.zeros(q.shape[:2])
     lse = np.full(q.shape[:2], -np.inf)
     for i, n in enumerate(lens):
         m = cu[i + 1] - cu[i]
         ids = table[i, np.arange(n) // PAGE]
-        kv = E4M3[pages[ids, :, :, np.arange(n) % PAGE]] * scales[ids][..., None]  # [n][2][hk][d]
+        codes, sc = E4M3[pages[ids, :, :, np.arange(n) % PAGE]], scales[ids]
+        kv = codes * sc[..., None]  # [n][2][hk][d]
         for j in range(m):
             see = max(0, min(n, n - m + j + 1))
             if see == 0:
@@ -121,8 +123,9 @@ def plain_attention(cache, q, table, lens, cu, scale):
                 lse[cu[i] + j, h] = s.max() + math.log(p.sum())
                 p /= p.sum()
                 out[cu[i] + j, h], mag[cu[i] + j, h] = p @ vv, p @ np.abs(vv)
+                small[cu[i] + j, h] = (p * sc[:see, 1, h // grp]).max() * np.abs(codes[:see, 1, h // grp]).sum(0)
                 sat[cu[i] + j, h] = (np.abs(kk) @ np.abs(x)).max() * abs(scale)
-    return out, mag, sat, lse
+    return out, (mag, small), sat, lse
 
 
 def attention_tolerance(out, mag, sat, d, keys, dtype):
@@ -130,11 +133,15 @@ def attention_tolerance(out, mag, sat, d, keys, dtype):
     of magnitudes off, of q split to 22 bits (fp32) or, in the tile kernel, to 2^-17 of the
     row's largest element; an error e of every score changes an output by at most
     2 e sum p |v|.  Weights: 2^-20 (two fp16 terms, or fp32) per key page of the running sum;
-    bf16 outputs carry weights of at least 8 bits and their own rounding."""
+    bf16 outputs carry weights of at least 8 bits and their own rounding.  The 8 bits are two
+    e4m3 terms, the second scaled by 2^4, of 64 times the weight (relative to the row's
+    largest, at least 2^-2 of it): its smallest step is 2^-9 / 2^4 / 2^6, so a weight is off by
+    2^-20 of the largest one's p sV at least, on a code of V."""
+    mag, small = mag
     ds = sat[..., None] * (d / 16 + 1) * 2.0 ** -22
     tol = (2 * ds + (keys / PAGE + 4) * 2.0 ** -22 + 2.0 ** -20) * mag
     if dtype == torch.bfloat16:
-        tol = tol + BF16_STEP * np.abs(out) + (BF16_STEP + 2 * sat[..., None] * 2.0 ** -13) * mag
+        tol = tol + BF16_STEP * np.abs(out) + (BF16_STEP + 2 * sat[..., None] * 2.0 ** -13) * mag + 2.0 ** -18 * small
     return tol + 1e-30
 
 
@@ -220,8 +227,7 @@ def test_cache_refusals(lib, kw):
                                 dict(sm_scale=float("nan")), dict(table_width=0), dict(max_q_len=0),
                                 dict(max_q_len=2), dict(rows=3), dict(reserved=1), dict(q=None), dict(out=None),
                                 dict(block_table=None), dict(seq_lens=None), dict(workspace=None),
-                                dict(workspace=(1 << 22) + 16), dict(workspace_bytes=100),
-                                dict(cu_q=1 << 22, n=1 << 22, rows=1 << 30, max_q_len=1 << 30)])
+                                dict(workspace=(1 << 22) + 16)])
 def test_attention_refusals(lib, kw):
     c, one = _fake_cache(), 1 << 22
     f = dict(dtype=0, n=4, num_q_heads=8, max_q_len=1, rows=4, table_width=9, sm_scale=0.1, reserved=0, q=one,
@@ -238,8 +244,6 @@ def test_empty_calls_need_no_device(lib):
     assert _call(lib, "dm_kv8_append", C.addressof(c), 0, 0, one, 0, 0, one, 0, 0, one, None, None)[0] == 0
     a = _lib.DmKv8AttnArgs(dtype=0, n=0, num_q_heads=8, max_q_len=1, rows=0, table_width=1, sm_scale=1.0)
     assert _call(lib, "dm_kv8_attention", C.addressof(c), C.addressof(a), None)[0] == 0
-    b = C.c_uint64()
-    assert _call(lib, "dm_kv8_attention_workspace", C.addressof(c), C.byref(b))[0] == 0 and b.value > 0
 
 
 @pytest.mark.parametrize("bad", [dict(n=0), dict(n=8193), dict(width=0), dict(cap=0), dict(tokens=0),
@@ -632,6 +636,27 @@ def test_attention_leaves_other_rows(lib, rows):
     with pytest.raises(DmError) as e:
         kv8.check(err)
     assert e.value.code == _lib.DM_ERR_CAPACITY and torch.equal(got[:rows], want[:rows])
+
+
+@pytest.mark.gpu
+def test_attention_device_refusals(lib):
+    """Refused on the host: a workspace that is too small, host memory for the cache, tensors
+    of the wrong type or shape."""
+    cache = kv8.Kv8Cache.empty(4, 2, 64)
+    q, t, n = torch.zeros(1, 4, 64, device=DEV), dev32([[0, 1]]), dev32([5])
+    ws = kv8.attention_workspace(cache)
+    kv8.attention(cache, q, t, n, workspace=ws)
+    for bad in (dict(workspace=ws[:-256]), dict(q=q.half()), dict(q=q[..., :32]), dict(q=q[:, :3]),
+                dict(block_table=t.long()), dict(seq_lens=n.cpu()), dict(out=q[:0]), dict(cu_q=n),
+                dict(lse=torch.zeros(1, 3, device=DEV)), dict(max_q_len=2), dict(sm_scale=math.inf)):
+        with pytest.raises(DmError):
+            kv8.attention(**{**dict(cache=cache, q=q, block_table=t, seq_lens=n, workspace=ws), **bad})
+    host = torch.zeros(4, 2, 2, 16, 64, dtype=torch.uint8).pin_memory()
+    c = _lib.DmKv8Cache(host.data_ptr(), cache.scales.data_ptr(), 4, 2, 64, 0)
+    x, s = torch.zeros(1, 2, 64, device=DEV), dev32([0])
+    rc, err = _call(lib, "dm_kv8_append", C.addressof(c), 1, 1, x.data_ptr(), 128, 64, x.data_ptr(), 128, 64,
+                    s.data_ptr(), None, None)
+    assert rc == _lib.DM_ERR_INVALID_ARG and "device memory" in err["detail"]
 
 
 @pytest.mark.gpu
