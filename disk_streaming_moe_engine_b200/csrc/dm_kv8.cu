@@ -275,120 +275,141 @@ struct RopeArgs {
     int64_t x_rs[2], x_hs[2], y_rs[2], y_hs[2];
     int heads[2];
     const int* positions;
-    int n, inplace[2];
+    int n, tok, inplace[2];
 };
 
-constexpr int kRopeTok = 8;  // tokens of a CTA
+constexpr int kRopeTok = 8;    // tokens of a CTA at most
+constexpr int kRopeBatch = 4;  // tokens whose loads a thread has in flight
 
+// 16 bytes (VEC elements) or one element (VEC = 1) as loaded, and as floats
 template <typename T, int VEC>
 struct RopeVec {
-    float v[VEC];
+    uint4 u;
     DM_DEV void load(const T* p) {
-        if constexpr (VEC == 1) {
-            v[0] = static_cast<float>(p[0]);
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            if constexpr (sizeof(T) == 4) {
+        if constexpr (VEC == 1) u.x = __float_as_uint(static_cast<float>(p[0]));
+        else u = *reinterpret_cast<const uint4*>(p);
+    }
+    DM_DEV void unpack(float (&v)[VEC]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+        for (int i = 0; i < (VEC == 1 ? 1 : 4); ++i) {
+            if constexpr (VEC != 8) {
+                v[i] = __uint_as_float(w[i]);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = bf16lo(w[i]);
-                    v[2 * i + 1] = bf16hi(w[i]);
-                }
+                v[2 * i] = bf16lo(w[i]);
+                v[2 * i + 1] = bf16hi(w[i]);
             }
         }
     }
     DM_DEV void store(T* p) const {
-        if constexpr (VEC == 1) {
-            p[0] = static_cast<T>(v[0]);
-        } else {
+        if constexpr (VEC == 1) p[0] = static_cast<T>(__uint_as_float(u.x));
+        else *reinterpret_cast<uint4*>(p) = u;
+    }
+    DM_DEV void pack(const float (&v)[VEC]) {
+        if constexpr (VEC == 8) {
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    w[i] = __float_as_uint(v[i]);
-                } else {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&b);
-                }
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&b);
             }
-            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            u = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            u.x = __float_as_uint(v[0]);
+            if constexpr (VEC == 4)
+                u.y = __float_as_uint(v[1]), u.z = __float_as_uint(v[2]), u.w = __float_as_uint(v[3]);
         }
     }
 };
 
 // VEC elements per access (16 bytes, or 1 when a pointer or stride is not a multiple of 16
 // bytes).  A unit of a head is VEC pairs (half layout: two accesses; interleaved: two
-// neighbouring ones, or one pair when VEC = 1) or VEC elements that pass through.
+// neighbouring ones, or one pair when VEC = 1) or VEC elements that pass through; a thread
+// keeps its unit over the CTA's tokens, and its first batch of loads is in flight while the
+// CTA computes the angles.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeArgs a) {
     __shared__ float2 cs[kRopeTok][128];
     __shared__ int s_pos[kRopeTok];
-    const int t0 = blockIdx.x * kRopeTok, nt = min(kRopeTok, a.n - t0);
+    const int t0 = blockIdx.x * a.tok, nt = min(a.tok, a.n - t0);
     const int rot = a.plan.rotary_dim, half = rot / 2, D = a.plan.head_dim;
-    for (int i = threadIdx.x; i < nt; i += blockDim.x) s_pos[i] = a.positions[t0 + i];
-    for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
-        const int t = i / half, j = i - t * half;
-        const double ang = static_cast<double>(a.positions[t0 + t]) * a.plan.freq[j];
-        const double red = fma(-rint(ang * 0.15915494309189535), 6.283185307179586, ang);
-        const float hi = static_cast<float>(red), lo = static_cast<float>(red - static_cast<double>(hi));
-        float s, c;
-        sincosf(hi, &s, &c);
-        cs[t][j] = make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
-    }
-    __syncthreads();
-    const int pu = half / VEC, upass = (D - rot) / VEC, units = pu + upass;
+    const bool inter = a.plan.layout == DM_ROPE_INTERLEAVED;
+    const int pu = half / VEC, units = pu + (D - rot) / VEC;
     const int total = (a.heads[0] + a.heads[1]) * units;
-    for (int u = threadIdx.x; u < total; u += blockDim.x) {
-        int h = u / units;
+    bool ready = false;
+    for (int base = 0; base < total; base += blockDim.x) {
+        const int u = base + threadIdx.x;
+        const bool live = u < total;
+        int h = live ? u / units : 0;
         const int unit = u - h * units;
         const int w = h >= a.heads[0];
         if (w) h -= a.heads[0];
         const T* x = static_cast<const T*>(a.x[w]) + static_cast<int64_t>(t0) * a.x_rs[w] + h * a.x_hs[w];
         T* y = static_cast<T*>(a.y[w]) + static_cast<int64_t>(t0) * a.y_rs[w] + h * a.y_hs[w];
-        if (unit >= pu) {
-            if (a.inplace[w]) continue;
-            const int e = rot + (unit - pu) * VEC;
-            for (int t = 0; t < nt; ++t) {
-                if (s_pos[t] < 0) continue;
-                RopeVec<T, VEC> r;
-                r.load(x + t * a.x_rs[w] + e);
-                r.store(y + t * a.y_rs[w] + e);
-            }
-            continue;
-        }
+        const bool turn = unit < pu;
+        const bool work = live && (turn || !a.inplace[w]);
         const int j0 = unit * VEC;
-        const bool inter = a.plan.layout == DM_ROPE_INTERLEAVED;
-        const int e0 = inter ? 2 * j0 : j0, e1 = inter ? 2 * j0 + VEC : j0 + half;
-        for (int t = 0; t < nt; ++t) {
-            if (s_pos[t] < 0) continue;
-            RopeVec<T, VEC> r0, r1;
-            r0.load(x + t * a.x_rs[w] + e0);
-            r1.load(x + t * a.x_rs[w] + e1);
-            if (!inter || VEC == 1) {
+        const int e0 = !turn ? rot + (unit - pu) * VEC : inter ? 2 * j0 : j0, e1 = inter ? 2 * j0 + VEC : j0 + half;
+        for (int tb = 0; tb < nt; tb += kRopeBatch) {
+            RopeVec<T, VEC> r0[kRopeBatch], r1[kRopeBatch];
+            if (work) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float2 f = cs[t][j0 + i];
-                    const float p = r0.v[i], q = r1.v[i];
-                    r0.v[i] = p * f.x - q * f.y;
-                    r1.v[i] = q * f.x + p * f.y;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC / 2; ++i) {
-                    const float2 f = cs[t][j0 + i], g = cs[t][j0 + VEC / 2 + i];
-                    const float p = r0.v[2 * i], q = r0.v[2 * i + 1], p2 = r1.v[2 * i], q2 = r1.v[2 * i + 1];
-                    r0.v[2 * i] = p * f.x - q * f.y;
-                    r0.v[2 * i + 1] = q * f.x + p * f.y;
-                    r1.v[2 * i] = p2 * g.x - q2 * g.y;
-                    r1.v[2 * i + 1] = q2 * g.x + p2 * g.y;
-                }
+                for (int i = 0; i < kRopeBatch; ++i)
+                    if (tb + i < nt) {
+                        r0[i].load(x + (tb + i) * a.x_rs[w] + e0);
+                        if (turn) r1[i].load(x + (tb + i) * a.x_rs[w] + e1);
+                    }
             }
-            r0.store(y + t * a.y_rs[w] + e0);
-            r1.store(y + t * a.y_rs[w] + e1);
+            if (!ready) {  // every thread of the CTA passes here in its first round
+                ready = true;
+                for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+                    const int t = i / half, j = i - t * half;
+                    const int pos = a.positions[t0 + t];
+                    if (j == 0) s_pos[t] = pos;
+                    const double ang = static_cast<double>(pos) * a.plan.freq[j];
+                    const double red = fma(-rint(ang * 0.15915494309189535), 6.283185307179586, ang);
+                    const float hi = static_cast<float>(red), lo = static_cast<float>(red - static_cast<double>(hi));
+                    float s, c;
+                    sincosf(hi, &s, &c);
+                    cs[t][j] = make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
+                }
+                __syncthreads();
+            }
+            if (!work) continue;
+#pragma unroll
+            for (int i = 0; i < kRopeBatch; ++i) {
+                const int t = tb + i;
+                if (t >= nt || s_pos[t] < 0) continue;
+                if (turn) {
+                    float p[VEC], q[VEC];
+                    r0[i].unpack(p);
+                    r1[i].unpack(q);
+                    if (!inter || VEC == 1) {
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) {
+                            const float2 f = cs[t][j0 + k];
+                            const float v = p[k], z = q[k];
+                            p[k] = v * f.x - z * f.y;
+                            q[k] = z * f.x + v * f.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < VEC / 2; ++k) {
+                            const float2 f = cs[t][j0 + k], g = cs[t][j0 + VEC / 2 + k];
+                            float v = p[2 * k], z = p[2 * k + 1];
+                            p[2 * k] = v * f.x - z * f.y;
+                            p[2 * k + 1] = z * f.x + v * f.y;
+                            v = q[2 * k], z = q[2 * k + 1];
+                            q[2 * k] = v * g.x - z * g.y;
+                            q[2 * k + 1] = z * g.x + v * g.y;
+                        }
+                    }
+                    r0[i].pack(p);
+                    r1[i].pack(q);
+                    r1[i].store(y + t * a.y_rs[w] + e1);
+                }
+                r0[i].store(y + t * a.y_rs[w] + e0);
+            }
         }
     }
 }
@@ -460,23 +481,26 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
     const int kv = blockIdx.y & 1, h = blockIdx.y >> 1, tid = threadIdx.x;
     const int row = tid / kLanes, col = (tid % kLanes) * 8;
     const T* x = static_cast<const T*>(a.x[kv]) + h * a.hs[kv] + col;
-    const int w0 = blockIdx.x * a.window, w1 = min(w0 + a.window, a.n);
-    int prev = w0 > 0 ? a.slots[w0 - 1] : -1;
-    for (int t = w0; t < w1;) {
-        const int slot = a.slots[t];
-        const int before = prev;
-        prev = slot;
-        // a run starts where the page changes; its rows follow slot by slot
-        if (slot < 0 || (before >= 0 && before / kKv8Page == slot / kKv8Page)) {
-            if (slot >= 0 && slot != before + 1 && tid == 0) raise_error(a.err, DM_DEVERR_RANGE);
-            ++t;
-            continue;
-        }
+    // lane l of every warp holds slot w0 - 1 + l: the window's rows are lanes 1 .. window, the
+    // lanes behind them the rest of the last run
+    const int w0 = blockIdx.x * a.window, lane = tid & 31;
+    const int at = w0 - 1 + lane;
+    const int slot_l = at >= 0 && at < a.n ? a.slots[at] : -1;
+    const int prev_l = __shfl_up_sync(0xffffffffu, slot_l, 1);
+    const bool same = lane > 0 && slot_l >= 0 && prev_l >= 0 && slot_l / kKv8Page == prev_l / kKv8Page;
+    const bool lead = lane > 0 && lane <= a.window && slot_l >= 0 && !same;
+    const unsigned follows = __ballot_sync(0xffffffffu, same && slot_l == prev_l + 1);
+    unsigned leads = __ballot_sync(0xffffffffu, lead);
+    if (same && slot_l != prev_l + 1 && lane <= a.window && tid < 32) raise_error(a.err, DM_DEVERR_RANGE);
+    while (leads) {
+        const int l = __ffs(leads) - 1;
+        leads &= leads - 1;
+        const int slot = __shfl_sync(0xffffffffu, slot_l, l);
         const int page = slot / kKv8Page, off = slot % kKv8Page;
-        int len = 1;
-        while (len < kKv8Page - off && t + len < a.n && a.slots[t + len] == slot + len) ++len;
-        const int t0 = t;
-        t += 1;
+        // rows that follow slot by slot
+        const unsigned rest = l < 31 ? ~(follows >> (l + 1)) : ~0u;
+        const int len = __ffs(rest);
+        const int t0 = w0 - 1 + l;
         if (page >= a.num_pages) {
             if (tid == 0) raise_error(a.err, DM_DEVERR_PAGE);
             continue;
@@ -718,14 +742,22 @@ extern "C" int32_t dm_rope(const dm_rope_plan* plan, int32_t dtype, int32_t n, c
         }
         vec = vec && aligned16(a.x[i], a.x_rs[i], a.x_hs[i], elem) && aligned16(a.y[i], a.y_rs[i], a.y_hs[i], elem);
     }
-    const int grid = (n + kRopeTok - 1) / kRopeTok;
+    // few tokens: a CTA each, for the shortest wait; many: 8, whose angles are then computed by
+    // the CTA's threads in one round (32771 tokens of 40 heads: see the figures above)
+    a.tok = n <= 8 * g.num_sms ? 1 : kRopeTok;
+    const int grid = (n + a.tok - 1) / a.tok;
+    // threads: the units of a token in equal rounds
+    const int v = vec ? 16 / elem : 1;
+    const int total = (Hq + Hk) * ((plan->head_dim - plan->rotary_dim / 2) / v);
+    const int rounds = (total + 383) / 384;
+    const int block = ((total + rounds - 1) / rounds + 31) / 32 * 32;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == DM_DTYPE_F32) {
-        if (vec) rope_kernel<float, 4><<<grid, 256, 0, s>>>(a);
-        else rope_kernel<float, 1><<<grid, 256, 0, s>>>(a);
+        if (vec) rope_kernel<float, 4><<<grid, block, 0, s>>>(a);
+        else rope_kernel<float, 1><<<grid, block, 0, s>>>(a);
     } else {
-        if (vec) rope_kernel<__nv_bfloat16, 8><<<grid, 256, 0, s>>>(a);
-        else rope_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(a);
+        if (vec) rope_kernel<__nv_bfloat16, 8><<<grid, block, 0, s>>>(a);
+        else rope_kernel<__nv_bfloat16, 1><<<grid, block, 0, s>>>(a);
     }
     return launch_status(cudaGetLastError(), st, eb, es);
 }
@@ -754,7 +786,9 @@ extern "C" int32_t dm_kv8_append(const dm_kv8_cache* c, int32_t dtype, int32_t n
     a.n = n;
     a.Hkv = c->num_kv_heads;
     a.num_pages = c->num_pages;
-    a.window = n <= 1024 ? 1 : 16;
+    // rows of a CTA: one when the rows may all be in pages of their own (a decode step), more
+    // for prompts, where a CTA per row would mostly find that an earlier one has its page
+    a.window = n <= 2048 ? 1 : n <= 8192 ? 4 : 16;
     a.vec = aligned16(k, k_rs, k_hs, elem) && aligned16(v, v_rs, v_hs, elem);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = dtype == DM_DTYPE_F32 ? launch_append<float>(a, c->head_dim, s)

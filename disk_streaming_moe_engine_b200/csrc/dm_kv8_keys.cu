@@ -24,9 +24,9 @@
 // leaves partial O, M, sum in the workspace, and the last of its CTAs to arrive joins them in
 // range order: the result does not depend on timing.
 //
-// Roles (192 threads): warps 0-3 softmax, epilogue and Q preparation; warp 4 producer (8 lanes,
-// one page each: page id and scales two tiles ahead, TMA boxes of 16 rows; a missing page
-// reads zeros); warp 5 MMA (one thread).  All waits are bounded; after a timeout every role
+// Roles (192 threads): warps 0-3 softmax, epilogue and Q preparation; warp 4 producer (groups
+// of 4 tiles, a lane per page: page ids and scales fetched groups ahead, TMA boxes of 16 rows;
+// a missing page reads zeros); warp 5 MMA (one thread).  All waits are bounded; after a timeout every role
 // leaves and copies and MMAs in flight are waited for.
 #include <cmath>
 
@@ -230,79 +230,85 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     const uint32_t tmem = s_tmem;
 
     if (active && warp == 4) {
-        // ---------------- producer: 8 lanes, one page of a tile each ----------------
+        // ---------------- producer: groups of 4 tiles, a lane per page ----------------
+        // Page ids are fetched two groups ahead of their use, scales one group ahead.
         uint32_t use = 0;  // tiles issued
         bool ok = true;
         KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
-        // pipeline over this CTA's tiles: page ids two ahead, scales one ahead
-        KeyWalk<RB> wi = w;      // walks ahead of w
-        int ti = -1, ei = 0;     // next tile of wi's item, end of its tiles
-        auto next_id = [&](int& id, int& h) {  // page id of this lane in the next tile (-1: none)
-            id = -1;
-            h = 0;
-            while (wi.unit < wi.end) {
+        int ti = -1, ei = 0, hi = 0;  // next tile of w's item, end of its tiles, its keys
+        struct Group {
+            int count = 0;             // tiles
+            int id = -1, h = 0;        // this lane's page (tile lane / 8, page lane % 8) and kv head
+            bool wanted = false;       // a key of the item lies on it
+            float2 sc = make_float2(0.0f, -1.0f);
+        };
+        auto fetch_ids = [&](Group& g) {
+            g = Group();
+            while (g.count < 32 / kKeyPages && w.unit < w.end) {
                 if (ti < 0) {
-                    int lo, hi;
-                    key_limits<RB>(a, wi.r, wi.blk, lo, hi);
-                    ti = wi.tile;
-                    ei = min(wi.tile + wi.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
+                    int lo;
+                    key_limits<RB>(a, w.r, w.blk, lo, hi);
+                    ti = w.tile;
+                    ei = min(w.tile + w.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
                 }
                 if (ti < ei) {
-                    int lo, hi;
-                    key_limits<RB>(a, wi.r, wi.blk, lo, hi);
-                    const int p = ti * kKeyPages + lane;
-                    if (lane < kKeyPages && p * kKv8Page < hi) id = max(-1, a.table[static_cast<size_t>(wi.req) * a.width + p]);
-                    else id = -2;  // beyond the keys: nothing to report
-                    h = wi.h;
+                    const int p = ti * kKeyPages + lane % kKeyPages;
+                    if (lane / kKeyPages == g.count) {
+                        g.h = w.h;
+                        g.wanted = p * kKv8Page < hi;
+                        if (g.wanted) g.id = a.table[static_cast<size_t>(w.req) * a.width + p];
+                    }
+                    ++g.count;
                     ++ti;
-                    return true;
+                } else {
+                    w.next(w.count());
+                    ti = -1;
                 }
-                wi.next(wi.count());
-                ti = -1;
             }
-            return false;
         };
-        auto scales_of = [&](int id, int h) {
-            float2 s = make_float2(0.0f, -1.0f);
-            if (id >= 0 && id < a.num_pages) {
-                const float* sc = a.scales + static_cast<size_t>(id) * 2 * a.Hkv + h;
-                s = make_float2(sc[0], sc[a.Hkv]);
-            } else if (id != -2 && lane < kKeyPages) {
+        auto fetch_scales = [&](Group& g) {
+            if (!g.wanted) return;
+            if (g.id >= 0 && g.id < a.num_pages) {
+                const float* sc = a.scales + static_cast<size_t>(g.id) * 2 * a.Hkv + g.h;
+                g.sc = make_float2(sc[0], sc[a.Hkv]);
+            } else {
                 raise_error(a.err, DM_DEVERR_PAGE);
             }
-            return s;
         };
-        int id0, h0, id1, h1;
-        bool have0 = next_id(id0, h0);
-        bool have1 = next_id(id1, h1);
-        float2 sc0 = have0 ? scales_of(id0, h0) : make_float2(0.0f, -1.0f);
-        while (have0 && ok) {
-            const uint32_t si = use % ST, ph = (use / ST) & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
-                ok = false;
-                break;
-            }
-            if (lane < kKeyPages) s_meta[si][lane] = sc0;
-            __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(&full[si], S::kStage);
-            __syncwarp();
-            if (lane < kKeyPages) {
-                const int page = sc0.y < 0.0f ? a.num_pages : id0;
-                const uint32_t k = smem_u32(sm + si * S::kStage) + lane * (kKv8Page * CW);
+        Group g0, g1, g2;
+        fetch_ids(g0);
+        fetch_ids(g1);
+        fetch_scales(g0);
+        while (g0.count > 0 && ok) {
+            fetch_ids(g2);
+            fetch_scales(g1);
+            for (int k = 0; k < g0.count; ++k) {
+                const uint32_t si = use % ST, ph = (use / ST) & 1u;
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                const bool mine = lane / kKeyPages == k;
+                const int pg = lane % kKeyPages;
+                if (mine) s_meta[si][pg] = g0.sc;
+                __syncwarp();
+                if (lane == 0) mbar_arrive_expect_tx(&full[si], S::kStage);
+                __syncwarp();
+                if (mine) {
+                    const int page = g0.sc.y < 0.0f ? a.num_pages : g0.id;
+                    const uint32_t kt = smem_u32(sm + si * S::kStage) + pg * (kKv8Page * CW);
 #pragma unroll
-                for (int c = 0; c < S::kChunks; ++c)
-                    tma_load_3d(k + c * (kKeyTile * CW), &ka.map, c * CW, h0 * kKv8Page, page, &full[si]);
+                    for (int c = 0; c < S::kChunks; ++c)
+                        tma_load_3d(kt + c * (kKeyTile * CW), &ka.map, c * CW, g0.h * kKv8Page, page, &full[si]);
 #pragma unroll
-                for (int c = 0; c < S::kChunks; ++c)
-                    tma_load_3d(k + S::kTileBytes + c * (kKeyTile * CW), &ka.map, c * CW, (a.Hkv + h0) * kKv8Page, page,
-                                &full[si]);
+                    for (int c = 0; c < S::kChunks; ++c)
+                        tma_load_3d(kt + S::kTileBytes + c * (kKeyTile * CW), &ka.map, c * CW, (a.Hkv + g0.h) * kKv8Page,
+                                    page, &full[si]);
+                }
+                ++use;
             }
-            ++use;
-            id0 = id1;
-            h0 = h1;
-            have0 = have1;
-            if (have0) sc0 = scales_of(id0, h0);
-            if (have1) have1 = next_id(id1, h1);
+            g0 = g1;
+            g1 = g2;
         }
         if (lane == 0)
             for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
@@ -633,29 +639,47 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                 }
                 named_bar_sync(1, 128);
                 if (s_last) {
+                    // references and sums of all parts by all threads, then the O rows, several
+                    // parts' loads in flight per thread
                     auto part_of = [&](int c) {
                         return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
                     };
-                    for (int r = 0; r < nrow; ++r) {
-                        float mm = -INFINITY, ll = 0.0f;
-                        float o[S::kChunks];
+                    constexpr int TR = 128 / RB;
+                    const int r = tid / TR, parts = c_last - c_first + 1;
+                    float mm = -INFINITY, ll = 0.0f;
+                    for (int c = tid % TR; c < parts; c += TR) mm = fmaxf(mm, __ldcg(part_of(c_first + c) + RB * D + r));
 #pragma unroll
-                        for (int c = 0; c < S::kChunks; ++c) o[c] = 0.0f;
-                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + r));
-                        const float mu = mm == -INFINITY ? 0.0f : mm;
-                        for (int c = c_first; c <= c_last; ++c) {
-                            const float* p = part_of(c);
-                            const float mc = __ldcg(p + RB * D + r);
-                            const float f = mc == mm ? 1.0f : exp2f(mc - mu);
-                            ll = fmaf(__ldcg(p + RB * D + RB + r), f, ll);
-                            if (tid < CW)
-#pragma unroll
-                                for (int k = 0; k < S::kChunks; ++k) o[k] = fmaf(__ldcg(p + r * D + k * CW + tid), f, o[k]);
-                        }
-                        if (tid < CW)
-#pragma unroll
-                            for (int k = 0; k < S::kChunks; ++k) put(r, k * CW + tid, o[k], mm, ll);
+                    for (int o = TR / 2; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+                    auto factor = [](float m, float top) { return m == top ? 1.0f : exp2f(m - top); };
+                    for (int c = tid % TR; c < parts; c += TR) {
+                        const float* p = part_of(c_first + c) + RB * D;
+                        ll = fmaf(__ldcg(p + RB + r), factor(__ldcg(p + r), mm), ll);
                     }
+#pragma unroll
+                    for (int o = TR / 2; o >= 1; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+                    if (tid % TR == 0) {
+                        s_red[0][r] = mm;
+                        s_red[1][r] = ll;
+                    }
+                    named_bar_sync(1, 128);
+#pragma unroll
+                    for (int k = 0; k < S::kChunks; ++k) {
+                        float o[RB];
+#pragma unroll
+                        for (int j = 0; j < RB; ++j) o[j] = 0.0f;
+                        if (tid < CW) {
+#pragma unroll 2
+                            for (int c = 0; c < parts; ++c) {
+                                const float* p = part_of(c_first + c);
+#pragma unroll
+                                for (int j = 0; j < RB; ++j)
+                                    o[j] = fmaf(__ldcg(p + j * D + k * CW + tid), factor(__ldcg(p + RB * D + j), s_red[0][j]), o[j]);
+                            }
+#pragma unroll
+                            for (int j = 0; j < RB; ++j) put(j, k * CW + tid, o[j], s_red[0][j], s_red[1][j]);
+                        }
+                    }
+                    named_bar_sync(1, 128);  // s_red is free again
                 }
             }
             w.next(cnt);
