@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     __shared__ float2 s_meta[ST][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
-    __shared__ float s_red[4][RB];
+    __shared__ float s_red[4][RB], s_fac[32][RB];
     __shared__ unsigned long long s_sum[kKeyThreads / 32 + 1];
     __shared__ long long s_rem;
     __shared__ unsigned long long s_total;
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
 
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 2);  // the copies, and the scales
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -290,12 +290,10 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                 }
                 const bool mine = lane / kKeyPages == k;
                 const int pg = lane % kKeyPages;
-                if (mine) s_meta[si][pg] = g0.sc;
-                __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&full[si], S::kStage);
                 __syncwarp();
                 if (mine) {
-                    const int page = g0.sc.y < 0.0f ? a.num_pages : g0.id;
+                    const int page = g0.id >= 0 && g0.id < a.num_pages ? g0.id : a.num_pages;
                     const uint32_t kt = smem_u32(sm + si * S::kStage) + pg * (kKv8Page * CW);
 #pragma unroll
                     for (int c = 0; c < S::kChunks; ++c)
@@ -304,7 +302,10 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                     for (int c = 0; c < S::kChunks; ++c)
                         tma_load_3d(kt + S::kTileBytes + c * (kKeyTile * CW), &ka.map, c * CW, (a.Hkv + g0.h) * kKv8Page,
                                     page, &full[si]);
+                    s_meta[si][pg] = g0.sc;
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[si]);
                 ++use;
             }
             g0 = g1;
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
             const long long tot = static_cast<long long>(total), gr = static_cast<long long>(grid);
             const int c_first = static_cast<int>(((item0 + 1) * gr - 1) / tot);
             const int c_last = static_cast<int>(((item0 + real) * gr - 1) / tot);
-            constexpr int kSlot = RB * (D + 2);
+            constexpr int kSlot = (RB * (D + 2) + 3) / 4 * 4;
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
             auto put = [&](int r, int d, float o, float mm, float ll) {
                 if (r >= nrow) return;
@@ -639,45 +640,58 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                 }
                 named_bar_sync(1, 128);
                 if (s_last) {
-                    // references and sums of all parts by all threads, then the O rows, several
-                    // parts' loads in flight per thread
+                    // the parts' references and sums to factors, 32 parts at a time, then O: every
+                    // thread sums its float4s over the parts, four parts' loads in flight
                     auto part_of = [&](int c) {
                         return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
                     };
-                    constexpr int TR = 128 / RB;
+                    constexpr int TR = 128 / RB, kVec = RB * D / 4 / 128;
                     const int r = tid / TR, parts = c_last - c_first + 1;
                     float mm = -INFINITY, ll = 0.0f;
                     for (int c = tid % TR; c < parts; c += TR) mm = fmaxf(mm, __ldcg(part_of(c_first + c) + RB * D + r));
 #pragma unroll
                     for (int o = TR / 2; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-                    auto factor = [](float m, float top) { return m == top ? 1.0f : exp2f(m - top); };
-                    for (int c = tid % TR; c < parts; c += TR) {
-                        const float* p = part_of(c_first + c) + RB * D;
-                        ll = fmaf(__ldcg(p + RB + r), factor(__ldcg(p + r), mm), ll);
+                    float4 o[kVec];
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int c0 = 0; c0 < parts; c0 += 32) {
+                        const int nc = min(32, parts - c0);
+                        for (int c = tid % TR; c < nc; c += TR) {
+                            const float* p = part_of(c_first + c0 + c) + RB * D;
+                            const float mc = __ldcg(p + r);
+                            const float f = mc == mm ? 1.0f : exp2f(mc - mm);
+                            s_fac[c][r] = f;
+                            ll = fmaf(__ldcg(p + RB + r), f, ll);
+                        }
+                        named_bar_sync(1, 128);
+#pragma unroll 4
+                        for (int c = 0; c < nc; ++c) {
+                            const float4* p = reinterpret_cast<const float4*>(part_of(c_first + c0 + c));
+#pragma unroll
+                            for (int j = 0; j < kVec; ++j) {
+                                const float4 x = __ldcg(p + j * 128 + tid);
+                                const float f = s_fac[c][(j * 128 + tid) * 4 / D];
+                                o[j].x = fmaf(x.x, f, o[j].x), o[j].y = fmaf(x.y, f, o[j].y);
+                                o[j].z = fmaf(x.z, f, o[j].z), o[j].w = fmaf(x.w, f, o[j].w);
+                            }
+                        }
+                        named_bar_sync(1, 128);
                     }
 #pragma unroll
-                    for (int o = TR / 2; o >= 1; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+                    for (int x = TR / 2; x >= 1; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
                     if (tid % TR == 0) {
                         s_red[0][r] = mm;
                         s_red[1][r] = ll;
                     }
                     named_bar_sync(1, 128);
 #pragma unroll
-                    for (int k = 0; k < S::kChunks; ++k) {
-                        float o[RB];
-#pragma unroll
-                        for (int j = 0; j < RB; ++j) o[j] = 0.0f;
-                        if (tid < CW) {
-#pragma unroll 2
-                            for (int c = 0; c < parts; ++c) {
-                                const float* p = part_of(c_first + c);
-#pragma unroll
-                                for (int j = 0; j < RB; ++j)
-                                    o[j] = fmaf(__ldcg(p + j * D + k * CW + tid), factor(__ldcg(p + RB * D + j), s_red[0][j]), o[j]);
-                            }
-#pragma unroll
-                            for (int j = 0; j < RB; ++j) put(j, k * CW + tid, o[j], s_red[0][j], s_red[1][j]);
-                        }
+                    for (int j = 0; j < kVec; ++j) {
+                        const int e = (j * 128 + tid) * 4, row = e / D, d = e % D;
+                        const float m2 = s_red[0][row], l2 = s_red[1][row];
+                        put(row, d, o[j].x, m2, l2);
+                        put(row, d + 1, o[j].y, m2, l2);
+                        put(row, d + 2, o[j].z, m2, l2);
+                        put(row, d + 3, o[j].w, m2, l2);
                     }
                     named_bar_sync(1, 128);  // s_red is free again
                 }
