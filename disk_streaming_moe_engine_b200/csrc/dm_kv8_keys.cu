@@ -8,7 +8,7 @@
 //   O^T [D x N]         += codeV^T [D x 128] . Pterms [128 x N]
 // N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
 // scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
-// before it left) and costs only N: 2 terms give bf16's 8 bits, 6 give 24.  The tensor time of
+// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  The tensor time of
 // a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
 // below the time of the tile's bytes from HBM, which is what bounds the kernel.
 //
@@ -16,17 +16,18 @@
 //   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
 // M the row's reference for x + v: raised to the running maximum whenever some x + v exceeds
 // it by more than 2 (then O^T and the sums are rescaled), so w <= 4 and 64 w stays in e4m3's
-// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t owns token t of the tile: its scores, its
-// weights, its share of the row sums; nothing else crosses threads but the reference.
+// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t of a group of 128 owns token t of the
+// tile for 8 of the rows: scores, weights, its share of the row sums; only the reference
+// crosses threads.
 //
 // Split: all items' tiles in one sequence, cut into one contiguous range per CTA (one CTA per
 // SM, persistent), so ragged lengths balance to a tile.  An item cut by a range boundary
 // leaves partial O, M, sum in the workspace, and the last of its CTAs to arrive joins them in
 // range order: the result does not depend on timing.
 //
-// Roles (192 threads): warps 0-3 softmax, epilogue and Q preparation; warp 4 producer (groups
-// of 4 tiles, a lane per page: page ids and scales fetched groups ahead, TMA boxes of 16 rows;
-// a missing page reads zeros); warp 5 MMA (one thread).  All waits are bounded; after a timeout every role
+// Roles: RB / 8 groups of 4 warps for softmax, epilogue and Q preparation; a producer warp
+// (groups of 4 tiles, a lane per page: page ids and scales fetched groups ahead, TMA boxes of 16
+// rows; a missing page reads zeros); an MMA warp (one thread).  All waits are bounded; after a timeout every role
 // leaves and copies and MMAs in flight are waited for.
 #include <cmath>
 
@@ -34,17 +35,18 @@
 
 namespace dm {
 
-constexpr int kKeyThreads = 192;
 constexpr int kKeyTile = 128;
 constexpr int kKeyPages = kKeyTile / kKv8Page;
-constexpr int kKeySmem = 227 * 1024 - 2048;  // dynamic shared memory (static arrays beside it)
+constexpr int kKeySmem = 227 * 1024 - 4096;  // dynamic shared memory (static arrays beside it)
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
 
 template <typename T, int D, int RB>
 struct KeyShape {
-    static constexpr int kTerms = sizeof(T) == 4 ? 6 : 2;
-    static constexpr int kN = RB * kTerms;
+    static constexpr int kTerms = sizeof(T) == 4 ? 5 : 2;
+    static constexpr int kN = (RB * kTerms + 15) / 16 * 16;  // columns behind the terms are never read
+    static constexpr int kSoft = RB * 16;                    // softmax threads
+    static constexpr int kThreads = kSoft + 64;
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
     static constexpr int kTileBytes = kKeyTile * D;   // K or V of a tile
@@ -146,9 +148,10 @@ struct KeyWalk {
 };
 
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
+__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB>;
-    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages;
+    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages, SOFT = S::kSoft;
+    constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
     extern __shared__ __align__(1024) uint8_t key_raw[];
     uint8_t* sm = key_raw + ((1024u - (smem_u32(key_raw) & 1023u)) & 1023u);
@@ -159,11 +162,12 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
     __shared__ float s_red[4][RB], s_fac[32][RB];
-    __shared__ unsigned long long s_sum[kKeyThreads / 32 + 1];
+    __shared__ unsigned long long s_sum[NT / 32 + 1];
     __shared__ long long s_rem;
     __shared__ unsigned long long s_total;
     __shared__ uint32_t s_tmem;
     __shared__ int s_req, s_abort;
+    __shared__ uint8_t s_nan[kKeyTile];
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &s_abort;
@@ -175,18 +179,18 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_ready[i], 128);
+            mbar_init(&p_ready[i], SOFT);
             mbar_init(&pv_done[i], 1);
         }
-        mbar_init(&q_ready, 128);
+        mbar_init(&q_ready, SOFT);
         mbar_init(&done_bar, 1);
         mbar_fence_init();
         s_abort = 0;
     }
-    if (warp == 5) tc_alloc(&s_tmem, S::kCols);
+    if (warp == W_MMA) tc_alloc(&s_tmem, S::kCols);
 
     // this CTA's range of the tile sequence: block-wide sums of the requests' tiles
-    const int per = (a.n + kKeyThreads - 1) / kKeyThreads;
+    const int per = (a.n + NT - 1) / NT;
     const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
     unsigned long long mine = 0;
     for (int i = i0; i < i1; ++i) {
@@ -204,7 +208,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     __syncthreads();
     tc_fence_after();
     unsigned long long base = 0, total = 0;
-    for (int w = 0; w < kKeyThreads / 32; ++w) {
+    for (int w = 0; w < NT / 32; ++w) {
         if (w < warp) base += s_sum[w];
         total += s_sum[w];
     }
@@ -229,7 +233,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     __syncthreads();
     const uint32_t tmem = s_tmem;
 
-    if (active && warp == 4) {
+    if (active && warp == W_LOAD) {
         // ---------------- producer: groups of 4 tiles, a lane per page ----------------
         // Page ids are fetched two groups ahead of their use, scales one group ahead.
         uint32_t use = 0;  // tiles issued
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
         if (lane == 0)
             for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
                 mbar_wait_bounded(&full[u % ST], (u / ST) & 1u, a.err, nullptr);
-    } else if (active && warp == 5) {
+    } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
             uint32_t t = 0, item = 0;
@@ -370,7 +374,8 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
         }
     } else if (active) {
         // ---------------- softmax, epilogue, Q ----------------
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+        const int tt = tid & 127, r0 = tid / 128 * 8, wq = warp & 3;  // token, first row, warp of the group
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + r0;
         uint32_t t = 0;
         bool ok = true;
         KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
@@ -385,9 +390,9 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                 continue;
             }
             const int nrow = min(RB, w.r.m * a.group - w.blk * RB);
-            {   // Q terms: 128 / RB threads per row
-                constexpr int TR = 128 / RB, E = D / TR;
-                const int r = tid / TR, e0 = (tid % TR) * E;
+            {   // Q terms: 16 threads per row
+                constexpr int E = D / 16;
+                const int r = tid / 16, e0 = (tid % 16) * E;
                 const int f = w.blk * RB + min(r, nrow - 1);
                 const int tok = f / a.group, head = w.h * a.group + f % a.group;
                 const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(w.r.row0 + tok) * a.q_rs +
@@ -395,17 +400,18 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                 float x[E];
                 float amax = 0.0f;
 #pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = r < nrow ? static_cast<float>(q[e]) : 0.0f;
+#pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    x[e] = r < nrow ? static_cast<float>(q[e]) : 0.0f;
                     if (!(fabsf(x[e]) <= 3.402823466e38f)) x[e] = __int_as_float(0x7fc00000);
                     amax = fmaxf(amax, fabsf(x[e]));
                 }
 #pragma unroll
-                for (int o = TR / 2; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 // largest magnitude of the row to [2^7, 2^8)
                 const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
                 const float mul = __int_as_float((127 - ex) << 23);
-                if (tid % TR == 0) {
+                if (tid % 16 == 0) {
                     s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
                     s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
                 }
@@ -425,138 +431,153 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                     }
                 fence_proxy_async_smem();
                 mbar_arrive(&q_ready);
-                named_bar_sync(1, 128);
+                named_bar_sync(1, SOFT);
             }
-            float mref[RB], l[RB];
+            float mref[8], l[8], frow[8];
 #pragma unroll
-            for (int r = 0; r < RB; ++r) mref[r] = -INFINITY, l[r] = 0.0f;
+            for (int r = 0; r < 8; ++r) mref[r] = -INFINITY, l[r] = 0.0f, frow[r] = s_frow[r0 + r];
 
             for (int i = 0; i < nt; ++i) {
                 const uint32_t x = t + i, si = x % ST;
-                const int key = (t_begin + i) * kKeyTile + tid;
-                const int tile_end = (t_begin + i + 1) * kKeyTile;
-                ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag);
-                ok = ok && mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag);
-                // every thread of the four warps leaves together
-                if (named_bar_or(1, 128, !ok)) {
-                    ok = false;
-                    break;
+                const int key = (t_begin + i) * kKeyTile + tt;
+                // the tile's copies and scales, its scores, and (from the third tile on) the P buffer,
+                // tried together since they are mostly there
+                const bool t1 = mbar_try_wait(&full[si], (x / ST) & 1u);
+                const bool t2 = mbar_try_wait(&s_full[x & 1u], (x >> 1) & 1u);
+                const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
+                if (!(t1 && t2 && t3)) {
+                    ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag) &&
+                         mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag) &&
+                         (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
                 }
+                __syncwarp();  // the loads below are the whole warp's
                 tc_fence_after();
-                const float2 sc = s_meta[si][tid >> 4];
+                const float2 sc = s_meta[si][tt >> 4];
                 const float vexp = static_cast<float>(((__float_as_int(sc.y) >> 23) & 0xff) - 127);
-                float y[RB];
+                float y[8];
                 {
-                    float c[16];
+                    float c[TERMS][8];
 #pragma unroll
-                    for (int b = 0; b < N / 16; ++b) {
-                        tc_ld16(lanes + (x & 1u) * N + b * 16, c);
-                        tc_wait_ld();
+                    for (int b = 0; b < TERMS; ++b) tc_ld8(lanes + (x & 1u) * N + b * RB, c[b]);
+                    tc_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int n = b * 16 + j, term = n / RB, r = n % RB;
-                            const float s = 1.0f / static_cast<float>(1 << (4 * term));
-                            y[r] = term == 0 ? c[j] : fmaf(c[j], s, y[r]);
-                        }
+                    for (int r = 0; r < 8; ++r) {
+                        y[r] = c[0][r];
+#pragma unroll
+                        for (int b = 1; b < TERMS; ++b) y[r] = fmaf(c[b][r], 1.0f / static_cast<float>(1 << (4 * b)), y[r]);
+                        y[r] = fmaf(y[r], frow[r] * sc.x, vexp);
                     }
                 }
-                const bool edge = tile_end > lim_min;
-                bool over = false;
+                const bool edge = (t_begin + i + 1) * kKeyTile > lim_min;
+                bool over = !ok;
+                if (edge) {
 #pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    y[r] = fmaf(y[r], s_frow[r] * sc.x, vexp);
-                    if (edge && key >= s_lim[r]) y[r] = -INFINITY;
-                    if (sc.y < 0.0f) y[r] = -INFINITY;
-                    over = over || y[r] > mref[r] + kKeyLazy;
+                    for (int r = 0; r < 8; ++r)
+                        if (key >= s_lim[r0 + r]) y[r] = -INFINITY;
                 }
-                if (named_bar_or(1, 128, over)) {
-                    // raise the references to the maximum of this tile and rescale
+                if (sc.y < 0.0f) {
 #pragma unroll
-                    for (int r = 0; r < RB; ++r) {
+                    for (int r = 0; r < 8; ++r) y[r] = -INFINITY;
+                }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) over = over || y[r] > mref[r] + kKeyLazy;
+                if (named_bar_or(1, SOFT, over)) {
+                    // raise the references to the maximum of this tile and rescale; after a failed
+                    // wait all threads leave together here
+                    if (ok && i > 0)
+                        ok = mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
                         const float mx = warp_max(y[r]);
-                        if (lane == 0) s_red[warp][r] = mx;
+                        if (lane == 0) s_red[wq][r0 + r] = mx;
                     }
-                    named_bar_sync(1, 128);
-                    float fac[RB];
+                    if (named_bar_or(1, SOFT, !ok)) {
+                        ok = false;
+                        break;
+                    }
+                    float fac[8];
 #pragma unroll
-                    for (int r = 0; r < RB; ++r) {
-                        const float mx = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r]));
+                    for (int r = 0; r < 8; ++r) {
+                        const float mx = fmaxf(fmaxf(s_red[0][r0 + r], s_red[1][r0 + r]), fmaxf(s_red[2][r0 + r], s_red[3][r0 + r]));
                         const float nm = fmaxf(mref[r], mx);
                         fac[r] = nm == mref[r] ? 1.0f : exp2f(mref[r] - nm);
                         mref[r] = nm;
                         l[r] *= fac[r];
                     }
                     if (i > 0) {
-                        ok = mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
                         tc_fence_after();
 #pragma unroll
-                        for (int b = 0; b < S::kChunks * N / 16; ++b) {
-                            float c[16];
-                            uint32_t u[16];
-                            tc_ld16(lanes + 2 * N + b * 16, c);
-                            tc_wait_ld();
+                        for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(c[j] * fac[(b * 16 + j) % RB]);
-                            tc_st16(lanes + 2 * N + b * 16, u);
-                        }
+                            for (int b = 0; b < TERMS; ++b) {
+                                float o[8];
+                                tc_ld8(lanes + (2 + c) * N + b * RB, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int r = 0; r < 8; ++r) o[r] *= fac[r];
+                                tc_st8(lanes + (2 + c) * N + b * RB, o);
+                            }
                         tc_wait_st();
                     }
-                    named_bar_sync(1, 128);  // s_red is free again
+                    named_bar_sync(1, SOFT);  // s_red is free again
                 }
                 // weights, row sums, e4m3 terms
                 const float vinv = __int_as_float((127 - static_cast<int>(vexp)) << 23);
 #pragma unroll
-                for (int r = 0; r < RB; ++r) {
-                    const float wgt = exp2f(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
+                for (int r = 0; r < 8; ++r) {
+                    const float wgt = ex2(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
                     l[r] = fmaf(wgt, vinv, l[r]);
                     y[r] = wgt * kKeyBoost;
                 }
-                if (edge && sc.y >= 0.0f) {
+                if (edge) {
                     // V rows behind the last key become zeros; a NaN code that not every row sees
                     // becomes 0 and makes the sums of the rows that see it NaN
-                    uint8_t* v = sm + si * S::kStage + S::kTileBytes + tid * CW;
-                    if (key >= lim_max) {
-#pragma unroll
-                        for (int c = 0; c < S::kChunks; ++c)
-                            for (int u = 0; u < CW / 16; ++u)
-                                *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
-                    } else if (key >= lim_min) {
+                    if (r0 == 0) {
+                        uint8_t* v = sm + si * S::kStage + S::kTileBytes + tt * CW;
                         bool nan = false;
+                        if (key >= lim_max) {
 #pragma unroll
-                        for (int c = 0; c < S::kChunks; ++c)
-                            for (int u = 0; u < CW / 4; ++u) {
-                                uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
-                                const uint32_t bad = e4m3_nan_mask(*p);
-                                if (bad) {
-                                    *p &= ~bad;
-                                    nan = true;
+                            for (int c = 0; c < S::kChunks; ++c)
+                                for (int u = 0; u < CW / 16; ++u)
+                                    *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
+                        } else if (key >= lim_min) {
+#pragma unroll
+                            for (int c = 0; c < S::kChunks; ++c)
+                                for (int u = 0; u < CW / 4; ++u) {
+                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
+                                    const uint32_t bad = e4m3_nan_mask(*p);
+                                    if (bad) {
+                                        *p &= ~bad;
+                                        nan = true;
+                                    }
                                 }
-                            }
-                        if (nan)
+                        }
+                        s_nan[tt] = nan;
+                    }
+                    named_bar_sync(1, SOFT);
+                    if (s_nan[tt]) {
 #pragma unroll
-                            for (int r = 0; r < RB; ++r)
-                                if (key < s_lim[r]) l[r] = __int_as_float(0x7fc00000);
+                        for (int r = 0; r < 8; ++r)
+                            if (key < s_lim[r0 + r]) l[r] = __int_as_float(0x7fc00000);
                     }
                 }
-                if (ok && x >= 2 && i >= 2)
-                    ok = mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag);
-                uint8_t* p = s_p + (x & 1u) * S::kP + tid * 16;
-                uint32_t code[4] = {0, 0, 0, 0};
+                uint8_t* p = s_p + (x & 1u) * S::kP + tt * 16;
 #pragma unroll
-                for (int i2 = 0; i2 < TERMS; ++i2)
+                for (int b = 0; b < TERMS; ++b) {
+                    uint32_t code[4];
 #pragma unroll
-                    for (int r = 0; r < RB; r += 2) {
+                    for (int r = 0; r < 8; r += 2) {
                         float2 back;
-                        const uint32_t c2 = e4m3_round2(y[r], y[r + 1], back);
-                        if (i2 + 1 < TERMS) {
+                        code[r / 2] = e4m3_round2(y[r], y[r + 1], back);
+                        if (b + 1 < TERMS) {
                             y[r] = (y[r] - back.x) * 16.0f;
                             y[r + 1] = (y[r + 1] - back.y) * 16.0f;
                         }
-                        const int n = i2 * RB + r, wd = (n % 16) / 4;
-                        code[wd] = (n % 4 == 0) ? c2 : (code[wd] | (c2 << 16));
-                        if (n % 16 == 14)
-                            *reinterpret_cast<uint4*>(p + (n / 16) * (kKeyTile * 16)) = make_uint4(code[0], code[1], code[2], code[3]);
                     }
+                    const int n = b * RB + r0;
+                    *reinterpret_cast<uint2*>(p + (n / 16) * (kKeyTile * 16) + n % 16) =
+                        make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
+                }
                 fence_proxy_async_smem();
                 tc_fence_before();
                 mbar_arrive(&p_ready[x & 1u]);
@@ -565,19 +586,19 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
             t += nt;
             // the item's sums, then O
 #pragma unroll
-            for (int r = 0; r < RB; ++r) {
+            for (int r = 0; r < 8; ++r) {
                 const float s = warp_sum(l[r]);
-                if (lane == 0) s_red[warp][r] = s;
+                if (lane == 0) s_red[wq][r0 + r] = s;
             }
             ok = mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
-            if (named_bar_or(1, 128, !ok)) {
+            if (named_bar_or(1, SOFT, !ok)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
 #pragma unroll
-            for (int r = 0; r < RB; ++r) l[r] = s_red[0][r] + s_red[1][r] + s_red[2][r] + s_red[3][r];
-            named_bar_sync(1, 128);  // s_red is free again
+            for (int r = 0; r < 8; ++r) l[r] = s_red[0][r0 + r] + s_red[1][r0 + r] + s_red[2][r0 + r] + s_red[3][r0 + r];
+            named_bar_sync(1, SOFT);  // s_red is free again
 
             const long long item0 = w.unit - t_begin;  // the item's first tile in the sequence
             const bool whole = t_begin == 0 && nt == real;
@@ -599,38 +620,36 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
             };
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c) {
-                float o[RB];
-                float v[16];
+                float o[8], v[TERMS][8];
 #pragma unroll
-                for (int b = 0; b < N / 16; ++b) {
-                    tc_ld16(lanes + (2 + c) * N + b * 16, v);
-                    tc_wait_ld();
+                for (int b = 0; b < TERMS; ++b) tc_ld8(lanes + (2 + c) * N + b * RB, v[b]);
+                tc_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int n = b * 16 + j, term = n / RB, r = n % RB;
-                        const float s = 1.0f / (static_cast<float>(1 << (4 * term)) * kKeyBoost);
-                        o[r] = term == 0 ? v[j] * s : fmaf(v[j], s, o[r]);
-                    }
+                for (int r = 0; r < 8; ++r) {
+                    o[r] = v[0][r] * (1.0f / kKeyBoost);
+#pragma unroll
+                    for (int b = 1; b < TERMS; ++b)
+                        o[r] = fmaf(v[b][r], 1.0f / (static_cast<float>(1 << (4 * b)) * kKeyBoost), o[r]);
                 }
-                if (tid < CW) {
+                if (tt < CW) {
 #pragma unroll
-                    for (int r = 0; r < RB; ++r) {
-                        if (whole) put(r, c * CW + tid, o[r], mref[r], l[r]);
-                        else slot[r * D + c * CW + tid] = o[r];
+                    for (int r = 0; r < 8; ++r) {
+                        if (whole) put(r0 + r, c * CW + tt, o[r], mref[r], l[r]);
+                        else slot[(r0 + r) * D + c * CW + tt] = o[r];
                     }
                 }
             }
             tc_fence_before();
             if (!whole) {
-                if (tid == 0) {
+                if (tt == 0) {
 #pragma unroll
-                    for (int r = 0; r < RB; ++r) {
-                        slot[RB * D + r] = mref[r];
-                        slot[RB * D + RB + r] = l[r];
+                    for (int r = 0; r < 8; ++r) {
+                        slot[RB * D + r0 + r] = mref[r];
+                        slot[RB * D + RB + r0 + r] = l[r];
                     }
                 }
                 __threadfence();
-                named_bar_sync(1, 128);
+                named_bar_sync(1, SOFT);
                 if (tid == 0) {
                     const unsigned parts = static_cast<unsigned>(c_last - c_first + 1);
                     const unsigned got = atomicAdd(a.counters + c_first, 1u);
@@ -638,14 +657,14 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                     if (s_last) a.counters[c_first] = 0;
                     __threadfence();
                 }
-                named_bar_sync(1, 128);
+                named_bar_sync(1, SOFT);
                 if (s_last) {
                     // the parts' references and sums to factors, 32 parts at a time, then O: every
                     // thread sums its float4s over the parts, four parts' loads in flight
                     auto part_of = [&](int c) {
                         return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
                     };
-                    constexpr int TR = 128 / RB, kVec = RB * D / 4 / 128;
+                    constexpr int TR = 16, kVec = D / 64;
                     const int r = tid / TR, parts = c_last - c_first + 1;
                     float mm = -INFINITY, ll = 0.0f;
                     for (int c = tid % TR; c < parts; c += TR) mm = fmaxf(mm, __ldcg(part_of(c_first + c) + RB * D + r));
@@ -663,19 +682,19 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                             s_fac[c][r] = f;
                             ll = fmaf(__ldcg(p + RB + r), f, ll);
                         }
-                        named_bar_sync(1, 128);
+                        named_bar_sync(1, SOFT);
 #pragma unroll 4
                         for (int c = 0; c < nc; ++c) {
                             const float4* p = reinterpret_cast<const float4*>(part_of(c_first + c0 + c));
 #pragma unroll
                             for (int j = 0; j < kVec; ++j) {
-                                const float4 x = __ldcg(p + j * 128 + tid);
-                                const float f = s_fac[c][(j * 128 + tid) * 4 / D];
+                                const float4 x = __ldcg(p + j * SOFT + tid);
+                                const float f = s_fac[c][(j * SOFT + tid) * 4 / D];
                                 o[j].x = fmaf(x.x, f, o[j].x), o[j].y = fmaf(x.y, f, o[j].y);
                                 o[j].z = fmaf(x.z, f, o[j].z), o[j].w = fmaf(x.w, f, o[j].w);
                             }
                         }
-                        named_bar_sync(1, 128);
+                        named_bar_sync(1, SOFT);
                     }
 #pragma unroll
                     for (int x = TR / 2; x >= 1; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
@@ -683,17 +702,17 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
                         s_red[0][r] = mm;
                         s_red[1][r] = ll;
                     }
-                    named_bar_sync(1, 128);
+                    named_bar_sync(1, SOFT);
 #pragma unroll
                     for (int j = 0; j < kVec; ++j) {
-                        const int e = (j * 128 + tid) * 4, row = e / D, d = e % D;
+                        const int e = (j * SOFT + tid) * 4, row = e / D, d = e % D;
                         const float m2 = s_red[0][row], l2 = s_red[1][row];
                         put(row, d, o[j].x, m2, l2);
                         put(row, d + 1, o[j].y, m2, l2);
                         put(row, d + 2, o[j].z, m2, l2);
                         put(row, d + 3, o[j].w, m2, l2);
                     }
-                    named_bar_sync(1, 128);  // s_red is free again
+                    named_bar_sync(1, SOFT);  // s_red is free again
                 }
             }
             w.next(cnt);
@@ -701,7 +720,7 @@ __global__ void __launch_bounds__(kKeyThreads, 1) kv8_attn_keys_kernel(const __g
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == W_MMA) {
         tc_fence_after();
         tc_dealloc(tmem, S::kCols);
     }
@@ -740,7 +759,7 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
         if (e != cudaSuccess) return e;
         if (dev < 64) ready[dev] = true;
     }
-    kv8_attn_keys_kernel<T, D, RB><<<num_sms, kKeyThreads, S::kSmem, s>>>(ka);
+    kv8_attn_keys_kernel<T, D, RB><<<num_sms, S::kThreads, S::kSmem, s>>>(ka);
     return cudaGetLastError();
 }
 

@@ -82,7 +82,14 @@ DM_DEV uint32_t e4m3_round2(float a, float b, float2& back) {
 // 0xff in the bytes of w that hold a NaN code
 DM_DEV uint32_t e4m3_nan_mask(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
-// Barrier over the 128 softmax threads that also ORs a predicate.
+// 2^x of the special function unit (relative error 2^-22; results below 2^-126 become 0)
+DM_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Barrier over `count` threads that also ORs a predicate.
 DM_DEV bool named_bar_or(int id, int count, bool v) {
     uint32_t r;
     asm volatile(
