@@ -35,14 +35,14 @@ struct Kv8AttnArgs {
     const int* seq_lens;
     const int* cu_q;      // null: one row per request
     float* part;          // partial results of items that several CTAs share
-    unsigned* counters;   // [num_sms] their arrivals
+    unsigned* counters;   // [2 num_sms] their arrivals
     uint32_t* err;
     int64_t q_rs, q_hs, o_rs, o_hs;  // strides in elements
     float scale_log2;     // sm_scale * log2(e)
     int n, rows, Hq, Hkv, group, num_pages, width, max_q;
 };
 
-// dm_kv8_keys.cu: any row count and type, one CTA per SM.  Workspace: counters [num_sms], then
+// dm_kv8_keys.cu: any row count and type, one or two CTAs per SM.  Workspace: counters [2 num_sms], then
 // the partials' floats.
 cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f32, int num_sms, int dev, cudaStream_t s);
 size_t kv8_keys_part_floats(int D, int num_sms);

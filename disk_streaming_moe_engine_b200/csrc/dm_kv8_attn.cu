@@ -6,8 +6,8 @@
 
 namespace dm {
 
-// Workspace: counters [num_sms] (zero between calls), then the partial results.
-static size_t counter_bytes(int num_sms) { return (static_cast<size_t>(num_sms) * sizeof(unsigned) + 255) / 256 * 256; }
+// Workspace: a counter per CTA, two per SM at most (zero between calls), then the partial results.
+static size_t counter_bytes(int num_sms) { return (static_cast<size_t>(2 * num_sms) * sizeof(unsigned) + 255) / 256 * 256; }
 static size_t workspace_bytes(int D, int num_sms) {
     return counter_bytes(num_sms) + kv8_keys_part_floats(D, num_sms) * sizeof(float);
 }

@@ -20,7 +20,7 @@
 // tile for 8 of the rows: scores, weights, its share of the row sums; only the reference
 // crosses threads.
 //
-// Split: all items' tiles in one sequence, cut into one contiguous range per CTA (one CTA per
+// Split: all items' tiles in one sequence, cut into one contiguous range per CTA (one or two per
 // SM, persistent), so ragged lengths balance to a tile.  An item cut by a range boundary
 // leaves partial O, M, sum in the workspace, and the last of its CTAs to arrive joins them in
 // range order: the result does not depend on timing.
@@ -37,7 +37,7 @@ namespace dm {
 
 constexpr int kKeyTile = 128;
 constexpr int kKeyPages = kKeyTile / kKv8Page;
-constexpr int kKeySmem = 227 * 1024 - 4096;  // dynamic shared memory (static arrays beside it)
+constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its CTAs
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
 
@@ -54,7 +54,10 @@ struct KeyShape {
     static constexpr int kQ = kN * D;
     static constexpr int kP = kN * kKeyTile;          // one of two buffers
     static constexpr int kFixed = kQ + 2 * kP + 1024;
-    static constexpr int kFit = (kKeySmem - kFixed) / kStage;
+    // a tile's chain of waits takes about 0.65 us whatever D is, its bytes from HBM 0.37 us at
+    // D = 64 and 1.5 us at D = 256: the smaller heads take two CTAs per SM
+    static constexpr int kCtas = D <= 128 && RB == 8 ? 2 : 1;
+    static constexpr int kFit = (kKeySmem / kCtas - 5120 - kFixed) / kStage;  // static arrays and 1 KB per CTA beside it
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kFixed;
     static constexpr int kColsUsed = (2 + kChunks) * kN;
@@ -73,22 +76,29 @@ struct KeyReq {
     int row0, m, len, full, blocks, tiles;
 };
 
+struct KeyRaw {  // a request's words as loaded
+    int c0, c1, len;
+};
+DM_DEV KeyRaw key_raw(const Kv8AttnArgs& a, int i) {
+    KeyRaw w = {i, i + 1, 0};
+    if (i >= a.n) return w;
+    if (a.cu_q) w.c0 = a.cu_q[i], w.c1 = a.cu_q[i + 1];
+    w.len = a.seq_lens[i];
+    return w;
+}
+
 template <int RB>
-DM_DEV KeyReq key_req(const Kv8AttnArgs& a, int i, bool report) {
+DM_DEV KeyReq key_req(const Kv8AttnArgs& a, const KeyRaw& w, bool report) {
     KeyReq r;
-    r.row0 = i;
-    r.m = 1;
-    if (a.cu_q) {
-        r.row0 = a.cu_q[i];
-        const long long m = static_cast<long long>(a.cu_q[i + 1]) - r.row0;
-        if (r.row0 < 0 || m < 0 || m > a.max_q || r.row0 + m > a.rows) {
-            if (report) raise_error(a.err, DM_DEVERR_RANGE);
-            r.m = 0;
-        } else {
-            r.m = static_cast<int>(m);
-        }
+    r.row0 = w.c0;
+    const long long m = static_cast<long long>(w.c1) - w.c0;
+    if (w.c0 < 0 || m < 0 || m > a.max_q || w.c0 + m > a.rows) {
+        if (report) raise_error(a.err, DM_DEVERR_RANGE);
+        r.m = 0;
+    } else {
+        r.m = static_cast<int>(m);
     }
-    r.full = a.seq_lens[i];
+    r.full = w.len;
     if (r.full < 0) {
         if (report) raise_error(a.err, DM_DEVERR_RANGE);
         r.full = 0;
@@ -119,9 +129,11 @@ struct KeyWalk {
     long long unit, end;  // this CTA's range
     int req, blk, h, tile;
     KeyReq r;
+    KeyRaw ahead;  // of request req + 1, loaded before it is needed
     DM_DEV KeyWalk(const Kv8AttnArgs& args, long long u0, long long u1, int rq, long long rem) : a(args), unit(u0), end(u1) {
         req = rq;
-        r = key_req<RB>(a, req, false);
+        r = key_req<RB>(a, key_raw(a, req), false);
+        ahead = key_raw(a, req + 1);
         tile = static_cast<int>(rem % r.tiles);
         const long long q = rem / r.tiles;
         h = static_cast<int>(q % a.Hkv);
@@ -142,19 +154,20 @@ struct KeyWalk {
                 end = unit;
                 return;
             }
-            r = key_req<RB>(a, req, false);
+            r = key_req<RB>(a, ahead, false);
+            ahead = key_raw(a, req + 1);
         } while (r.blocks == 0);
     }
 };
 
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
+__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, RB>::kCtas) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB>;
     constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages, SOFT = S::kSoft;
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
-    extern __shared__ __align__(1024) uint8_t key_raw[];
-    uint8_t* sm = key_raw + ((1024u - (smem_u32(key_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t key_smem[];
+    uint8_t* sm = key_smem + ((1024u - (smem_u32(key_smem) & 1023u)) & 1023u);
     uint8_t* s_q = sm + ST * S::kStage;
     uint8_t* s_p = s_q + S::kQ;
     __shared__ __align__(8) uint64_t full[ST], empty[ST], s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
@@ -194,7 +207,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys
     const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
     unsigned long long mine = 0;
     for (int i = i0; i < i1; ++i) {
-        const KeyReq r = key_req<RB>(a, i, blockIdx.x == 0);
+        const KeyReq r = key_req<RB>(a, key_raw(a, i), blockIdx.x == 0);
         mine += static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
     }
     unsigned long long pre = mine;
@@ -213,14 +226,15 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys
         total += s_sum[w];
     }
     pre += base - mine;  // tiles before this thread's requests
-    const unsigned long long grid = min(static_cast<unsigned long long>(gridDim.x), total);
+    // two tiles per CTA at least: a part costs more to join than a second tile takes
+    const unsigned long long grid = min(static_cast<unsigned long long>(gridDim.x), (total + 1) / 2);
     const bool active = blockIdx.x < grid;
     const long long u0 = active ? static_cast<long long>(total * blockIdx.x / grid) : 0;
     const long long u1 = active ? static_cast<long long>(total * (blockIdx.x + 1) / grid) : 0;
     if (active && static_cast<unsigned long long>(u0) >= pre && static_cast<unsigned long long>(u0) < pre + mine) {
         unsigned long long at = pre;
         for (int i = i0; i < i1; ++i) {
-            const KeyReq r = key_req<RB>(a, i, false);
+            const KeyReq r = key_req<RB>(a, key_raw(a, i), false);
             const unsigned long long c = static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
             if (static_cast<unsigned long long>(u0) < at + c) {
                 s_req = i;
@@ -648,14 +662,12 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys
                         slot[RB * D + RB + r0 + r] = l[r];
                     }
                 }
-                __threadfence();
                 named_bar_sync(1, SOFT);
                 if (tid == 0) {
                     const unsigned parts = static_cast<unsigned>(c_last - c_first + 1);
-                    const unsigned got = atomicAdd(a.counters + c_first, 1u);
+                    const unsigned got = atom_add_acq_rel(a.counters + c_first, 1u);
                     s_last = got + 1 == parts;
                     if (s_last) a.counters[c_first] = 0;
-                    __threadfence();
                 }
                 named_bar_sync(1, SOFT);
                 if (s_last) {
@@ -683,7 +695,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, 1) kv8_attn_keys
                             ll = fmaf(__ldcg(p + RB + r), f, ll);
                         }
                         named_bar_sync(1, SOFT);
-#pragma unroll 4
+#pragma unroll 8
                         for (int c = 0; c < nc; ++c) {
                             const float4* p = reinterpret_cast<const float4*>(part_of(c_first + c0 + c));
 #pragma unroll
@@ -759,7 +771,7 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
         if (e != cudaSuccess) return e;
         if (dev < 64) ready[dev] = true;
     }
-    kv8_attn_keys_kernel<T, D, RB><<<num_sms, S::kThreads, S::kSmem, s>>>(ka);
+    kv8_attn_keys_kernel<T, D, RB><<<num_sms * S::kCtas, S::kThreads, S::kSmem, s>>>(ka);
     return cudaGetLastError();
 }
 
@@ -783,6 +795,6 @@ cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f3
                 : launch_keys_d<__nv_bfloat16, 8>(ka, c->head_dim, num_sms, dev, s);
 }
 
-size_t kv8_keys_part_floats(int D, int num_sms) { return static_cast<size_t>(num_sms) * 2 * 16 * (D + 2); }
+size_t kv8_keys_part_floats(int D, int num_sms) { return static_cast<size_t>(num_sms) * 2 * 2 * 16 * (D + 2); }
 
 }  // namespace dm

@@ -89,6 +89,14 @@ DM_DEV float ex2(float x) {
     return y;
 }
 
+// Counts an arrival: what the CTA wrote before its last barrier is visible to whoever sees the
+// count, and what the others wrote before theirs to this CTA after its next barrier.
+DM_DEV unsigned atom_add_acq_rel(unsigned* p, unsigned v) {
+    unsigned old;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
+}
+
 // Barrier over `count` threads that also ORs a predicate.
 DM_DEV bool named_bar_or(int id, int count, bool v) {
     uint32_t r;
