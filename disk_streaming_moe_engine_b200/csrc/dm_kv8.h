@@ -24,6 +24,10 @@ struct Kv8Device {
 
 int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t es);
 
+inline bool kv8_aligned16(const void* p, int64_t stride_a, int64_t stride_b, int elem) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_a * elem % 16 == 0 && stride_b * elem % 16 == 0;
+}
+
 // Attention over the cache, as the kernels see it.
 struct Kv8AttnArgs {
     const uint8_t* pages;
@@ -40,11 +44,16 @@ struct Kv8AttnArgs {
     int64_t q_rs, q_hs, o_rs, o_hs;  // strides in elements
     float scale_log2;     // sm_scale * log2(e)
     int n, rows, Hq, Hkv, group, num_pages, width, max_q;
+    int q_vec, o_vec;     // q / out: pointer and strides are multiples of 16 bytes
 };
 
 // dm_kv8_keys.cu: any row count and type, one or two CTAs per SM.  Workspace: counters [2 num_sms], then
 // the partials' floats.
 cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f32, int num_sms, int dev, cudaStream_t s);
 size_t kv8_keys_part_floats(int D, int num_sms);
+
+// dm_kv8_queries.cu: bf16, 128 query rows per item.
+cudaError_t launch_kv8_queries(const dm_kv8_cache* c, const Kv8AttnArgs& a, int num_sms, int dev, cudaStream_t s);
+size_t kv8_queries_part_floats(int D, int num_sms);
 
 }  // namespace dm

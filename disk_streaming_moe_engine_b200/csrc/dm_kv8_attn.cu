@@ -9,7 +9,8 @@ namespace dm {
 // Workspace: a counter per CTA, two per SM at most (zero between calls), then the partial results.
 static size_t counter_bytes(int num_sms) { return (static_cast<size_t>(2 * num_sms) * sizeof(unsigned) + 255) / 256 * 256; }
 static size_t workspace_bytes(int D, int num_sms) {
-    return counter_bytes(num_sms) + kv8_keys_part_floats(D, num_sms) * sizeof(float);
+    const size_t k = kv8_keys_part_floats(D, num_sms), q = kv8_queries_part_floats(D, num_sms);
+    return counter_bytes(num_sms) + (k > q ? k : q) * sizeof(float);
 }
 
 }  // namespace dm
@@ -79,8 +80,15 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     a.max_q = static_cast<int>(p->max_q_len);
     a.counters = static_cast<unsigned*>(p->workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + counter_bytes(g.num_sms));
-    const cudaError_t e =
-        launch_kv8_keys(c, a, p->dtype == DM_DTYPE_F32, g.num_sms, g.dev, static_cast<cudaStream_t>(stream));
+    const bool f32 = p->dtype == DM_DTYPE_F32;
+    const int elem = f32 ? 4 : 2;
+    a.q_vec = kv8_aligned16(a.q, a.q_rs, a.q_hs, elem);
+    a.o_vec = kv8_aligned16(a.out, a.o_rs, a.o_hs, elem);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // many bf16 rows per request and kv head: queries on the M side
+    const bool many = !f32 && static_cast<int64_t>(a.max_q) * a.group >= 64;
+    const cudaError_t e = many ? launch_kv8_queries(c, a, g.num_sms, g.dev, s)
+                               : launch_kv8_keys(c, a, f32, g.num_sms, g.dev, s);
     if (e != cudaSuccess)
         return kv8_err(eb, es, e == cudaErrorInvalidValue ? DM_ERR_INVALID_ARG : DM_ERR_CUDA, "CUDA_ERROR", st,
                        "launch: %s", cudaGetErrorString(e));

@@ -31,12 +31,10 @@
 // leaves and copies and MMAs in flight are waited for.
 #include <cmath>
 
-#include "dm_kv8_tc.cuh"
+#include "dm_kv8_walk.cuh"
 
 namespace dm {
 
-constexpr int kKeyTile = 128;
-constexpr int kKeyPages = kKeyTile / kKv8Page;
 constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its CTAs
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
@@ -71,97 +69,9 @@ struct KeyArgs {
     Kv8AttnArgs a;
 };
 
-// What a role knows of the request it is at.
-struct KeyReq {
-    int row0, m, len, full, blocks, tiles;
-};
-
-struct KeyRaw {  // a request's words as loaded
-    int c0, c1, len;
-};
-DM_DEV KeyRaw key_raw(const Kv8AttnArgs& a, int i) {
-    KeyRaw w = {i, i + 1, 0};
-    if (i >= a.n) return w;
-    if (a.cu_q) w.c0 = a.cu_q[i], w.c1 = a.cu_q[i + 1];
-    w.len = a.seq_lens[i];
-    return w;
-}
-
-template <int RB>
-DM_DEV KeyReq key_req(const Kv8AttnArgs& a, const KeyRaw& w, bool report) {
-    KeyReq r;
-    r.row0 = w.c0;
-    const long long m = static_cast<long long>(w.c1) - w.c0;
-    if (w.c0 < 0 || m < 0 || m > a.max_q || w.c0 + m > a.rows) {
-        if (report) raise_error(a.err, DM_DEVERR_RANGE);
-        r.m = 0;
-    } else {
-        r.m = static_cast<int>(m);
-    }
-    r.full = w.len;
-    if (r.full < 0) {
-        if (report) raise_error(a.err, DM_DEVERR_RANGE);
-        r.full = 0;
-    }
-    r.len = r.full;
-    if (r.len > a.width * kKv8Page) {
-        if (report) raise_error(a.err, DM_DEVERR_CAPACITY);
-        r.len = a.width * kKv8Page;
-    }
-    r.blocks = static_cast<int>((static_cast<long long>(r.m) * a.group + RB - 1) / RB);
-    r.tiles = max(1, (r.len + kKeyTile - 1) / kKeyTile);
-    return r;
-}
-
-// keys that a block's rows see: every row those before lo, its last token's rows those before hi
-template <int RB>
-DM_DEV void key_limits(const Kv8AttnArgs& a, const KeyReq& r, int blk, int& lo, int& hi) {
-    const int rows = r.m * a.group;
-    const int first = blk * RB / a.group, last = (min(rows, (blk + 1) * RB) - 1) / a.group;
-    lo = min(r.len, max(0, r.full - r.m + first + 1));
-    hi = min(r.len, max(0, r.full - r.m + last + 1));
-}
-
-// Position in the sequence of all items' tiles: request, then row block, kv head, tile.
-template <int RB>
-struct KeyWalk {
-    const Kv8AttnArgs& a;
-    long long unit, end;  // this CTA's range
-    int req, blk, h, tile;
-    KeyReq r;
-    KeyRaw ahead;  // of request req + 1, loaded before it is needed
-    DM_DEV KeyWalk(const Kv8AttnArgs& args, long long u0, long long u1, int rq, long long rem) : a(args), unit(u0), end(u1) {
-        req = rq;
-        r = key_req<RB>(a, key_raw(a, req), false);
-        ahead = key_raw(a, req + 1);
-        tile = static_cast<int>(rem % r.tiles);
-        const long long q = rem / r.tiles;
-        h = static_cast<int>(q % a.Hkv);
-        blk = static_cast<int>(q / a.Hkv);
-    }
-    // tiles of the current item in the range: [tile, tile + count) of the sequence
-    DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(r.tiles - tile), end - unit)); }
-    DM_DEV void next(int cnt) {
-        unit += cnt;
-        if (unit >= end) return;
-        tile = 0;
-        if (++h < a.Hkv) return;
-        h = 0;
-        if (++blk < r.blocks) return;
-        blk = 0;
-        do {
-            if (++req >= a.n) {  // only if the lengths changed under the kernel
-                end = unit;
-                return;
-            }
-            r = key_req<RB>(a, ahead, false);
-            ahead = key_raw(a, req + 1);
-        } while (r.blocks == 0);
-    }
-};
-
 template <typename T, int D, int RB>
-__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, RB>::kCtas) kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
+__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, RB>::kCtas)
+    kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB>;
     constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages, SOFT = S::kSoft;
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
@@ -175,9 +85,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
     __shared__ float s_red[4][RB], s_fac[32][RB];
-    __shared__ unsigned long long s_sum[NT / 32 + 1];
-    __shared__ long long s_rem;
-    __shared__ unsigned long long s_total;
+    __shared__ long long s_sum[NT / 32], s_rem;
     __shared__ uint32_t s_tmem;
     __shared__ int s_req, s_abort;
     __shared__ uint8_t s_nan[kKeyTile];
@@ -202,136 +110,15 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     }
     if (warp == W_MMA) tc_alloc(&s_tmem, S::kCols);
 
-    // this CTA's range of the tile sequence: block-wide sums of the requests' tiles
-    const int per = (a.n + NT - 1) / NT;
-    const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-    unsigned long long mine = 0;
-    for (int i = i0; i < i1; ++i) {
-        const KeyReq r = key_req<RB>(a, key_raw(a, i), blockIdx.x == 0);
-        mine += static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
-    }
-    unsigned long long pre = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, pre, o);
-        if (lane >= o) pre += y;
-    }
-    if (lane == 31) s_sum[warp] = pre;
     tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    unsigned long long base = 0, total = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) base += s_sum[w];
-        total += s_sum[w];
-    }
-    pre += base - mine;  // tiles before this thread's requests
+    long long u0, u1, total, grid;
     // two tiles per CTA at least: a part costs more to join than a second tile takes
-    const unsigned long long grid = min(static_cast<unsigned long long>(gridDim.x), (total + 1) / 2);
-    const bool active = blockIdx.x < grid;
-    const long long u0 = active ? static_cast<long long>(total * blockIdx.x / grid) : 0;
-    const long long u1 = active ? static_cast<long long>(total * (blockIdx.x + 1) / grid) : 0;
-    if (active && static_cast<unsigned long long>(u0) >= pre && static_cast<unsigned long long>(u0) < pre + mine) {
-        unsigned long long at = pre;
-        for (int i = i0; i < i1; ++i) {
-            const KeyReq r = key_req<RB>(a, key_raw(a, i), false);
-            const unsigned long long c = static_cast<unsigned long long>(r.blocks) * a.Hkv * r.tiles;
-            if (static_cast<unsigned long long>(u0) < at + c) {
-                s_req = i;
-                s_rem = static_cast<long long>(u0 - at);
-                break;
-            }
-            at += c;
-        }
-    }
-    __syncthreads();
+    const bool active = key_range<RB, NT>(a, 2, s_sum, &s_req, &s_rem, u0, u1, total, grid);
+    tc_fence_after();
     const uint32_t tmem = s_tmem;
 
     if (active && warp == W_LOAD) {
-        // ---------------- producer: groups of 4 tiles, a lane per page ----------------
-        // Page ids are fetched two groups ahead of their use, scales one group ahead.
-        uint32_t use = 0;  // tiles issued
-        bool ok = true;
-        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
-        int ti = -1, ei = 0, hi = 0;  // next tile of w's item, end of its tiles, its keys
-        struct Group {
-            int count = 0;             // tiles
-            int id = -1, h = 0;        // this lane's page (tile lane / 8, page lane % 8) and kv head
-            bool wanted = false;       // a key of the item lies on it
-            float2 sc = make_float2(0.0f, -1.0f);
-        };
-        auto fetch_ids = [&](Group& g) {
-            g = Group();
-            while (g.count < 32 / kKeyPages && w.unit < w.end) {
-                if (ti < 0) {
-                    int lo;
-                    key_limits<RB>(a, w.r, w.blk, lo, hi);
-                    ti = w.tile;
-                    ei = min(w.tile + w.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
-                }
-                if (ti < ei) {
-                    const int p = ti * kKeyPages + lane % kKeyPages;
-                    if (lane / kKeyPages == g.count) {
-                        g.h = w.h;
-                        g.wanted = p * kKv8Page < hi;
-                        if (g.wanted) g.id = a.table[static_cast<size_t>(w.req) * a.width + p];
-                    }
-                    ++g.count;
-                    ++ti;
-                } else {
-                    w.next(w.count());
-                    ti = -1;
-                }
-            }
-        };
-        auto fetch_scales = [&](Group& g) {
-            if (!g.wanted) return;
-            if (g.id >= 0 && g.id < a.num_pages) {
-                const float* sc = a.scales + static_cast<size_t>(g.id) * 2 * a.Hkv + g.h;
-                g.sc = make_float2(sc[0], sc[a.Hkv]);
-            } else {
-                raise_error(a.err, DM_DEVERR_PAGE);
-            }
-        };
-        Group g0, g1, g2;
-        fetch_ids(g0);
-        fetch_ids(g1);
-        fetch_scales(g0);
-        while (g0.count > 0 && ok) {
-            fetch_ids(g2);
-            fetch_scales(g1);
-            for (int k = 0; k < g0.count; ++k) {
-                const uint32_t si = use % ST, ph = (use / ST) & 1u;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
-                    ok = false;
-                    break;
-                }
-                const bool mine = lane / kKeyPages == k;
-                const int pg = lane % kKeyPages;
-                if (lane == 0) mbar_arrive_expect_tx(&full[si], S::kStage);
-                __syncwarp();
-                if (mine) {
-                    const int page = g0.id >= 0 && g0.id < a.num_pages ? g0.id : a.num_pages;
-                    const uint32_t kt = smem_u32(sm + si * S::kStage) + pg * (kKv8Page * CW);
-#pragma unroll
-                    for (int c = 0; c < S::kChunks; ++c)
-                        tma_load_3d(kt + c * (kKeyTile * CW), &ka.map, c * CW, g0.h * kKv8Page, page, &full[si]);
-#pragma unroll
-                    for (int c = 0; c < S::kChunks; ++c)
-                        tma_load_3d(kt + S::kTileBytes + c * (kKeyTile * CW), &ka.map, c * CW, (a.Hkv + g0.h) * kKv8Page,
-                                    page, &full[si]);
-                    s_meta[si][pg] = g0.sc;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[si]);
-                ++use;
-            }
-            g0 = g1;
-            g1 = g2;
-        }
-        if (lane == 0)
-            for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
-                mbar_wait_bounded(&full[u % ST], (u / ST) & 1u, a.err, nullptr);
+        key_produce<RB, D, ST>(a, &ka.map, sm, full, empty, s_meta, u0, u1, s_req, s_rem, abort_flag);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
@@ -354,7 +141,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
             KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
             while (w.unit < w.end && ok) {
                 int lo, hi;
-                key_limits<RB>(a, w.r, w.blk, lo, hi);
+                key_limits<RB>(a, w.r, w.block(), lo, hi);
                 const int cnt = w.count();
                 const int nt = min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) - w.tile;
                 if (nt > 0) {
@@ -371,7 +158,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                         const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
-                            const uint64_t ad = f8_desc_m<CW>(v + c * (kKeyTile * CW));
+                            const uint64_t ad = f8_desc_m<CW>(v + c * (kKeyTile * CW), 0);  // 64 wide: M rows 64-127 repeat 0-63
 #pragma unroll
                             for (int j = 0; j < kKeyTile / 32; ++j)
                                 f8_mma(tmem + (2 + c) * N, ad + j * (32 * CW / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
@@ -395,7 +182,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
         KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
         while (w.unit < w.end && ok) {
             int lim_min, lim_max;
-            key_limits<RB>(a, w.r, w.blk, lim_min, lim_max);
+            key_limits<RB>(a, w.r, w.block(), lim_min, lim_max);
             const int cnt = w.count();
             const int real = max(1, (lim_max + kKeyTile - 1) / kKeyTile);  // tiles of the item
             const int t_begin = w.tile, nt = min(w.tile + cnt, real) - w.tile;
@@ -403,11 +190,11 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                 w.next(cnt);
                 continue;
             }
-            const int nrow = min(RB, w.r.m * a.group - w.blk * RB);
+            const int nrow = min(RB, w.r.m * a.group - w.block() * RB);
             {   // Q terms: 16 threads per row
                 constexpr int E = D / 16;
                 const int r = tid / 16, e0 = (tid % 16) * E;
-                const int f = w.blk * RB + min(r, nrow - 1);
+                const int f = w.block() * RB + min(r, nrow - 1);
                 const int tok = f / a.group, head = w.h * a.group + f % a.group;
                 const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(w.r.row0 + tok) * a.q_rs +
                              static_cast<int64_t>(head) * a.q_hs + e0;
@@ -616,14 +403,12 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
 
             const long long item0 = w.unit - t_begin;  // the item's first tile in the sequence
             const bool whole = t_begin == 0 && nt == real;
-            const long long tot = static_cast<long long>(total), gr = static_cast<long long>(grid);
-            const int c_first = static_cast<int>(((item0 + 1) * gr - 1) / tot);
-            const int c_last = static_cast<int>(((item0 + real) * gr - 1) / tot);
+            const int c_first = key_owner(item0, total, grid), c_last = key_owner(item0 + real - 1, total, grid);
             constexpr int kSlot = (RB * (D + 2) + 3) / 4 * 4;
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
             auto put = [&](int r, int d, float o, float mm, float ll) {
                 if (r >= nrow) return;
-                const int f = w.blk * RB + r;
+                const int f = w.block() * RB + r;
                 const int64_t row = w.r.row0 + f / a.group;
                 const int head = w.h * a.group + f % a.group;
                 // a row that saw no key keeps the reference -inf

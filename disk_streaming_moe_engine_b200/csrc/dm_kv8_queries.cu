@@ -1,0 +1,550 @@
+// dm_kv8_queries.cu — attention over the 8-bit paged cache with the queries on the tensor
+// cores' M side: prompts and chunks of many bf16 query rows.
+//
+// Work: an item is 128 query rows (a row = one query token and one query head; the heads of a
+// group share their keys, so a group's rows go together) of one request and kv head; its keys
+// come in tiles of 128 tokens.  Per tile, on tcgen05 with e4m3 operands straight from the cache:
+//   S [128 x 128] = (Q0 + Q1) [128 x D] . codeK^T,   O [128 x D] += (P0 + P1) [128 x 128] . codeV
+// q and the weights are sums of two e4m3 terms of one scale, so both products of a pair add into
+// one accumulator at the cost of one bf16 product (e4m3 runs at twice its rate), and the cache
+// needs no conversion.  bf16's 8 bits fit two terms: q, scaled to a largest magnitude in
+// [2^7, 2^8) per row, is exact down to 2^-10 of it and off by 2^-18 of it at most; a weight is
+// off by 2^-8 of itself or 2^-16 of the row's largest.
+//
+// Softmax as in the key-side kernel: y = x + v - M in log2 units with the page's sV = 2^v folded
+// in, M raised when some y exceeds 2, o = sum w codeV / sum w 2^-v.  A row belongs to two
+// threads, 64 keys of the tile each, that meet at a 64-thread barrier to agree on M; O is
+// rescaled only by warps with a raised row.
+//
+// Roles (384 threads): 8 softmax warps (two per quarter of the rows), 2 warps that turn the next
+// item's q rows into terms as soon as its predecessor's last scores are done, a producer and an
+// MMA warp.  The scores of tile x + 1 follow as soon as those of tile x are in registers and run
+// before the O product of tile x, so the softmax has the time of two products.  Tensor memory: the
+// scores (128 columns), two buffers of weights (64), O (D).  Split of the work, joins and
+// bounded waits as in the key-side kernel; after a failed wait every thread runs through the
+// remaining barriers without work.
+#include <cmath>
+
+#include "dm_kv8_walk.cuh"
+
+namespace dm {
+
+constexpr int kQryRows = 128;
+constexpr int kQrySoft = 256;
+constexpr int kQryThreads = kQrySoft + 64 + 64;
+constexpr float kQryLazy = 2.0f;
+constexpr float kQryBoost = 6.0f;  // weights enter as 2^6 w <= 256
+
+template <int D>
+struct QryShape {
+    static constexpr int CW = D >= 128 ? 128 : D;
+    static constexpr int kChunks = D / CW;
+    static constexpr int kTileBytes = kKeyTile * D;
+    static constexpr int kStage = 2 * kTileBytes;
+    static constexpr int kTerm = kQryRows * D;  // one term of Q
+    static constexpr int kFixed = 2 * kTerm + 1024;
+    static constexpr int kFit = (227 * 1024 - 6144 - kFixed) / kStage;
+    static constexpr int kStages = kFit > 6 ? 6 : kFit;
+    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kFixed;
+    static_assert(kStages >= 2, "shape");
+};
+
+struct QryArgs {
+    CUtensorMap map;
+    Kv8AttnArgs a;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const __grid_constant__ QryArgs qa) {
+    using S = QryShape<D>;
+    constexpr int CW = S::CW, ST = S::kStages, RB = kQryRows;
+    constexpr uint32_t kPw = 128, kO = 256;  // tensor memory columns: scores, weights (two buffers of 64), O
+    const Kv8AttnArgs& a = qa.a;
+    extern __shared__ __align__(1024) uint8_t qry_smem[];
+    uint8_t* sm = qry_smem + ((1024u - (smem_u32(qry_smem) & 1023u)) & 1023u);
+    uint8_t* s_q = sm + ST * S::kStage;
+    __shared__ __align__(8) uint64_t full[ST], empty[ST], s_full, s_free, p_ready[2], pv_done[2], q_ready, q_free, done_bar;
+    __shared__ float2 s_meta[ST][kKeyPages];
+    __shared__ float s_frow[RB], s_max[2][RB], s_l[2][RB];
+    __shared__ int s_lim[RB];
+    __shared__ long long s_sum[kQryThreads / 32], s_rem;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_req, s_abort;
+    __shared__ uint8_t s_nan[kKeyTile];
+    __shared__ unsigned s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* abort_flag = &s_abort;
+    constexpr int W_Q = 8, W_LOAD = 10, W_MMA = 11;
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&full[i], 2);  // the copies, and the scales
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&p_ready[i], kQrySoft);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(&s_full, 1);
+        mbar_init(&s_free, kQrySoft);
+        mbar_init(&q_ready, 64);
+        mbar_init(&q_free, kQrySoft + 1);  // its score products are done, its scales and limits read
+        mbar_init(&done_bar, 1);
+        mbar_fence_init();
+        s_abort = 0;
+    }
+    if (warp == W_MMA) tc_alloc(&s_tmem, 512);
+    tc_fence_before();
+    long long u0, u1, total, grid;
+    // a part of 128 rows is costly to join: four tiles per CTA at least
+    const bool active = key_range<RB, kQryThreads>(a, 4, s_sum, &s_req, &s_rem, u0, u1, total, grid);
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    if (active && warp == W_LOAD) {
+        key_produce<RB, D, ST>(a, &qa.map, sm, full, empty, s_meta, u0, u1, s_req, s_rem, abort_flag);
+    } else if (active && warp == W_MMA) {
+        // ---------------- MMA ----------------
+        if (lane == 0) {
+            bool ok = true;
+            const uint32_t i_s = f8_idesc(128, kKeyTile, false, false), i_o = f8_idesc(128, D, false, true);
+            const uint32_t sq = smem_u32(s_q);
+            // scores run one tile ahead of the O products, across items too
+            KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+            uint32_t x = 0, sx = 0, item = 0;
+            int left = 0;         // score tiles left of the walked item
+            unsigned firsts = 0;  // bit (x & 1): tile x is its item's first
+            auto next_scores = [&]() -> bool {
+                bool first = false;
+                while (left == 0) {
+                    if (w.unit >= w.end) return false;
+                    int lo, hi;
+                    key_limits<RB>(a, w.r, w.block(), lo, hi);
+                    const int cnt = w.count();
+                    left = max(0, min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) - w.tile);
+                    w.next(cnt);
+                    first = left > 0;
+                }
+                if (first && !(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) return false;
+                if (!(ok = mbar_wait_bounded(&full[sx % ST], (sx / ST) & 1u, a.err, abort_flag))) return false;
+                if (!(ok = mbar_wait_bounded(&s_free, (sx & 1u) ^ 1u, a.err, abort_flag))) return false;
+                tc_fence_after();
+                const uint32_t k = smem_u32(sm + (sx % ST) * S::kStage);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int c = 0; c < S::kChunks; ++c) {
+                        const uint64_t ad = f8_desc_k<CW>(sq + t * S::kTerm + c * (RB * CW));
+                        const uint64_t bd = f8_desc_k<CW>(k + c * (kKeyTile * CW));
+#pragma unroll
+                        for (int j = 0; j < CW / 32; ++j)
+                            f8_mma(tmem, ad + 2 * j, bd + 2 * j, i_s, t > 0 || c > 0 || j > 0);
+                    }
+                tc_commit(&s_full);
+                firsts = (firsts & ~(1u << (sx & 1u))) | ((first ? 1u : 0u) << (sx & 1u));
+                ++sx;
+                if (--left == 0) {
+                    tc_commit(&q_free);
+                    ++item;
+                }
+                return true;
+            };
+            bool more = next_scores();
+            while (more && ok) {
+                more = next_scores();
+                if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
+                tc_fence_after();
+                const bool first = (firsts >> (x & 1u)) & 1u;
+                const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (x % ST) * S::kStage) + S::kTileBytes, kKeyTile * CW);
+                const uint32_t p = tmem + kPw + (x & 1u) * 64;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < kKeyTile / 32; ++j)
+                        f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o,
+                                  !first || t > 0 || j > 0);
+                tc_commit(&empty[x % ST]);
+                tc_commit(&pv_done[x & 1u]);
+                ++x;
+            }
+            tc_commit(&done_bar);
+            mbar_wait_bounded(&done_bar, 0, a.err, nullptr);
+        }
+    } else if (active && warp >= W_Q) {
+        // ---------------- Q terms: a quarter-warp per row, 8 elements per access ----------------
+        uint32_t item = 0;
+        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        while (w.unit < w.end) {
+            int lo, hi;
+            key_limits<RB>(a, w.r, w.block(), lo, hi);
+            const int cnt = w.count();
+            if (min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) <= w.tile) {
+                w.next(cnt);
+                continue;
+            }
+            const int rows = w.r.m * a.group, nrow = min(RB, rows - w.block() * RB);
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&q_free, (item & 1u) ^ 1u, a.err, abort_flag))) break;
+            constexpr int P = D / 64;  // accesses of a lane and row
+#pragma unroll 2
+            for (int i = 0; i < 16; ++i) {
+                const int r = (warp - W_Q) * 64 + i * 4 + lane / 8;
+                const int f = w.block() * RB + min(r, nrow - 1);
+                const int tok = f / a.group, head = w.h * a.group + f % a.group;
+                const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
+                                         static_cast<int64_t>(w.r.row0 + tok) * a.q_rs + static_cast<int64_t>(head) * a.q_hs;
+                float v[P][8];
+                float amax = 0.0f;
+#pragma unroll
+                for (int c = 0; c < P; ++c) {
+                    const __nv_bfloat16* s = q + c * 64 + (lane % 8) * 8;
+                    if (a.q_vec) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(s);
+                        const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[c][2 * j] = bf16lo(wd[j]), v[c][2 * j + 1] = bf16hi(wd[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[c][j] = static_cast<float>(s[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (r >= nrow) v[c][j] = 0.0f;
+                        if (!(fabsf(v[c][j]) <= 3.402823466e38f)) v[c][j] = __int_as_float(0x7fc00000);
+                        amax = fmaxf(amax, fabsf(v[c][j]));
+                    }
+                }
+#pragma unroll
+                for (int o = 4; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
+                const float mul = __int_as_float((127 - ex) << 23);
+                if (lane % 8 == 0) {
+                    s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
+                    s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
+                }
+#pragma unroll
+                for (int c = 0; c < P; ++c) {
+                    uint32_t t0[4], t1[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e4m3_terms2(v[c][2 * j] * mul, v[c][2 * j + 1] * mul, t0[j], t1[j]);
+                    const int d = c * 64 + (lane % 8) * 8;
+                    uint8_t* dst = s_q + (d / CW) * (RB * CW) + f8_unit<CW>(r, (d % CW) / 16) + d % 16;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(t0[0] | (t0[1] << 16), t0[2] | (t0[3] << 16));
+                    *reinterpret_cast<uint2*>(dst + S::kTerm) = make_uint2(t1[0] | (t1[1] << 16), t1[2] | (t1[3] << 16));
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&q_ready);
+            ++item;
+            w.next(cnt);
+        }
+    } else if (active) {
+        // ---------------- softmax, epilogue ----------------
+        const int row = tid & 127, half = tid >> 7, wq = warp & 3;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16);
+        uint32_t t = 0, item = 0;
+        bool ok = true;
+        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        while (w.unit < w.end) {
+            int lim_min, lim_max;
+            key_limits<RB>(a, w.r, w.block(), lim_min, lim_max);
+            const int cnt = w.count();
+            const int real = max(1, (lim_max + kKeyTile - 1) / kKeyTile);
+            const int t_begin = w.tile, nt = min(w.tile + cnt, real) - w.tile;
+            if (nt <= 0) {
+                w.next(cnt);
+                continue;
+            }
+            ok = ok && mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag);
+            const int nrow = min(RB, w.r.m * a.group - w.block() * RB);
+            const float frow = s_frow[row];
+            const int lim = s_lim[row];
+            mbar_arrive(&q_free);
+            float mref = -INFINITY, l = 0.0f;
+            bool nan_row = false;
+
+            for (int i = 0; i < nt; ++i) {
+                const uint32_t x = t + i, si = x % ST, pb = kPw + (x & 1u) * 64 + half * 16;
+                const int tile0 = (t_begin + i) * kKeyTile;
+                const bool t1 = mbar_try_wait(&full[si], (x / ST) & 1u);
+                const bool t2 = mbar_try_wait(&s_full, x & 1u);
+                const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
+                if (ok && !(t1 && t2 && t3))
+                    ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag) &&
+                         mbar_wait_bounded(&s_full, x & 1u, a.err, abort_flag) &&
+                         (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
+                __syncwarp();
+                tc_fence_after();
+                float s[64];
+                tc_ld32(lanes + half * 64, s);
+                tc_ld32(lanes + half * 64 + 32, s + 32);
+                // the half's pages: y = s f + g
+                float f[4], g[4], vinv[4];
+                const float base = mref == -INFINITY ? 0.0f : kQryBoost - mref;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const float2 sc = s_meta[si][half * 4 + p];
+                    const int ve = ((__float_as_int(sc.y) >> 23) & 0xff) - 127;
+                    f[p] = frow * sc.x;
+                    g[p] = sc.y < 0.0f ? -INFINITY : static_cast<float>(ve) + base;
+                    vinv[p] = __int_as_float((127 - ve) << 23);
+                }
+                tc_wait_ld();
+                tc_fence_before();
+                mbar_arrive(&s_free);
+                const bool edge = tile0 + kKeyTile > lim_min;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 64; ++c) {
+                    s[c] = fmaf(s[c], f[c / 16], g[c / 16]);
+                    if (g[c / 16] == -INFINITY) s[c] = -INFINITY;
+                }
+                if (edge) {
+                    const int seen = lim - tile0 - half * 64;
+#pragma unroll
+                    for (int c = 0; c < 64; ++c)
+                        if (c >= seen) s[c] = -INFINITY;
+                }
+#pragma unroll
+                for (int c = 0; c < 64; ++c) mx = fmaxf(mx, s[c]);
+                const bool over = mref == -INFINITY ? mx > -INFINITY : mx > kQryBoost + kQryLazy;
+                if (named_bar_or(2 + wq, 64, over)) {
+                    // the row's two threads agree on its reference; O of the raised rows follows
+                    s_max[half][row] = mx;
+                    named_bar_sync(2 + wq, 64);
+                    const float both = fmaxf(s_max[0][row], s_max[1][row]);  // in units of the old reference
+                    named_bar_sync(2 + wq, 64);
+                    const bool raise = mref == -INFINITY ? both > -INFINITY : both > kQryBoost + kQryLazy;
+                    float fac = 1.0f;
+                    if (raise) {
+                        const float nm = mref == -INFINITY ? both : both - kQryBoost + mref;
+                        const float shift = mref == -INFINITY ? kQryBoost - nm : mref - nm;
+                        fac = mref == -INFINITY ? 0.0f : exp2f(shift);
+                        mref = nm;
+                        l *= fac;
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) s[c] += shift;
+                    }
+                    if (__any_sync(0xffffffffu, raise) && i > 0) {
+                        ok = ok && mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
+                        __syncwarp();
+                        tc_fence_after();
+                        // each of the two threads rescales one half of the row's O
+#pragma unroll 1
+                        for (int c = 0; c < D / 2; c += 32) {
+                            float o[32];
+                            tc_ld32(lanes + kO + half * (D / 2) + c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] *= fac;
+                            tc_st32(lanes + kO + half * (D / 2) + c, o);
+                        }
+                        tc_wait_st();
+                    }
+                }
+                // weights, sums, terms: columns of P0 and P1 of this half's 64 keys
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    float sum = 0.0f;
+                    uint32_t p0[4], p1[4];
+#pragma unroll
+                    for (int c = 0; c < 16; c += 4) {
+                        float* y = s + p * 16 + c;
+                        uint32_t a0, a1, b0, b1;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            y[j] = ex2(y[j]);
+                            sum += y[j];
+                        }
+                        e4m3_terms2(y[0], y[1], a0, a1);
+                        e4m3_terms2(y[2], y[3], b0, b1);
+                        p0[c / 4] = a0 | (b0 << 16);
+                        p1[c / 4] = a1 | (b1 << 16);
+                    }
+                    l = fmaf(sum, vinv[p], l);
+                    tc_st4(lanes + pb + p * 4, p0);
+                    tc_st4(lanes + pb + 32 + p * 4, p1);
+                }
+                if (edge) {
+                    // V rows behind the last key become zeros; a NaN code that not every row sees
+                    // becomes 0 and makes the sums of the rows that see it NaN
+                    if (half == 0) {
+                        uint8_t* v = sm + si * S::kStage + S::kTileBytes + row * CW;
+                        const int key = tile0 + row;
+                        bool nan = false;
+                        if (key >= lim_max) {
+#pragma unroll
+                            for (int c = 0; c < S::kChunks; ++c)
+                                for (int u = 0; u < CW / 16; ++u)
+                                    *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
+                        } else if (key >= lim_min) {
+#pragma unroll
+                            for (int c = 0; c < S::kChunks; ++c)
+                                for (int u = 0; u < CW / 4; ++u) {
+                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
+                                    const uint32_t bad = e4m3_nan_mask(*p);
+                                    if (bad) {
+                                        *p &= ~bad;
+                                        nan = true;
+                                    }
+                                }
+                        }
+                        s_nan[row] = nan;
+                        fence_proxy_async_smem();
+                        nan_row = nan;
+                    }
+                    if (named_bar_or(1, kQrySoft, half == 0 && nan_row)) {
+                        nan_row = false;
+                        for (int k = 0; k < kKeyTile; ++k)
+                            if (s_nan[k] && tile0 + k < lim) l = __int_as_float(0x7fc00000);
+                        named_bar_sync(1, kQrySoft);
+                    }
+                    nan_row = false;
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_ready[x & 1u]);
+            }
+            t += nt;
+            ++item;
+            // both halves' sums, then O
+            s_l[half][row] = l;
+            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
+            named_bar_sync(2 + wq, 64);
+            l = s_l[0][row] + s_l[1][row];
+            named_bar_sync(2 + wq, 64);
+            tc_fence_after();
+
+            const long long item0 = w.unit - t_begin;
+            const bool whole = t_begin == 0 && nt == real;
+            constexpr int kSlot = RB * (D + 2);
+            float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
+            const int fq = w.block() * RB + row;
+            const int64_t orow = w.r.row0 + fq / a.group;
+            const int head = w.h * a.group + fq % a.group;
+            const bool live = ok && row < nrow;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + orow * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
+            // 16 consecutive results of this row from element d on
+            auto put16 = [&](const float* o, int d, float inv, bool none) {
+                if (a.o_vec) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 8) {
+                        uint32_t wd[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : o[j + 2 * k] * inv,
+                                                                           none ? 0.0f : o[j + 2 * k + 1] * inv);
+                            wd[k] = *reinterpret_cast<const uint32_t*>(&b);
+                        }
+                        *reinterpret_cast<uint4*>(out + d + j) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) out[d + j] = __float2bfloat16_rn(none ? 0.0f : o[j] * inv);
+                }
+            };
+            auto put_lse = [&](float mm, float ll) {
+                if (a.lse && half == 0)
+                    a.lse[orow * a.Hq + head] = ll == 0.0f ? -INFINITY : (mm - kQryBoost + log2f(ll)) * 0.6931471805599453f;
+            };
+            const float inv = 1.0f / l;
+            const bool none = mref == -INFINITY && l == 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 32) {
+                const int d = half * (D / 2) + c;
+                float o[32];
+                tc_ld32(lanes + kO + d, o);
+                tc_wait_ld();
+                if (whole) {
+                    if (live) {
+                        put16(o, d, inv, none);
+                        put16(o + 16, d + 16, inv, none);
+                    }
+                } else if (ok) {
+                    // element-major, so that a warp's stores are contiguous
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) slot[(d + j) * RB + row] = o[j];
+                }
+            }
+            tc_fence_before();
+            if (whole) {
+                if (live) put_lse(mref, l);
+            } else {
+                if (half == 0 && ok) {
+                    slot[RB * D + row] = mref;
+                    slot[RB * D + RB + row] = l;
+                }
+                const int c_first = key_owner(item0, total, grid), c_last = key_owner(item0 + real - 1, total, grid);
+                if (!named_bar_or(1, kQrySoft, !ok)) {
+                    if (tid == 0) {
+                        const unsigned got = atom_add_acq_rel(a.counters + c_first, 1u);
+                        s_last = got + 1 == static_cast<unsigned>(c_last - c_first + 1);
+                        if (s_last) a.counters[c_first] = 0;
+                    }
+                    named_bar_sync(1, kQrySoft);
+                    if (s_last) {
+                        auto part_of = [&](int c) {
+                            return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
+                        };
+                        float mm = -INFINITY, ll = 0.0f;
+                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + row));
+                        for (int c = c_first; c <= c_last; ++c) {
+                            const float* p = part_of(c) + RB * D + row;
+                            const float mc = __ldcg(p);
+                            ll = fmaf(__ldcg(p + RB), mc == mm ? 1.0f : exp2f(mc - mm), ll);
+                        }
+                        const float linv = 1.0f / ll;
+#pragma unroll 1
+                        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
+                            float o[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+                            for (int c = c_first; c <= c_last; ++c) {
+                                const float* p = part_of(c);
+                                const float mc = __ldcg(p + RB * D + row);
+                                const float fc = mc == mm ? 1.0f : exp2f(mc - mm);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = fmaf(__ldcg(p + (d + j) * RB + row), fc, o[j]);
+                            }
+                            if (live) put16(o, d, linv, mm == -INFINITY && ll == 0.0f);
+                        }
+                        if (live) put_lse(mm, ll);
+                    }
+                }
+            }
+            w.next(cnt);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        tc_dealloc(tmem, 512);
+    }
+}
+
+template <int D>
+static cudaError_t launch_queries(const QryArgs& qa, int num_sms, int dev, cudaStream_t s) {
+    using S = QryShape<D>;
+    static bool ready[64] = {};
+    if (dev >= 64 || !ready[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kv8_attn_queries_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(S::kSmem));
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready[dev] = true;
+    }
+    kv8_attn_queries_kernel<D><<<num_sms, kQryThreads, S::kSmem, s>>>(qa);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv8_queries(const dm_kv8_cache* c, const Kv8AttnArgs& a, int num_sms, int dev, cudaStream_t s) {
+    QryArgs qa{};
+    if (!kv8_encode_map(c, &qa.map)) return cudaErrorNotSupported;
+    qa.a = a;
+    if (c->head_dim == 64) return launch_queries<64>(qa, num_sms, dev, s);
+    if (c->head_dim == 128) return launch_queries<128>(qa, num_sms, dev, s);
+    return launch_queries<256>(qa, num_sms, dev, s);
+}
+
+size_t kv8_queries_part_floats(int D, int num_sms) { return static_cast<size_t>(num_sms) * 2 * kQryRows * (D + 2); }
+
+}  // namespace dm

@@ -24,12 +24,12 @@ DM_DEV uint64_t f8_desc_k(uint32_t addr) {
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(8 * CW / 16) << 32) |
            kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
 }
-// M-major operand: 8-token groups 8 CW bytes apart (stride byte offset); the second CW
-// elements of M (CW = 64 only) at leading byte offset 0, i.e. M rows 64-127 repeat rows 0-63.
+// M- or N-major operand: 8-token groups 8 CW bytes apart (stride byte offset), the next CW
+// elements of M or N `chunk` bytes on (leading byte offset; 0 repeats the first CW elements).
 template <int CW>
-DM_DEV uint64_t f8_desc_m(uint32_t addr) {
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(8 * CW / 16) << 32) | kDescVersion |
-           (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
+DM_DEV uint64_t f8_desc_m(uint32_t addr, uint32_t chunk) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(chunk / 16) << 16) |
+           (static_cast<uint64_t>(8 * CW / 16) << 32) | kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
 }
 // N-major operand without swizzle: per 16 N columns a block of 16-byte rows, one per K;
 // 8-row groups 128 bytes apart (leading byte offset), blocks `block` bytes apart (stride).
@@ -51,6 +51,17 @@ DM_DEV void f8_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t i
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+// The same with A in tensor memory: row m in lane m, four consecutive K elements per 32-bit
+// column, 8 columns per K = 32 step.
+DM_DEV void f8_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
 
@@ -81,6 +92,15 @@ DM_DEV uint32_t e4m3_round2(float a, float b, float2& back) {
 }
 // 0xff in the bytes of w that hold a NaN code
 DM_DEV uint32_t e4m3_nan_mask(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+// e4m3 terms of two values: the nearest codes, and those of what they leave (as they are, no
+// scaling), through fp16 (11 bits, twice what the two terms hold)
+DM_DEV void e4m3_terms2(float a, float b, uint32_t& t0, uint32_t& t1) {
+    const __half2 h = __floats2half2_rn(a, b);
+    t0 = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E4M3);
+    const __half2 back(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(t0), __NV_E4M3));
+    t1 = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(__hsub2(h, back)), __NV_SATFINITE, __NV_E4M3);
+}
 
 // 2^x of the special function unit (relative error 2^-22; results below 2^-126 become 0)
 DM_DEV float ex2(float x) {

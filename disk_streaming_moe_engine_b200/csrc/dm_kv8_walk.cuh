@@ -1,0 +1,250 @@
+// dm_kv8_walk.cuh — what the attention kernels over the 8-bit cache share: the sequence of
+// (request, row block, kv head, key tile), its cut into one range per CTA, and the producer that
+// brings a range's key tiles into shared memory.
+#pragma once
+#include "dm_kv8_tc.cuh"
+
+namespace dm {
+
+constexpr int kKeyTile = 128;  // keys of a tile
+constexpr int kKeyPages = kKeyTile / kKv8Page;
+
+// What a role knows of the request it is at.
+struct KeyReq {
+    int row0, m, len, full, blocks, tiles;
+};
+
+struct KeyRaw {  // a request's words as loaded
+    int c0, c1, len;
+};
+DM_DEV KeyRaw key_raw(const Kv8AttnArgs& a, int i) {
+    KeyRaw w = {i, i + 1, 0};
+    if (i >= a.n) return w;
+    if (a.cu_q) w.c0 = a.cu_q[i], w.c1 = a.cu_q[i + 1];
+    w.len = a.seq_lens[i];
+    return w;
+}
+
+template <int RB>
+DM_DEV KeyReq key_req(const Kv8AttnArgs& a, const KeyRaw& w, bool report) {
+    KeyReq r;
+    r.row0 = w.c0;
+    const long long m = static_cast<long long>(w.c1) - w.c0;
+    if (w.c0 < 0 || m < 0 || m > a.max_q || w.c0 + m > a.rows) {
+        if (report) raise_error(a.err, DM_DEVERR_RANGE);
+        r.m = 0;
+    } else {
+        r.m = static_cast<int>(m);
+    }
+    r.full = w.len;
+    if (r.full < 0) {
+        if (report) raise_error(a.err, DM_DEVERR_RANGE);
+        r.full = 0;
+    }
+    r.len = r.full;
+    if (r.len > a.width * kKv8Page) {
+        if (report) raise_error(a.err, DM_DEVERR_CAPACITY);
+        r.len = a.width * kKv8Page;
+    }
+    r.blocks = static_cast<int>((static_cast<long long>(r.m) * a.group + RB - 1) / RB);
+    r.tiles = max(1, (r.len + kKeyTile - 1) / kKeyTile);
+    return r;
+}
+
+// keys that a block's rows see: every row those before lo, its last token's rows those before hi
+template <int RB>
+DM_DEV void key_limits(const Kv8AttnArgs& a, const KeyReq& r, int blk, int& lo, int& hi) {
+    const int rows = r.m * a.group;
+    const int first = blk * RB / a.group, last = (min(rows, (blk + 1) * RB) - 1) / a.group;
+    lo = min(r.len, max(0, r.full - r.m + first + 1));
+    hi = min(r.len, max(0, r.full - r.m + last + 1));
+}
+
+// Position in the sequence of all items' tiles: request, then row block (first, last, second,
+// second to last, ...: under a causal mask neighbours then cost the same together), kv head,
+// tile.  Every block has the tiles of the request's whole length there; those that its rows do
+// not see are skipped.
+template <int RB>
+struct KeyWalk {
+    const Kv8AttnArgs& a;
+    long long unit, end;  // this CTA's range
+    int req, blk, h, tile;
+    KeyReq r;
+    KeyRaw ahead;  // of request req + 1, loaded before it is needed
+    DM_DEV KeyWalk(const Kv8AttnArgs& args, long long u0, long long u1, int rq, long long rem) : a(args), unit(u0), end(u1) {
+        req = rq;
+        r = key_req<RB>(a, key_raw(a, req), false);
+        ahead = key_raw(a, req + 1);
+        tile = static_cast<int>(rem % r.tiles);
+        const long long q = rem / r.tiles;
+        h = static_cast<int>(q % a.Hkv);
+        blk = static_cast<int>(q / a.Hkv);
+    }
+    DM_DEV int block() const { return blk & 1 ? r.blocks - 1 - (blk >> 1) : blk >> 1; }
+    // tiles of the current item in the range: [tile, tile + count) of the sequence
+    DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(r.tiles - tile), end - unit)); }
+    DM_DEV void next(int cnt) {
+        unit += cnt;
+        if (unit >= end) return;
+        tile = 0;
+        if (++h < a.Hkv) return;
+        h = 0;
+        if (++blk < r.blocks) return;
+        blk = 0;
+        do {
+            if (++req >= a.n) {  // only if the lengths changed under the kernel
+                end = unit;
+                return;
+            }
+            r = key_req<RB>(a, ahead, false);
+            ahead = key_raw(a, req + 1);
+        } while (r.blocks == 0);
+    }
+};
+
+// This CTA's range [u0, u1) of the sequence and where it starts: every thread sums its share of
+// the requests, one block-wide scan.  At most one CTA per `min_tiles` tiles takes part; false:
+// this one does not.  Called by all NT threads; ends with a barrier.
+template <int RB, int NT>
+DM_DEV bool key_range(const Kv8AttnArgs& a, int min_tiles, long long* s_sum, int* s_req, long long* s_rem, long long& u0,
+                      long long& u1, long long& total, long long& grid) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int per = (a.n + NT - 1) / NT;
+    const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
+    auto tiles_of = [&](int i, bool report) {
+        const KeyReq r = key_req<RB>(a, key_raw(a, i), report);
+        return static_cast<long long>(r.blocks) * a.Hkv * r.tiles;
+    };
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) mine += tiles_of(i, blockIdx.x == 0);
+    long long pre = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, pre, o);
+        if (lane >= o) pre += y;
+    }
+    if (lane == 31) s_sum[warp] = pre;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w == warp) pre += total - mine;  // tiles before this thread's requests
+        total += s_sum[w];
+    }
+    grid = min(static_cast<long long>(gridDim.x), (total + min_tiles - 1) / min_tiles);
+    const bool active = blockIdx.x < grid;
+    u0 = active ? total * blockIdx.x / grid : 0;
+    u1 = active ? total * (blockIdx.x + 1) / grid : 0;
+    if (active && u0 >= pre && u0 < pre + mine) {
+        long long at = pre;
+        for (int i = i0; i < i1; ++i) {
+            const long long c = tiles_of(i, false);
+            if (u0 < at + c) {
+                *s_req = i;
+                *s_rem = u0 - at;
+                break;
+            }
+            at += c;
+        }
+    }
+    __syncthreads();
+    return active;
+}
+
+// The CTA whose range holds tile u.
+DM_DEV int key_owner(long long u, long long total, long long grid) { return static_cast<int>(((u + 1) * grid - 1) / total); }
+
+// Producer (one warp): per tile K then V of its 8 pages in chunks of CW bytes, TMA boxes of 16
+// token rows; groups of 4 tiles, a lane per page, page ids fetched two groups ahead of their use,
+// scales one group ahead.  A page that is missing or holds no key of the item reads zeros.
+// full[stage] (2 arrivals) completes with the copies and s_meta (sK, sV; sV < 0: no page).
+template <int RB, int D, int ST>
+DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, uint64_t* full, uint64_t* empty,
+                        float2 (*s_meta)[kKeyPages], long long u0, long long u1, int req, long long rem,
+                        volatile int* abort_flag) {
+    constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW, kTileBytes = kKeyTile * D, kStage = 2 * kTileBytes;
+    const int lane = threadIdx.x & 31;
+    uint32_t use = 0;  // tiles issued
+    bool ok = true;
+    KeyWalk<RB> w(a, u0, u1, req, rem);
+    int ti = -1, ei = 0, hi = 0;  // next tile of w's item, end of its tiles, its keys
+    struct Group {
+        int count = 0;             // tiles
+        int id = -1, h = 0;        // this lane's page (tile lane / 8, page lane % 8) and kv head
+        bool wanted = false;       // a key of the item lies on it
+        float2 sc = make_float2(0.0f, -1.0f);
+    };
+    auto fetch_ids = [&](Group& g) {
+        g = Group();
+        while (g.count < 32 / kKeyPages && w.unit < w.end) {
+            if (ti < 0) {
+                int lo;
+                key_limits<RB>(a, w.r, w.block(), lo, hi);
+                ti = w.tile;
+                ei = min(w.tile + w.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
+            }
+            if (ti < ei) {
+                const int p = ti * kKeyPages + lane % kKeyPages;
+                if (lane / kKeyPages == g.count) {
+                    g.h = w.h;
+                    g.wanted = p * kKv8Page < hi;
+                    if (g.wanted) g.id = a.table[static_cast<size_t>(w.req) * a.width + p];
+                }
+                ++g.count;
+                ++ti;
+            } else {
+                w.next(w.count());
+                ti = -1;
+            }
+        }
+    };
+    auto fetch_scales = [&](Group& g) {
+        if (!g.wanted) return;
+        if (g.id >= 0 && g.id < a.num_pages) {
+            const float* sc = a.scales + static_cast<size_t>(g.id) * 2 * a.Hkv + g.h;
+            g.sc = make_float2(sc[0], sc[a.Hkv]);
+        } else {
+            raise_error(a.err, DM_DEVERR_PAGE);
+        }
+    };
+    Group g0, g1, g2;
+    fetch_ids(g0);
+    fetch_ids(g1);
+    fetch_scales(g0);
+    while (g0.count > 0 && ok) {
+        fetch_ids(g2);
+        fetch_scales(g1);
+        for (int k = 0; k < g0.count; ++k) {
+            const uint32_t si = use % ST, ph = (use / ST) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
+                ok = false;
+                break;
+            }
+            const bool mine = lane / kKeyPages == k;
+            const int pg = lane % kKeyPages;
+            if (lane == 0) mbar_arrive_expect_tx(&full[si], kStage);
+            __syncwarp();
+            if (mine) {
+                const int page = g0.id >= 0 && g0.id < a.num_pages ? g0.id : a.num_pages;
+                const uint32_t kt = smem_u32(sm + si * kStage) + pg * (kKv8Page * CW);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+                    tma_load_3d(kt + c * (kKeyTile * CW), map, c * CW, g0.h * kKv8Page, page, &full[si]);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+                    tma_load_3d(kt + kTileBytes + c * (kKeyTile * CW), map, c * CW, (a.Hkv + g0.h) * kKv8Page,
+                                page, &full[si]);
+                s_meta[si][pg] = g0.sc;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[si]);
+            ++use;
+        }
+        g0 = g1;
+        g1 = g2;
+    }
+    if (lane == 0)
+        for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
+            mbar_wait_bounded(&full[u % ST], (u / ST) & 1u, a.err, nullptr);
+}
+
+}  // namespace dm
