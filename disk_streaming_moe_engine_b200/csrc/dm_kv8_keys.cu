@@ -48,19 +48,19 @@ struct KeyShape {
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
     static constexpr int kTileBytes = kKeyTile * D;   // K or V of a tile
-    static constexpr int kStage = 2 * kTileBytes;
     static constexpr int kQ = kN * D;
     static constexpr int kP = kN * kKeyTile;          // one of two buffers
     static constexpr int kFixed = kQ + 2 * kP + 1024;
     // a tile's chain of waits takes about 0.65 us whatever D is, its bytes from HBM 0.37 us at
     // D = 64 and 1.5 us at D = 256: the smaller heads take two CTAs per SM
     static constexpr int kCtas = D <= 128 && RB == 8 ? 2 : 1;
-    static constexpr int kFit = (kKeySmem / kCtas - 5120 - kFixed) / kStage;  // static arrays and 1 KB per CTA beside it
-    static constexpr int kStages = kFit > 8 ? 8 : kFit;
-    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kFixed;
+    static constexpr int kSlot = 2 * kTileBytes;      // K and V of a tile
+    static constexpr int kFit = (kKeySmem / kCtas - 6144 - kFixed) / kSlot;  // static arrays and 1 KB per CTA beside it
+    static constexpr int kSlots = kFit > kKeyMaxSlots ? kKeyMaxSlots : kFit;
+    static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kSlot + kFixed;
     static constexpr int kColsUsed = (2 + kChunks) * kN;
     static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
-    static_assert(kStages >= 2 && kN % 16 == 0 && kColsUsed <= 512, "shape");
+    static_assert(kSlots >= 2 && kN % 16 == 0 && kColsUsed <= 512, "shape");
     static_assert(kQ % 1024 == 0 && kP % 1024 == 0, "tiles start at the swizzle's 1024 bytes");
 };
 
@@ -73,15 +73,15 @@ template <typename T, int D, int RB>
 __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, RB>::kCtas)
     kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB>;
-    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, ST = S::kStages, SOFT = S::kSoft;
+    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
     extern __shared__ __align__(1024) uint8_t key_smem[];
     uint8_t* sm = key_smem + ((1024u - (smem_u32(key_smem) & 1023u)) & 1023u);
-    uint8_t* s_q = sm + ST * S::kStage;
+    uint8_t* s_q = sm + SL * S::kSlot;
     uint8_t* s_p = s_q + S::kQ;
-    __shared__ __align__(8) uint64_t full[ST], empty[ST], s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
-    __shared__ float2 s_meta[ST][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
+    __shared__ __align__(8) KeyRing<SL, true> ring;
+    __shared__ __align__(8) uint64_t s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
     __shared__ float s_red[4][RB], s_fac[32][RB];
@@ -94,10 +94,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     volatile int* abort_flag = &s_abort;
 
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(&full[i], 2);  // the copies, and the scales
-            mbar_init(&empty[i], 1);
-        }
+        ring.init();
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], SOFT);
@@ -118,7 +115,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     const uint32_t tmem = s_tmem;
 
     if (active && warp == W_LOAD) {
-        key_produce<RB, D, ST>(a, &ka.map, sm, full, empty, s_meta, u0, u1, s_req, s_rem, abort_flag);
+        key_produce<RB, D, SL, true>(a, &ka.map, sm, ring, u0, u1, s_req, s_rem, abort_flag);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
@@ -127,9 +124,10 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
             const uint32_t i_s = f8_idesc(128, N, false, false), i_o = f8_idesc(128, N, true, true);
             const uint32_t sq = smem_u32(s_q), sp = smem_u32(s_p);
             auto scores = [&](uint32_t x) {  // S^T of tile x into its buffer
-                if (!(ok = mbar_wait_bounded(&full[x % ST], (x / ST) & 1u, a.err, abort_flag))) return;
+                const uint32_t ld = ring.k_load(x);
+                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return;
                 tc_fence_after();
-                const uint32_t k = smem_u32(sm + (x % ST) * S::kStage);
+                const uint32_t k = smem_u32(sm + (ld % SL) * S::kSlot);
 #pragma unroll
                 for (int c = 0; c < S::kChunks; ++c) {
                     const uint64_t ad = f8_desc_k<CW>(k + c * (kKeyTile * CW)), bd = f8_desc_k<CW>(sq + c * (N * CW));
@@ -154,7 +152,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                         if (i + 1 < nt) scores(x + 1);
                         if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
                         tc_fence_after();
-                        const uint32_t v = smem_u32(sm + (x % ST) * S::kStage) + S::kTileBytes;
+                        const uint32_t ld = ring.v_load(x);
+                        const uint32_t v = smem_u32(sm + (ld % SL) * S::kSlot) + S::kTileBytes;
                         const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                             for (int j = 0; j < kKeyTile / 32; ++j)
                                 f8_mma(tmem + (2 + c) * N, ad + j * (32 * CW / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
                         }
-                        tc_commit(&empty[x % ST]);
+                        tc_commit(&ring.empty[ld % SL]);
                         tc_commit(&pv_done[x & 1u]);
                     }
                     t += nt;
@@ -239,21 +238,21 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
             for (int r = 0; r < 8; ++r) mref[r] = -INFINITY, l[r] = 0.0f, frow[r] = s_frow[r0 + r];
 
             for (int i = 0; i < nt; ++i) {
-                const uint32_t x = t + i, si = x % ST;
+                const uint32_t x = t + i;
                 const int key = (t_begin + i) * kKeyTile + tt;
-                // the tile's copies and scales, its scores, and (from the third tile on) the P buffer,
+                // the tile's scales, its scores, and (from the third tile on) the P buffer,
                 // tried together since they are mostly there
-                const bool t1 = mbar_try_wait(&full[si], (x / ST) & 1u);
+                const bool t1 = ring.try_meta(x);
                 const bool t2 = mbar_try_wait(&s_full[x & 1u], (x >> 1) & 1u);
                 const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
                 if (!(t1 && t2 && t3)) {
-                    ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag) &&
+                    ok = ring.wait_meta(x, a.err, abort_flag) &&
                          mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag) &&
                          (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
                 }
                 __syncwarp();  // the loads below are the whole warp's
                 tc_fence_after();
-                const float2 sc = s_meta[si][tt >> 4];
+                const float2 sc = ring.meta[x % kKeyMeta][tt >> 4];
                 const float vexp = static_cast<float>(((__float_as_int(sc.y) >> 23) & 0xff) - 127);
                 float y[8];
                 {
@@ -334,7 +333,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     // V rows behind the last key become zeros; a NaN code that not every row sees
                     // becomes 0 and makes the sums of the rows that see it NaN
                     if (r0 == 0) {
-                        uint8_t* v = sm + si * S::kStage + S::kTileBytes + tt * CW;
+                        ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
+                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kSlot + S::kTileBytes + tt * CW;
                         bool nan = false;
                         if (key >= lim_max) {
 #pragma unroll

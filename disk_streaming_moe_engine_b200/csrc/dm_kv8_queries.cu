@@ -40,13 +40,12 @@ struct QryShape {
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
     static constexpr int kTileBytes = kKeyTile * D;
-    static constexpr int kStage = 2 * kTileBytes;
     static constexpr int kTerm = kQryRows * D;  // one term of Q
     static constexpr int kFixed = 2 * kTerm + 1024;
-    static constexpr int kFit = (227 * 1024 - 6144 - kFixed) / kStage;
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
-    static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStage + kFixed;
-    static_assert(kStages >= 2, "shape");
+    static constexpr int kFit = (227 * 1024 - 6144 - kFixed) / kTileBytes;
+    static constexpr int kSlots = kFit > kKeyMaxSlots ? kKeyMaxSlots : kFit;
+    static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kTileBytes + kFixed;
+    static_assert(kSlots >= 4, "shape");
 };
 
 struct QryArgs {
@@ -57,14 +56,14 @@ struct QryArgs {
 template <int D>
 __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const __grid_constant__ QryArgs qa) {
     using S = QryShape<D>;
-    constexpr int CW = S::CW, ST = S::kStages, RB = kQryRows;
+    constexpr int CW = S::CW, SL = S::kSlots, RB = kQryRows;
     constexpr uint32_t kPw = 128, kO = 256;  // tensor memory columns: scores, weights (two buffers of 64), O
     const Kv8AttnArgs& a = qa.a;
     extern __shared__ __align__(1024) uint8_t qry_smem[];
     uint8_t* sm = qry_smem + ((1024u - (smem_u32(qry_smem) & 1023u)) & 1023u);
-    uint8_t* s_q = sm + ST * S::kStage;
-    __shared__ __align__(8) uint64_t full[ST], empty[ST], s_full, s_free, p_ready[2], pv_done[2], q_ready, q_free, done_bar;
-    __shared__ float2 s_meta[ST][kKeyPages];
+    uint8_t* s_q = sm + SL * S::kTileBytes;
+    __shared__ __align__(8) KeyRing<SL, false> ring;
+    __shared__ __align__(8) uint64_t s_full, s_free, p_ready[2], pv_done[2], q_ready, q_free, done_bar;
     __shared__ float s_frow[RB], s_max[2][RB], s_l[2][RB];
     __shared__ int s_lim[RB];
     __shared__ long long s_sum[kQryThreads / 32], s_rem;
@@ -77,10 +76,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     constexpr int W_Q = 8, W_LOAD = 10, W_MMA = 11;
 
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(&full[i], 2);  // the copies, and the scales
-            mbar_init(&empty[i], 1);
-        }
+        ring.init();
         for (int i = 0; i < 2; ++i) {
             mbar_init(&p_ready[i], kQrySoft);
             mbar_init(&pv_done[i], 1);
@@ -102,7 +98,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     const uint32_t tmem = s_tmem;
 
     if (active && warp == W_LOAD) {
-        key_produce<RB, D, ST>(a, &qa.map, sm, full, empty, s_meta, u0, u1, s_req, s_rem, abort_flag);
+        key_produce<RB, D, SL, false>(a, &qa.map, sm, ring, u0, u1, s_req, s_rem, abort_flag);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
@@ -126,10 +122,11 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     first = left > 0;
                 }
                 if (first && !(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) return false;
-                if (!(ok = mbar_wait_bounded(&full[sx % ST], (sx / ST) & 1u, a.err, abort_flag))) return false;
+                const uint32_t ld = ring.k_load(sx);
+                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return false;
                 if (!(ok = mbar_wait_bounded(&s_free, (sx & 1u) ^ 1u, a.err, abort_flag))) return false;
                 tc_fence_after();
-                const uint32_t k = smem_u32(sm + (sx % ST) * S::kStage);
+                const uint32_t k = smem_u32(sm + (ld % SL) * S::kTileBytes);
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -140,6 +137,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                         for (int j = 0; j < CW / 32; ++j)
                             f8_mma(tmem, ad + 2 * j, bd + 2 * j, i_s, t > 0 || c > 0 || j > 0);
                     }
+                tc_commit(&ring.empty[ld % SL]);
                 tc_commit(&s_full);
                 firsts = (firsts & ~(1u << (sx & 1u))) | ((first ? 1u : 0u) << (sx & 1u));
                 ++sx;
@@ -153,9 +151,11 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             while (more && ok) {
                 more = next_scores();
                 if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
+                const uint32_t ld = ring.v_load(x);
+                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) break;
                 tc_fence_after();
                 const bool first = (firsts >> (x & 1u)) & 1u;
-                const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (x % ST) * S::kStage) + S::kTileBytes, kKeyTile * CW);
+                const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), kKeyTile * CW);
                 const uint32_t p = tmem + kPw + (x & 1u) * 64;
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     for (int j = 0; j < kKeyTile / 32; ++j)
                         f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o,
                                   !first || t > 0 || j > 0);
-                tc_commit(&empty[x % ST]);
+                tc_commit(&ring.empty[ld % SL]);
                 tc_commit(&pv_done[x & 1u]);
                 ++x;
             }
@@ -263,13 +263,13 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             bool nan_row = false;
 
             for (int i = 0; i < nt; ++i) {
-                const uint32_t x = t + i, si = x % ST, pb = kPw + (x & 1u) * 64 + half * 16;
+                const uint32_t x = t + i, pb = kPw + (x & 1u) * 64 + half * 16;
                 const int tile0 = (t_begin + i) * kKeyTile;
-                const bool t1 = mbar_try_wait(&full[si], (x / ST) & 1u);
+                const bool t1 = ring.try_meta(x);
                 const bool t2 = mbar_try_wait(&s_full, x & 1u);
                 const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
                 if (ok && !(t1 && t2 && t3))
-                    ok = mbar_wait_bounded(&full[si], (x / ST) & 1u, a.err, abort_flag) &&
+                    ok = ring.wait_meta(x, a.err, abort_flag) &&
                          mbar_wait_bounded(&s_full, x & 1u, a.err, abort_flag) &&
                          (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
                 __syncwarp();
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 const float base = mref == -INFINITY ? 0.0f : kQryBoost - mref;
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const float2 sc = s_meta[si][half * 4 + p];
+                    const float2 sc = ring.meta[x % kKeyMeta][half * 4 + p];
                     const int ve = ((__float_as_int(sc.y) >> 23) & 0xff) - 127;
                     f[p] = frow * sc.x;
                     g[p] = sc.y < 0.0f ? -INFINITY : static_cast<float>(ve) + base;
@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     // V rows behind the last key become zeros; a NaN code that not every row sees
                     // becomes 0 and makes the sums of the rows that see it NaN
                     if (half == 0) {
-                        uint8_t* v = sm + si * S::kStage + S::kTileBytes + row * CW;
+                        ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
+                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kTileBytes + row * CW;
                         const int key = tile0 + row;
                         bool nan = false;
                         if (key >= lim_max) {

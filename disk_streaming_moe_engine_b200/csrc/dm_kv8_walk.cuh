@@ -153,17 +153,46 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_tiles, long long* s_sum, int
 // The CTA whose range holds tile u.
 DM_DEV int key_owner(long long u, long long total, long long grid) { return static_cast<int>(((u + 1) * grid - 1) / total); }
 
-// Producer (one warp): per tile K then V of its 8 pages in chunks of CW bytes, TMA boxes of 16
-// token rows; groups of 4 tiles, a lane per page, page ids fetched two groups ahead of their use,
-// scales one group ahead.  A page that is missing or holds no key of the item reads zeros.
-// full[stage] (2 arrivals) completes with the copies and s_meta (sK, sV; sV < 0: no page).
-template <int RB, int D, int ST>
-DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, uint64_t* full, uint64_t* empty,
-                        float2 (*s_meta)[kKeyPages], long long u0, long long u1, int req, long long rem,
-                        volatile int* abort_flag) {
-    constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW, kTileBytes = kKeyTile * D, kStage = 2 * kTileBytes;
+// Shared memory of the key tiles: a ring of SL slots.  PAIR: a slot takes a tile's K and V and is
+// free again after its O product.  Else a slot takes K or V of one tile, loaded in the order K0,
+// K1, V0, K2, V1, ..., and is free as soon as the one product that reads it is done: the ring then
+// holds what the next products need.  The query-side kernel is bound by its products and by how
+// early the next tile is there (4 x 8192 prompts 3.24 ms in pairs, 2.73 ms single); the key-side
+// one by the bytes (64 x 32768 384 us in pairs, 405 us single).
+constexpr int kKeyMeta = 8;      // tiles whose scales are kept (at least slots / 2 + 2)
+constexpr int kKeyMaxSlots = 12;
+
+template <int SL, bool PAIR>
+struct KeyRing {
+    uint64_t full[SL], empty[SL], meta_full[kKeyMeta];
+    float2 meta[kKeyMeta][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
+    static DM_DEV uint32_t k_load(uint32_t tile) { return PAIR ? tile : tile ? 2 * tile - 1 : 0; }
+    static DM_DEV uint32_t v_load(uint32_t tile) { return PAIR ? tile : 2 * tile + 2; }
+    DM_DEV void init() {               // one thread
+        for (int i = 0; i < SL; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < kKeyMeta; ++i) mbar_init(&meta_full[i], 1);
+    }
+    DM_DEV bool wait_full(uint32_t load, uint32_t* err, volatile int* abort_flag) {
+        return mbar_wait_bounded(&full[load % SL], (load / SL) & 1u, err, abort_flag);
+    }
+    // scales of tile x: ready (or not yet)
+    DM_DEV bool try_meta(uint32_t x) { return mbar_try_wait(&meta_full[x % kKeyMeta], (x / kKeyMeta) & 1u); }
+    DM_DEV bool wait_meta(uint32_t x, uint32_t* err, volatile int* abort_flag) {
+        return mbar_wait_bounded(&meta_full[x % kKeyMeta], (x / kKeyMeta) & 1u, err, abort_flag);
+    }
+};
+
+// Producer (one warp): a tile's K or V as TMA boxes of 16 token rows by CW bytes, one lane per
+// page; page ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A
+// page that is missing or holds no key of the item reads zeros.
+template <int RB, int D, int SL, bool PAIR>
+DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, KeyRing<SL, PAIR>& ring, long long u0,
+                        long long u1, int req, long long rem, volatile int* abort_flag) {
+    constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW, kSlot = (PAIR ? 2 : 1) * kKeyTile * D;
     const int lane = threadIdx.x & 31;
-    uint32_t use = 0;  // tiles issued
     bool ok = true;
     KeyWalk<RB> w(a, u0, u1, req, rem);
     int ti = -1, ei = 0, hi = 0;  // next tile of w's item, end of its tiles, its keys
@@ -203,48 +232,60 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
             const float* sc = a.scales + static_cast<size_t>(g.id) * 2 * a.Hkv + g.h;
             g.sc = make_float2(sc[0], sc[a.Hkv]);
         } else {
+            g.id = -1;
             raise_error(a.err, DM_DEVERR_PAGE);
         }
+    };
+    int last = -1;  // lane i: the last ring position loaded into slot i
+    // the tile with these pages into ring position `at`: rows from `row` on, in pairs V's behind K's
+    auto load = [&](uint32_t at, int id, int row) {
+        const uint32_t si = at % SL;
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[si], ((at / SL) & 1u) ^ 1u, a.err, abort_flag))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&ring.full[si], kSlot);
+        if (lane == static_cast<int>(si)) last = static_cast<int>(at);
+        __syncwarp();
+        if (lane < kKeyPages) {
+            const uint32_t dst = smem_u32(sm + si * kSlot) + lane * (kKv8Page * CW);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+                tma_load_3d(dst + c * (kKeyTile * CW), map, c * CW, row, id < 0 ? a.num_pages : id, &ring.full[si]);
+            if constexpr (PAIR)
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+                    tma_load_3d(dst + (kChunks + c) * (kKeyTile * CW), map, c * CW, row + a.Hkv * kKv8Page,
+                                id < 0 ? a.num_pages : id, &ring.full[si]);
+        }
+        return true;
     };
     Group g0, g1, g2;
     fetch_ids(g0);
     fetch_ids(g1);
     fetch_scales(g0);
+    uint32_t x = 0;                // tile
+    int prev_id = -1, prev_h = 0;  // pages of the tile before, by lane % 8
     while (g0.count > 0 && ok) {
         fetch_ids(g2);
         fetch_scales(g1);
-        for (int k = 0; k < g0.count; ++k) {
-            const uint32_t si = use % ST, ph = (use / ST) & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[si], ph ^ 1u, a.err, abort_flag))) {
-                ok = false;
-                break;
-            }
-            const bool mine = lane / kKeyPages == k;
-            const int pg = lane % kKeyPages;
-            if (lane == 0) mbar_arrive_expect_tx(&full[si], kStage);
+        for (int k = 0; k < g0.count && ok; ++k, ++x) {
+            const int from = k * kKeyPages + lane % kKeyPages;
+            const int h = __shfl_sync(0xffffffffu, g0.h, from);
+            int id = __shfl_sync(0xffffffffu, g0.id, from);
+            if (id >= a.num_pages) id = -1;
+            const float2 sc = make_float2(__shfl_sync(0xffffffffu, g0.sc.x, from), __shfl_sync(0xffffffffu, g0.sc.y, from));
+            if (!(ok = load(ring.k_load(x), id, h * kKv8Page))) break;
+            if (lane < kKeyPages) ring.meta[x % kKeyMeta][lane] = sc;
             __syncwarp();
-            if (mine) {
-                const int page = g0.id >= 0 && g0.id < a.num_pages ? g0.id : a.num_pages;
-                const uint32_t kt = smem_u32(sm + si * kStage) + pg * (kKv8Page * CW);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    tma_load_3d(kt + c * (kKeyTile * CW), map, c * CW, g0.h * kKv8Page, page, &full[si]);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    tma_load_3d(kt + kTileBytes + c * (kKeyTile * CW), map, c * CW, (a.Hkv + g0.h) * kKv8Page,
-                                page, &full[si]);
-                s_meta[si][pg] = g0.sc;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[si]);
-            ++use;
+            if (lane == 0) mbar_arrive(&ring.meta_full[x % kKeyMeta]);
+            if (!PAIR && x > 0) ok = load(ring.v_load(x - 1), prev_id, (a.Hkv + prev_h) * kKv8Page);
+            prev_id = id;
+            prev_h = h;
         }
         g0 = g1;
         g1 = g2;
     }
-    if (lane == 0)
-        for (uint32_t u = use > ST ? use - ST : 0; u < use; ++u)
-            mbar_wait_bounded(&full[u % ST], (u / ST) & 1u, a.err, nullptr);
+    if (!PAIR && ok && x > 0) ok = load(ring.v_load(x - 1), prev_id, (a.Hkv + prev_h) * kKv8Page);
+    // no copy is left in flight, whoever gave up
+    if (last >= 0) ring.wait_full(static_cast<uint32_t>(last), a.err, nullptr);
 }
 
 }  // namespace dm
