@@ -736,7 +736,7 @@ extern "C" int32_t dm_rope(const dm_rope_plan* plan, int32_t dtype, int32_t n, c
                 return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "in place needs the same strides");
             a.inplace[i] = 1;
         }
-        vec = vec && kv8_aligned16(a.x[i], a.x_rs[i], a.x_hs[i], elem) && kv8_aligned16(a.y[i], a.y_rs[i], a.y_hs[i], elem);
+        vec = vec && kv8_aligned(a.x[i], a.x_rs[i], a.x_hs[i], elem, 16) && kv8_aligned(a.y[i], a.y_rs[i], a.y_hs[i], elem, 16);
     }
     // few tokens: a CTA each, for the shortest wait; many: 8, whose angles are then computed by
     // the CTA's threads in one round (32771 tokens of 40 heads: see the figures above)
@@ -785,7 +785,7 @@ extern "C" int32_t dm_kv8_append(const dm_kv8_cache* c, int32_t dtype, int32_t n
     // rows of a CTA: one when the rows may all be in pages of their own (a decode step), more
     // for prompts, where a CTA per row would mostly find that an earlier one has its page
     a.window = n <= 2048 ? 1 : n <= 8192 ? 4 : 16;
-    a.vec = kv8_aligned16(k, k_rs, k_hs, elem) && kv8_aligned16(v, v_rs, v_hs, elem);
+    a.vec = kv8_aligned(k, k_rs, k_hs, elem, 16) && kv8_aligned(v, v_rs, v_hs, elem, 16);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = dtype == DM_DTYPE_F32 ? launch_append<float>(a, c->head_dim, s)
                                                 : launch_append<__nv_bfloat16>(a, c->head_dim, s);

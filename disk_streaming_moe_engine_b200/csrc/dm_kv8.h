@@ -24,8 +24,8 @@ struct Kv8Device {
 
 int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t es);
 
-inline bool kv8_aligned16(const void* p, int64_t stride_a, int64_t stride_b, int elem) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_a * elem % 16 == 0 && stride_b * elem % 16 == 0;
+inline bool kv8_aligned(const void* p, int64_t stride_a, int64_t stride_b, int elem, int to) {
+    return reinterpret_cast<uintptr_t>(p) % to == 0 && stride_a * elem % to == 0 && stride_b * elem % to == 0;
 }
 
 // Attention over the cache, as the kernels see it.
@@ -44,8 +44,15 @@ struct Kv8AttnArgs {
     int64_t q_rs, q_hs, o_rs, o_hs;  // strides in elements
     float scale_log2;     // sm_scale * log2(e)
     int n, rows, Hq, Hkv, group, num_pages, width, max_q;
-    int q_vec, o_vec;     // q / out: pointer and strides are multiples of 16 bytes
+    int exact;            // the work is cut by exact tile counts (few requests, or few blocks in each)
+    int q_vec, o_vec;     // q / out: pointer and strides are multiples of 32 bytes
 };
+
+// Exact tile counts cost a pass over all row blocks in every CTA: taken where a warp goes through a
+// request's blocks (up to 64 requests) or no request has more than 8.
+inline int kv8_exact(const Kv8AttnArgs& a, int rows_per_block) {
+    return a.n <= 64 || (static_cast<int64_t>(a.max_q) * a.group + rows_per_block - 1) / rows_per_block <= 8;
+}
 
 // dm_kv8_keys.cu: any row count and type, one or two CTAs per SM.  Workspace: counters [2 num_sms], then
 // the partials' floats.

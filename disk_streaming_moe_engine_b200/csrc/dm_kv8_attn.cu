@@ -82,8 +82,8 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + counter_bytes(g.num_sms));
     const bool f32 = p->dtype == DM_DTYPE_F32;
     const int elem = f32 ? 4 : 2;
-    a.q_vec = kv8_aligned16(a.q, a.q_rs, a.q_hs, elem);
-    a.o_vec = kv8_aligned16(a.out, a.o_rs, a.o_hs, elem);
+    a.q_vec = kv8_aligned(a.q, a.q_rs, a.q_hs, elem, 32);
+    a.o_vec = kv8_aligned(a.out, a.o_rs, a.o_hs, elem, 32);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // many bf16 rows per request and kv head: queries on the M side
     const bool many = !f32 && static_cast<int64_t>(a.max_q) * a.group >= 64;

@@ -36,6 +36,7 @@
 namespace dm {
 
 constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its CTAs
+constexpr int kKeyLead = 1;                  // an item's start and end in tiles (KeyWalk)
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
 
@@ -85,9 +86,10 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
     __shared__ float s_red[4][RB], s_fac[32][RB];
-    __shared__ long long s_sum[NT / 32], s_rem;
+    __shared__ long long s_sum[64];
+    __shared__ KeyRange s_range;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_req, s_abort;
+    __shared__ int s_abort;
     __shared__ uint8_t s_nan[kKeyTile];
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -108,14 +110,13 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     if (warp == W_MMA) tc_alloc(&s_tmem, S::kCols);
 
     tc_fence_before();
-    long long u0, u1, total, grid;
     // two tiles per CTA at least: a part costs more to join than a second tile takes
-    const bool active = key_range<RB, NT>(a, 2, s_sum, &s_req, &s_rem, u0, u1, total, grid);
+    const bool active = key_range<RB, kKeyLead, NT>(a, 2 + kKeyLead, s_sum, &s_range);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
     if (active && warp == W_LOAD) {
-        key_produce<RB, D, SL, true>(a, &ka.map, sm, ring, u0, u1, s_req, s_rem, abort_flag);
+        key_produce<RB, kKeyLead, D, SL, true>(a, &ka.map, sm, ring, s_range, abort_flag);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
@@ -136,12 +137,11 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                 }
                 tc_commit(&s_full[x & 1u]);
             };
-            KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+            KeyWalk<RB, kKeyLead> w(a, s_range);
             while (w.unit < w.end && ok) {
-                int lo, hi;
-                key_limits<RB>(a, w.r, w.block(), lo, hi);
-                const int cnt = w.count();
-                const int nt = min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) - w.tile;
+                int first, last, real;
+                w.span(first, last, real);
+                const int nt = last - first;
                 if (nt > 0) {
                     if (!(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) break;
                     ++item;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     }
                     t += nt;
                 }
-                w.next(cnt);
+                w.next();
             }
             tc_commit(&done_bar);
             mbar_wait_bounded(&done_bar, 0, a.err, nullptr);
@@ -178,15 +178,15 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + r0;
         uint32_t t = 0;
         bool ok = true;
-        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        KeyWalk<RB, kKeyLead> w(a, s_range);
         while (w.unit < w.end && ok) {
             int lim_min, lim_max;
             key_limits<RB>(a, w.r, w.block(), lim_min, lim_max);
-            const int cnt = w.count();
-            const int real = max(1, (lim_max + kKeyTile - 1) / kKeyTile);  // tiles of the item
-            const int t_begin = w.tile, nt = min(w.tile + cnt, real) - w.tile;
+            int t_begin, t_end, real;
+            w.span(t_begin, t_end, real);
+            const int nt = t_end - t_begin;
             if (nt <= 0) {
-                w.next(cnt);
+                w.next();
                 continue;
             }
             const int nrow = min(RB, w.r.m * a.group - w.block() * RB);
@@ -401,9 +401,9 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
             for (int r = 0; r < 8; ++r) l[r] = s_red[0][r0 + r] + s_red[1][r0 + r] + s_red[2][r0 + r] + s_red[3][r0 + r];
             named_bar_sync(1, SOFT);  // s_red is free again
 
-            const long long item0 = w.unit - t_begin;  // the item's first tile in the sequence
+            const long long item0 = w.tile0();  // the item's first tile in the sequence
             const bool whole = t_begin == 0 && nt == real;
-            const int c_first = key_owner(item0, total, grid), c_last = key_owner(item0 + real - 1, total, grid);
+            const int c_first = key_owner(item0, s_range.total, s_range.grid), c_last = key_owner(item0 + real - 1, s_range.total, s_range.grid);
             constexpr int kSlot = (RB * (D + 2) + 3) / 4 * 4;
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
             auto put = [&](int r, int d, float o, float mm, float ll) {
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     named_bar_sync(1, SOFT);  // s_red is free again
                 }
             }
-            w.next(cnt);
+            w.next();
         }
     }
     tc_fence_before();
@@ -574,6 +574,7 @@ cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f3
     if (!kv8_encode_map(c, &ka.map)) return cudaErrorNotSupported;
     ka.a = a;
     const bool wide = static_cast<int64_t>(a.max_q) * a.group > 8;
+    ka.a.exact = kv8_exact(a, wide ? 16 : 8);
     if (f32) return wide ? launch_keys_d<float, 16>(ka, c->head_dim, num_sms, dev, s)
                          : launch_keys_d<float, 8>(ka, c->head_dim, num_sms, dev, s);
     return wide ? launch_keys_d<__nv_bfloat16, 16>(ka, c->head_dim, num_sms, dev, s)

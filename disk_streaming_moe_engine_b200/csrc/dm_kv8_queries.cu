@@ -16,14 +16,17 @@
 // threads, 64 keys of the tile each, that meet at a 64-thread barrier to agree on M; O is
 // rescaled only by warps with a raised row.
 //
-// Roles (384 threads): 8 softmax warps (two per quarter of the rows), 2 warps that turn the next
-// item's q rows into terms as soon as its predecessor's last scores are done, a producer and an
-// MMA warp.  The scores of tile x + 1 follow as soon as those of tile x are in registers and run
-// before the O product of tile x, so the softmax has the time of two products.  Tensor memory: the
-// scores (128 columns), two buffers of weights (64), O (D).  Split of the work, joins and
-// bounded waits as in the key-side kernel; after a failed wait every thread runs through the
-// remaining barriers without work.
+// Roles (320 threads): 8 softmax warps (two per quarter of the rows), a producer and an MMA warp.
+// The scores of tile x + 1 follow as soon as those of tile x are in registers and run before the
+// O product of tile x, so the softmax has the time of two products.  Between items the softmax
+// warps turn the next item's q rows into terms while the last O product runs, then write the
+// item's O while the next scores run (two separate warps for the terms were slower: the
+// conversions are ALU work that all four schedulers have to share).  Tensor memory: the scores
+// (128 columns), two buffers of weights (64), O (D).  Split of the work, joins and bounded waits
+// as in the key-side kernel; after a failed wait every thread runs through the remaining barriers
+// without work.
 #include <cmath>
+#include <type_traits>
 
 #include "dm_kv8_walk.cuh"
 
@@ -31,7 +34,8 @@ namespace dm {
 
 constexpr int kQryRows = 128;
 constexpr int kQrySoft = 256;
-constexpr int kQryThreads = kQrySoft + 64 + 64;
+constexpr int kQryThreads = kQrySoft + 64;
+constexpr int kQryLead = 2;        // an item's start and end in tiles (KeyWalk)
 constexpr float kQryLazy = 2.0f;
 constexpr float kQryBoost = 6.0f;  // weights enter as 2^6 w <= 256
 
@@ -63,17 +67,17 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     uint8_t* sm = qry_smem + ((1024u - (smem_u32(qry_smem) & 1023u)) & 1023u);
     uint8_t* s_q = sm + SL * S::kTileBytes;
     __shared__ __align__(8) KeyRing<SL, false> ring;
-    __shared__ __align__(8) uint64_t s_full, s_free, p_ready[2], pv_done[2], q_ready, q_free, done_bar;
-    __shared__ float s_frow[RB], s_max[2][RB], s_l[2][RB];
-    __shared__ int s_lim[RB];
-    __shared__ long long s_sum[kQryThreads / 32], s_rem;
+    __shared__ __align__(8) uint64_t s_full, s_free, p_ready[2], pv_done[2], q_ready, done_bar;
+    __shared__ float s_max[2][RB], s_l[2][RB];
+    __shared__ long long s_sum[64];
+    __shared__ KeyRange s_range;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_req, s_abort;
+    __shared__ int s_abort;
     __shared__ uint8_t s_nan[kKeyTile];
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &s_abort;
-    constexpr int W_Q = 8, W_LOAD = 10, W_MMA = 11;
+    constexpr int W_LOAD = 8, W_MMA = 9;
 
     if (tid == 0) {
         ring.init();
@@ -83,22 +87,20 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
         }
         mbar_init(&s_full, 1);
         mbar_init(&s_free, kQrySoft);
-        mbar_init(&q_ready, 64);
-        mbar_init(&q_free, kQrySoft + 1);  // its score products are done, its scales and limits read
+        mbar_init(&q_ready, kQrySoft);
         mbar_init(&done_bar, 1);
         mbar_fence_init();
         s_abort = 0;
     }
     if (warp == W_MMA) tc_alloc(&s_tmem, 512);
     tc_fence_before();
-    long long u0, u1, total, grid;
     // a part of 128 rows is costly to join: four tiles per CTA at least
-    const bool active = key_range<RB, kQryThreads>(a, 4, s_sum, &s_req, &s_rem, u0, u1, total, grid);
+    const bool active = key_range<RB, kQryLead, kQryThreads>(a, 4 + kQryLead, s_sum, &s_range);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
     if (active && warp == W_LOAD) {
-        key_produce<RB, D, SL, false>(a, &qa.map, sm, ring, u0, u1, s_req, s_rem, abort_flag);
+        key_produce<RB, kQryLead, D, SL, false>(a, &qa.map, sm, ring, s_range, abort_flag);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {
@@ -106,25 +108,29 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             const uint32_t i_s = f8_idesc(128, kKeyTile, false, false), i_o = f8_idesc(128, D, false, true);
             const uint32_t sq = smem_u32(s_q);
             // scores run one tile ahead of the O products, across items too
-            KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+            KeyWalk<RB, kQryLead> w(a, s_range);
             uint32_t x = 0, sx = 0, item = 0;
             int left = 0;         // score tiles left of the walked item
             unsigned firsts = 0;  // bit (x & 1): tile x is its item's first
-            auto next_scores = [&]() -> bool {
-                bool first = false;
+            bool first = false;   // the next score tile is its item's first
+            enum { kNone, kIssued, kLater };
+            // S of the next tile; kLater: its item's terms are not ready and `wait` is not set
+            auto next_scores = [&](bool wait) -> int {
                 while (left == 0) {
-                    if (w.unit >= w.end) return false;
-                    int lo, hi;
-                    key_limits<RB>(a, w.r, w.block(), lo, hi);
-                    const int cnt = w.count();
-                    left = max(0, min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) - w.tile);
-                    w.next(cnt);
+                    if (w.unit >= w.end) return kNone;
+                    int begin, last, real;
+                    w.span(begin, last, real);
+                    left = max(0, last - begin);
+                    w.next();
                     first = left > 0;
                 }
-                if (first && !(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) return false;
+                if (first && !mbar_try_wait(&q_ready, item & 1u)) {
+                    if (!wait) return kLater;
+                    if (!(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) return kNone;
+                }
                 const uint32_t ld = ring.k_load(sx);
-                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return false;
-                if (!(ok = mbar_wait_bounded(&s_free, (sx & 1u) ^ 1u, a.err, abort_flag))) return false;
+                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return kNone;
+                if (!(ok = mbar_wait_bounded(&s_free, (sx & 1u) ^ 1u, a.err, abort_flag))) return kNone;
                 tc_fence_after();
                 const uint32_t k = smem_u32(sm + (ld % SL) * S::kTileBytes);
 #pragma unroll
@@ -140,21 +146,19 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 tc_commit(&ring.empty[ld % SL]);
                 tc_commit(&s_full);
                 firsts = (firsts & ~(1u << (sx & 1u))) | ((first ? 1u : 0u) << (sx & 1u));
+                first = false;
                 ++sx;
-                if (--left == 0) {
-                    tc_commit(&q_free);
-                    ++item;
-                }
-                return true;
+                if (--left == 0) ++item;
+                return kIssued;
             };
-            bool more = next_scores();
-            while (more && ok) {
-                more = next_scores();
+            int more = next_scores(true);
+            while (more == kIssued && ok) {
+                more = next_scores(false);
                 if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
                 const uint32_t ld = ring.v_load(x);
                 if (!(ok = ring.wait_full(ld, a.err, abort_flag))) break;
                 tc_fence_after();
-                const bool first = (firsts >> (x & 1u)) & 1u;
+                const bool fresh = (firsts >> (x & 1u)) & 1u;
                 const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), kKeyTile * CW);
                 const uint32_t p = tmem + kPw + (x & 1u) * 64;
 #pragma unroll
@@ -162,103 +166,187 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
 #pragma unroll
                     for (int j = 0; j < kKeyTile / 32; ++j)
                         f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o,
-                                  !first || t > 0 || j > 0);
+                                  !fresh || t > 0 || j > 0);
                 tc_commit(&ring.empty[ld % SL]);
                 tc_commit(&pv_done[x & 1u]);
                 ++x;
+                if (more == kLater) more = next_scores(true);
             }
             tc_commit(&done_bar);
             mbar_wait_bounded(&done_bar, 0, a.err, nullptr);
         }
-    } else if (active && warp >= W_Q) {
-        // ---------------- Q terms: a quarter-warp per row, 8 elements per access ----------------
-        uint32_t item = 0;
-        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
-        while (w.unit < w.end) {
-            int lo, hi;
-            key_limits<RB>(a, w.r, w.block(), lo, hi);
-            const int cnt = w.count();
-            if (min(w.tile + cnt, max(1, (hi + kKeyTile - 1) / kKeyTile)) <= w.tile) {
-                w.next(cnt);
-                continue;
-            }
-            const int rows = w.r.m * a.group, nrow = min(RB, rows - w.block() * RB);
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&q_free, (item & 1u) ^ 1u, a.err, abort_flag))) break;
-            constexpr int P = D / 64;  // accesses of a lane and row
-#pragma unroll 2
-            for (int i = 0; i < 16; ++i) {
-                const int r = (warp - W_Q) * 64 + i * 4 + lane / 8;
-                const int f = w.block() * RB + min(r, nrow - 1);
-                const int tok = f / a.group, head = w.h * a.group + f % a.group;
-                const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
-                                         static_cast<int64_t>(w.r.row0 + tok) * a.q_rs + static_cast<int64_t>(head) * a.q_hs;
-                float v[P][8];
-                float amax = 0.0f;
-#pragma unroll
-                for (int c = 0; c < P; ++c) {
-                    const __nv_bfloat16* s = q + c * 64 + (lane % 8) * 8;
-                    if (a.q_vec) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(s);
-                        const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[c][2 * j] = bf16lo(wd[j]), v[c][2 * j + 1] = bf16hi(wd[j]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[c][j] = static_cast<float>(s[j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (r >= nrow) v[c][j] = 0.0f;
-                        if (!(fabsf(v[c][j]) <= 3.402823466e38f)) v[c][j] = __int_as_float(0x7fc00000);
-                        amax = fmaxf(amax, fabsf(v[c][j]));
-                    }
-                }
-#pragma unroll
-                for (int o = 4; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
-                const float mul = __int_as_float((127 - ex) << 23);
-                if (lane % 8 == 0) {
-                    s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
-                    s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
-                }
-#pragma unroll
-                for (int c = 0; c < P; ++c) {
-                    uint32_t t0[4], t1[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) e4m3_terms2(v[c][2 * j] * mul, v[c][2 * j + 1] * mul, t0[j], t1[j]);
-                    const int d = c * 64 + (lane % 8) * 8;
-                    uint8_t* dst = s_q + (d / CW) * (RB * CW) + f8_unit<CW>(r, (d % CW) / 16) + d % 16;
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(t0[0] | (t0[1] << 16), t0[2] | (t0[3] << 16));
-                    *reinterpret_cast<uint2*>(dst + S::kTerm) = make_uint2(t1[0] | (t1[1] << 16), t1[2] | (t1[3] << 16));
-                }
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&q_ready);
-            ++item;
-            w.next(cnt);
-        }
     } else if (active) {
-        // ---------------- softmax, epilogue ----------------
+        // ---------------- Q terms, softmax, epilogue ----------------
         const int row = tid & 127, half = tid >> 7, wq = warp & 3;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16);
-        uint32_t t = 0, item = 0;
+        constexpr int H = D / 2;  // a thread's share of its row's q and O
+        uint32_t t = 0;
         bool ok = true;
-        KeyWalk<RB> w(a, u0, u1, s_req, s_rem);
+        struct Done {  // an item whose O waits for its epilogue
+            long long tile0;
+            int64_t row;
+            int t_begin, nt, real, head, live;
+            float mref, l;
+        } done;
+        done.nt = 0;
+        auto epilogue = [&] {
+            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
+            __syncwarp();
+            tc_fence_after();
+            const bool whole = done.t_begin == 0 && done.nt == done.real;
+            const float mref = done.mref, l = done.l;
+            constexpr int kSlot = RB * (D + 2);
+            float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (done.t_begin == 0 ? 1 : 0)) * kSlot;
+            const bool live = ok && done.live;
+            __nv_bfloat16* out =
+                static_cast<__nv_bfloat16*>(a.out) + done.row * a.o_rs + static_cast<int64_t>(done.head) * a.o_hs;
+            // 16 consecutive results of this row from element d on
+            auto put16 = [&](const float* o, int d, float inv, bool none) {
+                uint32_t wd[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : o[2 * k] * inv, none ? 0.0f : o[2 * k + 1] * inv);
+                    wd[k] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                if (a.o_vec) {
+                    stg_v8(out + d, wd);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        out[d + 2 * k] = __ushort_as_bfloat16(static_cast<unsigned short>(wd[k]));
+                        out[d + 2 * k + 1] = __ushort_as_bfloat16(static_cast<unsigned short>(wd[k] >> 16));
+                    }
+                }
+            };
+            auto put_lse = [&](float mm, float ll) {
+                if (a.lse && half == 0)
+                    a.lse[done.row * a.Hq + done.head] = ll == 0.0f ? -INFINITY : (mm - kQryBoost + log2f(ll)) * 0.6931471805599453f;
+            };
+            const float inv = 1.0f / l;
+            const bool none = mref == -INFINITY && l == 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 32) {
+                const int d = half * (D / 2) + c;
+                float o[32];
+                tc_ld32(lanes + kO + d, o);
+                tc_wait_ld();
+                if (whole) {
+                    if (live) {
+                        put16(o, d, inv, none);
+                        put16(o + 16, d + 16, inv, none);
+                    }
+                } else if (ok) {
+                    // element-major, so that a warp's stores are contiguous
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) slot[(d + j) * RB + row] = o[j];
+                }
+            }
+            tc_fence_before();
+            if (whole) {
+                if (live) put_lse(mref, l);
+            } else {
+                if (half == 0 && ok) {
+                    slot[RB * D + row] = mref;
+                    slot[RB * D + RB + row] = l;
+                }
+                const int c_first = key_owner(done.tile0, s_range.total, s_range.grid),
+                          c_last = key_owner(done.tile0 + done.real - 1, s_range.total, s_range.grid);
+                if (!named_bar_or(1, kQrySoft, !ok)) {
+                    if (tid == 0) {
+                        const unsigned got = atom_add_acq_rel(a.counters + c_first, 1u);
+                        s_last = got + 1 == static_cast<unsigned>(c_last - c_first + 1);
+                        if (s_last) a.counters[c_first] = 0;
+                    }
+                    named_bar_sync(1, kQrySoft);
+                    if (s_last) {
+                        auto part_of = [&](int c) {
+                            return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
+                        };
+                        float mm = -INFINITY, ll = 0.0f;
+                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + row));
+                        for (int c = c_first; c <= c_last; ++c) {
+                            const float* p = part_of(c) + RB * D + row;
+                            const float mc = __ldcg(p);
+                            ll = fmaf(__ldcg(p + RB), mc == mm ? 1.0f : exp2f(mc - mm), ll);
+                        }
+                        const float linv = 1.0f / ll;
+#pragma unroll 1
+                        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
+                            float o[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = 0.0f;
+                            for (int c = c_first; c <= c_last; ++c) {
+                                const float* p = part_of(c);
+                                const float mc = __ldcg(p + RB * D + row);
+                                const float fc = mc == mm ? 1.0f : exp2f(mc - mm);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = fmaf(__ldcg(p + (d + j) * RB + row), fc, o[j]);
+                            }
+                            if (live) put16(o, d, linv, mm == -INFINITY && ll == 0.0f);
+                        }
+                        if (live) put_lse(mm, ll);
+                    }
+                }
+            }
+        };
+        KeyWalk<RB, kQryLead> w(a, s_range);
         while (w.unit < w.end) {
             int lim_min, lim_max;
             key_limits<RB>(a, w.r, w.block(), lim_min, lim_max);
-            const int cnt = w.count();
-            const int real = max(1, (lim_max + kKeyTile - 1) / kKeyTile);
-            const int t_begin = w.tile, nt = min(w.tile + cnt, real) - w.tile;
+            int t_begin, t_end, real;
+            w.span(t_begin, t_end, real);
+            const int nt = t_end - t_begin;
             if (nt <= 0) {
-                w.next(cnt);
+                w.next();
                 continue;
             }
-            ok = ok && mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag);
             const int nrow = min(RB, w.r.m * a.group - w.block() * RB);
-            const float frow = s_frow[row];
-            const int lim = s_lim[row];
-            mbar_arrive(&q_free);
+            const int f = w.block() * RB + min(row, nrow - 1), tok = f / a.group, head = w.h * a.group + f % a.group;
+            const int lim = row < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
+            float frow;
+            {   // this half of the row: exact scaling to a largest magnitude in [2^7, 2^8), two terms
+                const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
+                                         static_cast<int64_t>(w.r.row0 + tok) * a.q_rs + static_cast<int64_t>(head) * a.q_hs +
+                                         half * H;
+                uint32_t x[H / 2];
+                if (a.q_vec) {
+#pragma unroll
+                    for (int c = 0; c < H / 2; c += 8) ldg_v8(x + c, q + 2 * c);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < H / 2; ++c)
+                        x[c] = __bfloat16_as_ushort(q[2 * c]) | static_cast<uint32_t>(__bfloat16_as_ushort(q[2 * c + 1])) << 16;
+                }
+                uint32_t top = 0;  // two largest magnitudes, NaN kept
+#pragma unroll
+                for (int c = 0; c < H / 2; ++c) top = bf16x2_max_nan(top, x[c] & 0x7fff7fffu);
+                float amax = bf16lo(top) <= 3.402823466e38f && bf16hi(top) <= 3.402823466e38f ? fmaxf(bf16lo(top), bf16hi(top))
+                                                                                             : INFINITY;
+                s_max[half][row] = amax;
+                named_bar_sync(2 + wq, 64);
+                amax = fmaxf(s_max[0][row], s_max[1][row]);
+                named_bar_sync(2 + wq, 64);
+                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
+                frow = a.scale_log2 * __int_as_float((127 + ex) << 23);
+                // a row with NaN or Inf becomes NaN, a row behind the last zero
+                const float mul = row >= nrow ? 0.0f : amax == INFINITY ? __int_as_float(0x7fc00000) : __int_as_float((127 - ex) << 23);
+#pragma unroll
+                for (int u = 0; u < H / 16; ++u) {  // 16 elements: one 16-byte unit of each term
+                    uint32_t t0[8], t1[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        e4m3_terms2(bf16lo(x[u * 8 + j]) * mul, bf16hi(x[u * 8 + j]) * mul, t0[j], t1[j]);
+                    const int d = half * H + u * 16;
+                    uint8_t* dst = s_q + (d / CW) * (RB * CW) + f8_unit<CW>(row, (d % CW) / 16);
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(t0[0] | (t0[1] << 16), t0[2] | (t0[3] << 16),
+                                                                t0[4] | (t0[5] << 16), t0[6] | (t0[7] << 16));
+                    *reinterpret_cast<uint4*>(dst + S::kTerm) = make_uint4(t1[0] | (t1[1] << 16), t1[2] | (t1[3] << 16),
+                                                                           t1[4] | (t1[5] << 16), t1[6] | (t1[7] << 16));
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&q_ready);
+            }
+            if (done.nt) epilogue();
             float mref = -INFINITY, l = 0.0f;
             bool nan_row = false;
 
@@ -406,114 +494,20 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 mbar_arrive(&p_ready[x & 1u]);
             }
             t += nt;
-            ++item;
-            // both halves' sums, then O
+            // both halves' sums
             s_l[half][row] = l;
-            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
             named_bar_sync(2 + wq, 64);
-            l = s_l[0][row] + s_l[1][row];
+            done.l = s_l[0][row] + s_l[1][row];
             named_bar_sync(2 + wq, 64);
-            tc_fence_after();
-
-            const long long item0 = w.unit - t_begin;
-            const bool whole = t_begin == 0 && nt == real;
-            constexpr int kSlot = RB * (D + 2);
-            float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
-            const int fq = w.block() * RB + row;
-            const int64_t orow = w.r.row0 + fq / a.group;
-            const int head = w.h * a.group + fq % a.group;
-            const bool live = ok && row < nrow;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + orow * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
-            // 16 consecutive results of this row from element d on
-            auto put16 = [&](const float* o, int d, float inv, bool none) {
-                if (a.o_vec) {
-#pragma unroll
-                    for (int j = 0; j < 16; j += 8) {
-                        uint32_t wd[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(none ? 0.0f : o[j + 2 * k] * inv,
-                                                                           none ? 0.0f : o[j + 2 * k + 1] * inv);
-                            wd[k] = *reinterpret_cast<const uint32_t*>(&b);
-                        }
-                        *reinterpret_cast<uint4*>(out + d + j) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) out[d + j] = __float2bfloat16_rn(none ? 0.0f : o[j] * inv);
-                }
-            };
-            auto put_lse = [&](float mm, float ll) {
-                if (a.lse && half == 0)
-                    a.lse[orow * a.Hq + head] = ll == 0.0f ? -INFINITY : (mm - kQryBoost + log2f(ll)) * 0.6931471805599453f;
-            };
-            const float inv = 1.0f / l;
-            const bool none = mref == -INFINITY && l == 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < D / 2; c += 32) {
-                const int d = half * (D / 2) + c;
-                float o[32];
-                tc_ld32(lanes + kO + d, o);
-                tc_wait_ld();
-                if (whole) {
-                    if (live) {
-                        put16(o, d, inv, none);
-                        put16(o + 16, d + 16, inv, none);
-                    }
-                } else if (ok) {
-                    // element-major, so that a warp's stores are contiguous
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) slot[(d + j) * RB + row] = o[j];
-                }
-            }
-            tc_fence_before();
-            if (whole) {
-                if (live) put_lse(mref, l);
-            } else {
-                if (half == 0 && ok) {
-                    slot[RB * D + row] = mref;
-                    slot[RB * D + RB + row] = l;
-                }
-                const int c_first = key_owner(item0, total, grid), c_last = key_owner(item0 + real - 1, total, grid);
-                if (!named_bar_or(1, kQrySoft, !ok)) {
-                    if (tid == 0) {
-                        const unsigned got = atom_add_acq_rel(a.counters + c_first, 1u);
-                        s_last = got + 1 == static_cast<unsigned>(c_last - c_first + 1);
-                        if (s_last) a.counters[c_first] = 0;
-                    }
-                    named_bar_sync(1, kQrySoft);
-                    if (s_last) {
-                        auto part_of = [&](int c) {
-                            return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
-                        };
-                        float mm = -INFINITY, ll = 0.0f;
-                        for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + row));
-                        for (int c = c_first; c <= c_last; ++c) {
-                            const float* p = part_of(c) + RB * D + row;
-                            const float mc = __ldcg(p);
-                            ll = fmaf(__ldcg(p + RB), mc == mm ? 1.0f : exp2f(mc - mm), ll);
-                        }
-                        const float linv = 1.0f / ll;
-#pragma unroll 1
-                        for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 16) {
-                            float o[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = 0.0f;
-                            for (int c = c_first; c <= c_last; ++c) {
-                                const float* p = part_of(c);
-                                const float mc = __ldcg(p + RB * D + row);
-                                const float fc = mc == mm ? 1.0f : exp2f(mc - mm);
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = fmaf(__ldcg(p + (d + j) * RB + row), fc, o[j]);
-                            }
-                            if (live) put16(o, d, linv, mm == -INFINITY && ll == 0.0f);
-                        }
-                        if (live) put_lse(mm, ll);
-                    }
-                }
-            }
-            w.next(cnt);
+            done.mref = mref;
+            done.tile0 = w.tile0();
+            done.row = w.r.row0 + tok;
+            done.head = head;
+            done.live = row < nrow;
+            done.t_begin = t_begin, done.nt = nt, done.real = real;
+            w.next();
         }
+        if (done.nt) epilogue();
     }
     tc_fence_before();
     __syncthreads();
@@ -541,6 +535,7 @@ cudaError_t launch_kv8_queries(const dm_kv8_cache* c, const Kv8AttnArgs& a, int 
     QryArgs qa{};
     if (!kv8_encode_map(c, &qa.map)) return cudaErrorNotSupported;
     qa.a = a;
+    qa.a.exact = kv8_exact(a, kQryRows);
     if (c->head_dim == 64) return launch_queries<64>(qa, num_sms, dev, s);
     if (c->head_dim == 128) return launch_queries<128>(qa, num_sms, dev, s);
     return launch_queries<256>(qa, num_sms, dev, s);

@@ -102,6 +102,25 @@ DM_DEV void e4m3_terms2(float a, float b, uint32_t& t0, uint32_t& t1) {
     t1 = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(__hsub2(h, back)), __NV_SATFINITE, __NV_E4M3);
 }
 
+// 32 bytes of one thread (32-byte aligned): whole sectors where every lane has a row of its own
+DM_DEV void ldg_v8(uint32_t* v, const void* p) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(p));
+}
+DM_DEV void stg_v8(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// larger of each half (bf16 pairs); NaN wins
+DM_DEV uint32_t bf16x2_max_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // 2^x of the special function unit (relative error 2^-22; results below 2^-126 become 0)
 DM_DEV float ex2(float x) {
     float y;

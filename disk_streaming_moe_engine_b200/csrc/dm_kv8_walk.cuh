@@ -51,6 +51,19 @@ DM_DEV KeyReq key_req(const Kv8AttnArgs& a, const KeyRaw& w, bool report) {
     return r;
 }
 
+constexpr int kKeyFew = 64;  // requests whose words a CTA keeps in shared memory
+
+struct KeyRange {  // a CTA's range of the sequence [u0, u1), and where it starts
+    long long u0, u1, total, rem;
+    long long grid;
+    int req, blk;
+    KeyRaw raw[kKeyFew];
+    DM_DEV KeyRaw request(const Kv8AttnArgs& a, int i) const {
+        if (a.n <= kKeyFew && i < a.n) return raw[i];
+        return key_raw(a, i);
+    }
+};
+
 // keys that a block's rows see: every row those before lo, its last token's rows those before hi
 template <int RB>
 DM_DEV void key_limits(const Kv8AttnArgs& a, const KeyReq& r, int blk, int& lo, int& hi) {
@@ -60,97 +73,204 @@ DM_DEV void key_limits(const Kv8AttnArgs& a, const KeyReq& r, int blk, int& lo, 
     hi = min(r.len, max(0, r.full - r.m + last + 1));
 }
 
-// Position in the sequence of all items' tiles: request, then row block (first, last, second,
-// second to last, ...: under a causal mask neighbours then cost the same together), kv head,
-// tile.  Every block has the tiles of the request's whole length there; those that its rows do
-// not see are skipped.
+// Tiles that a block's rows see (an item without keys has one, so that its rows are written).
 template <int RB>
+DM_DEV int key_tiles(const Kv8AttnArgs& a, const KeyReq& r, int blk) {
+    int lo, hi;
+    key_limits<RB>(a, r, blk, lo, hi);
+    return max(1, (hi + kKeyTile - 1) / kKeyTile);
+}
+
+// Position in the sequence of all items: request, then row block, kv head.  An item has LEAD
+// units for its start and end and one per tile; the CTA whose range holds a tile's unit works on
+// it.  exact: a block has the tiles that its rows see.  Else every block has those of the
+// request's whole length (what its rows do not see is skipped) and the blocks come as first,
+// last, second, second to last, ...: under a causal mask neighbours then cost the same together.
+template <int RB, int LEAD>
 struct KeyWalk {
     const Kv8AttnArgs& a;
+    const KeyRange& range;
     long long unit, end;  // this CTA's range
-    int req, blk, h, tile;
+    int req, blk, h, pos, tiles;
     KeyReq r;
     KeyRaw ahead;  // of request req + 1, loaded before it is needed
-    DM_DEV KeyWalk(const Kv8AttnArgs& args, long long u0, long long u1, int rq, long long rem) : a(args), unit(u0), end(u1) {
-        req = rq;
-        r = key_req<RB>(a, key_raw(a, req), false);
-        ahead = key_raw(a, req + 1);
-        tile = static_cast<int>(rem % r.tiles);
-        const long long q = rem / r.tiles;
-        h = static_cast<int>(q % a.Hkv);
-        blk = static_cast<int>(q / a.Hkv);
+    DM_DEV KeyWalk(const Kv8AttnArgs& args, const KeyRange& k)
+        : a(args), range(k), unit(k.u0), end(k.u1), req(k.req), blk(k.blk) {
+        r = key_req<RB>(a, range.request(a, req), false);
+        ahead = range.request(a, req + 1);
+        tiles = a.exact ? key_tiles<RB>(a, r, blk) : r.tiles;
+        pos = static_cast<int>(k.rem % (tiles + LEAD));
+        h = static_cast<int>(k.rem / (tiles + LEAD));
     }
-    DM_DEV int block() const { return blk & 1 ? r.blocks - 1 - (blk >> 1) : blk >> 1; }
-    // tiles of the current item in the range: [tile, tile + count) of the sequence
-    DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(r.tiles - tile), end - unit)); }
-    DM_DEV void next(int cnt) {
-        unit += cnt;
+    DM_DEV int block() const { return a.exact ? blk : blk & 1 ? r.blocks - 1 - (blk >> 1) : blk >> 1; }
+    DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(tiles + LEAD - pos), end - unit)); }
+    // this CTA's tiles of the item: [first, last) of the `real` ones that its rows see
+    DM_DEV void span(int& first, int& last, int& real) const {
+        real = a.exact ? tiles : key_tiles<RB>(a, r, block());
+        first = max(0, pos - LEAD);
+        last = min(real, max(0, pos + count() - LEAD));
+    }
+    DM_DEV long long tile0() const { return unit - pos + LEAD; }  // the unit of the item's first tile
+    DM_DEV void next() {
+        unit += count();
         if (unit >= end) return;
-        tile = 0;
+        pos = 0;
         if (++h < a.Hkv) return;
         h = 0;
-        if (++blk < r.blocks) return;
-        blk = 0;
-        do {
-            if (++req >= a.n) {  // only if the lengths changed under the kernel
-                end = unit;
-                return;
-            }
-            r = key_req<RB>(a, ahead, false);
-            ahead = key_raw(a, req + 1);
-        } while (r.blocks == 0);
+        if (++blk >= r.blocks) {
+            blk = 0;
+            do {
+                if (++req >= a.n) {  // only if the lengths changed under the kernel
+                    end = unit;
+                    return;
+                }
+                r = key_req<RB>(a, ahead, false);
+                ahead = range.request(a, req + 1);
+            } while (r.blocks == 0);
+        }
+        tiles = a.exact ? key_tiles<RB>(a, r, blk) : r.tiles;
     }
 };
 
-// This CTA's range [u0, u1) of the sequence and where it starts: every thread sums its share of
-// the requests, one block-wide scan.  At most one CTA per `min_tiles` tiles takes part; false:
-// this one does not.  Called by all NT threads; ends with a barrier.
-template <int RB, int NT>
-DM_DEV bool key_range(const Kv8AttnArgs& a, int min_tiles, long long* s_sum, int* s_req, long long* s_rem, long long& u0,
-                      long long& u1, long long& total, long long& grid) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int per = (a.n + NT - 1) / NT;
-    const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
-    auto tiles_of = [&](int i, bool report) {
-        const KeyReq r = key_req<RB>(a, key_raw(a, i), report);
-        return static_cast<long long>(r.blocks) * a.Hkv * r.tiles;
-    };
-    long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += tiles_of(i, blockIdx.x == 0);
-    long long pre = mine;
+template <typename V>
+DM_DEV V warp_scan(V v) {  // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, pre, o);
-        if (lane >= o) pre += y;
+        const V y = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += y;
     }
-    if (lane == 31) s_sum[warp] = pre;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w == warp) pre += total - mine;  // tiles before this thread's requests
-        total += s_sum[w];
-    }
-    grid = min(static_cast<long long>(gridDim.x), (total + min_tiles - 1) / min_tiles);
-    const bool active = blockIdx.x < grid;
-    u0 = active ? total * blockIdx.x / grid : 0;
-    u1 = active ? total * (blockIdx.x + 1) / grid : 0;
-    if (active && u0 >= pre && u0 < pre + mine) {
-        long long at = pre;
-        for (int i = i0; i < i1; ++i) {
-            const long long c = tiles_of(i, false);
-            if (u0 < at + c) {
-                *s_req = i;
-                *s_rem = u0 - at;
-                break;
+    return v;
+}
+
+// This CTA's range of the sequence and where it starts.  At most one CTA per `min_units` units
+// takes part; false: this one does not.  Up to 64 requests: a warp per request, a lane per
+// block; more: a thread per share of the requests (whose blocks are few where `exact` is set).
+// Called by all NT threads with s_sum [kKeyFew]; ends with a barrier.
+template <int RB, int LEAD, int NT>
+DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, KeyRange* out) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool report = blockIdx.x == 0;
+    long long total, u0 = 0;
+    bool active;
+    auto cut = [&] {
+        const long long grid = min(static_cast<long long>(gridDim.x), (total + min_units - 1) / min_units);
+        active = blockIdx.x < grid;
+        u0 = active ? total * blockIdx.x / grid : 0;
+        if (tid == 0) {
+            out->total = total;
+            out->grid = grid;
+            out->u0 = u0;
+            out->u1 = active ? total * (blockIdx.x + 1) / grid : 0;
+        }
+    };
+    if (a.n <= kKeyFew) {
+        if (tid < a.n) {
+            out->raw[tid] = key_raw(a, tid);
+            key_req<RB>(a, out->raw[tid], report);
+        }
+        __syncthreads();
+        for (int i = warp; i < a.n; i += NT / 32) {
+            const KeyReq r = key_req<RB>(a, out->raw[i], false);
+            long long sum = 0;
+            if (a.exact)
+                for (int b = lane; b < r.blocks; b += 32) sum += key_tiles<RB>(a, r, b) + LEAD;
+            else if (lane == 0)
+                sum = static_cast<long long>(r.blocks) * (r.tiles + LEAD);
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) s_sum[i] = sum * a.Hkv;
+        }
+        __syncthreads();
+        const long long v0 = lane < a.n ? s_sum[lane] : 0, v1 = lane + 32 < a.n ? s_sum[lane + 32] : 0;
+        const long long e0 = warp_scan(v0), t0 = __shfl_sync(0xffffffffu, e0, 31), e1 = t0 + warp_scan(v1);
+        total = __shfl_sync(0xffffffffu, e1, 31);
+        cut();
+        if (active && warp == 0) {
+            const unsigned m0 = __ballot_sync(0xffffffffu, u0 >= e0 - v0 && u0 < e0);
+            const unsigned m1 = __ballot_sync(0xffffffffu, u0 >= e1 - v1 && u0 < e1);
+            const int src = m0 ? __ffs(m0) - 1 : __ffs(m1) - 1;
+            const int req = m0 ? src : src + 32;
+            long long rem = u0 - (m0 ? __shfl_sync(0xffffffffu, e0 - v0, src) : __shfl_sync(0xffffffffu, e1 - v1, src));
+            const KeyReq r = key_req<RB>(a, out->raw[req], false);
+            int blk = 0;
+            if (a.exact) {  // 32 blocks at a time
+                for (;; blk += 32) {
+                    const long long c =
+                        blk + lane < r.blocks ? static_cast<long long>(key_tiles<RB>(a, r, blk + lane) + LEAD) * a.Hkv : 0;
+                    const long long e = warp_scan(c), all = __shfl_sync(0xffffffffu, e, 31);
+                    if (rem >= all && blk + 32 < r.blocks) {
+                        rem -= all;
+                        continue;
+                    }
+                    const unsigned m = __ballot_sync(0xffffffffu, rem < e);
+                    const int at = m ? __ffs(m) - 1 : 0;
+                    rem -= __shfl_sync(0xffffffffu, e - c, at);
+                    blk += at;
+                    break;
+                }
+            } else {
+                const long long c = static_cast<long long>(r.tiles + LEAD) * a.Hkv;
+                blk = static_cast<int>(rem / c);
+                rem -= blk * c;
             }
-            at += c;
+            if (lane == 0) {
+                out->req = req;
+                out->blk = blk;
+                out->rem = rem;
+            }
+        }
+    } else {
+        const int per = (a.n + NT - 1) / NT;
+        const int i0 = min(a.n, tid * per), i1 = min(a.n, i0 + per);
+        auto blocks_of = [&](int i, bool rep, auto&& each) {  // each(block, its units over the kv heads, ...) until true
+            const KeyReq r = key_req<RB>(a, key_raw(a, i), rep);
+            for (int b = 0; b < r.blocks; ++b) {
+                if (!a.exact) {  // all at once
+                    const long long c = static_cast<long long>(r.tiles + LEAD) * a.Hkv;
+                    return each(0, c * r.blocks, c);
+                }
+                const long long c = static_cast<long long>(key_tiles<RB>(a, r, b) + LEAD) * a.Hkv;
+                if (each(b, c, c)) return true;
+            }
+            return false;
+        };
+        long long mine = 0;
+        for (int i = i0; i < i1; ++i)
+            blocks_of(i, report, [&](int, long long c, long long) {
+                mine += c;
+                return false;
+            });
+        long long pre = warp_scan(mine);
+        if (lane == 31) s_sum[warp] = pre;
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < NT / 32; ++w) {
+            if (w == warp) pre += total - mine;  // tiles before this thread's requests
+            total += s_sum[w];
+        }
+        cut();
+        if (active && u0 >= pre && u0 < pre + mine) {
+            long long at = pre;
+            for (int i = i0; i < i1; ++i)
+                if (blocks_of(i, false, [&](int b, long long c, long long one) {
+                        if (u0 >= at + c) {
+                            at += c;
+                            return false;
+                        }
+                        const long long skip = (u0 - at) / one;
+                        out->req = i;
+                        out->blk = b + static_cast<int>(skip);
+                        out->rem = u0 - at - skip * one;
+                        return true;
+                    }))
+                    break;
         }
     }
     __syncthreads();
     return active;
 }
 
-// The CTA whose range holds tile u.
+// The CTA whose range holds unit u.
 DM_DEV int key_owner(long long u, long long total, long long grid) { return static_cast<int>(((u + 1) * grid - 1) / total); }
 
 // Shared memory of the key tiles: a ring of SL slots.  PAIR: a slot takes a tile's K and V and is
@@ -188,13 +308,13 @@ struct KeyRing {
 // Producer (one warp): a tile's K or V as TMA boxes of 16 token rows by CW bytes, one lane per
 // page; page ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A
 // page that is missing or holds no key of the item reads zeros.
-template <int RB, int D, int SL, bool PAIR>
-DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, KeyRing<SL, PAIR>& ring, long long u0,
-                        long long u1, int req, long long rem, volatile int* abort_flag) {
+template <int RB, int LEAD, int D, int SL, bool PAIR>
+DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, KeyRing<SL, PAIR>& ring,
+                        const KeyRange& range, volatile int* abort_flag) {
     constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW, kSlot = (PAIR ? 2 : 1) * kKeyTile * D;
     const int lane = threadIdx.x & 31;
     bool ok = true;
-    KeyWalk<RB> w(a, u0, u1, req, rem);
+    KeyWalk<RB, LEAD> w(a, range);
     int ti = -1, ei = 0, hi = 0;  // next tile of w's item, end of its tiles, its keys
     struct Group {
         int count = 0;             // tiles
@@ -206,10 +326,9 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
         g = Group();
         while (g.count < 32 / kKeyPages && w.unit < w.end) {
             if (ti < 0) {
-                int lo;
+                int lo, real;
                 key_limits<RB>(a, w.r, w.block(), lo, hi);
-                ti = w.tile;
-                ei = min(w.tile + w.count(), max(1, (hi + kKeyTile - 1) / kKeyTile));
+                w.span(ti, ei, real);
             }
             if (ti < ei) {
                 const int p = ti * kKeyPages + lane % kKeyPages;
@@ -221,7 +340,7 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
                 ++g.count;
                 ++ti;
             } else {
-                w.next(w.count());
+                w.next();
                 ti = -1;
             }
         }

@@ -560,6 +560,17 @@ def test_attention_chunks(lib, dtype, hk, grp, d, lens, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,len_hi,q_hi", [(65, 300, 1), (97, 500, 4), (70, 150, 40), (80, 40, 40), (600, 30, 1)])
+def test_attention_many_requests(lib, dtype, n, len_hi, q_hi):
+    """More than 64 requests, empty ones and ones without a query among them."""
+    g = np.random.default_rng(n)
+    lens, rows = g.integers(0, len_hi + 1, n), g.integers(0, q_hi + 1, n)
+    rows = np.minimum(rows, np.maximum(lens, 1))
+    check_attention([int(x) for x in lens], [int(x) for x in rows], 1, 8, 64, dtype, seed=n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attention_long_prompt(lib, dtype):
     check_attention([601, 300], [601, 129], 1, 2, 128, dtype, seed=3)
 
