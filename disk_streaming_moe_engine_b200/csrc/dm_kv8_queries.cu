@@ -16,9 +16,11 @@
 // threads, 64 keys of the tile each, that meet at a 64-thread barrier to agree on M; O is
 // rescaled only by warps with a raised row.
 //
-// Roles (320 threads): 8 softmax warps (two per quarter of the rows), a producer and an MMA warp.
-// The scores of tile x + 1 follow as soon as those of tile x are in registers and run before the
-// O product of tile x, so the softmax has the time of two products.  Between items the softmax
+// Roles (352 threads): 8 softmax warps (two per quarter of the rows), a producer warp, one warp
+// that issues the scores and one that issues the O products (each is held up by the tensor cores'
+// short queue and by its own waits; together they keep the queue filled).  The scores of tile x + 1
+// follow as soon as those of tile x are in registers and mostly run before the O product of tile
+// x, so the softmax has the time of two products.  Between items the softmax
 // warps turn the next item's q rows into terms while the last O product runs, then write the
 // item's O while the next scores run (two separate warps for the terms were slower: the
 // conversions are ALU work that all four schedulers have to share).  Tensor memory: the scores
@@ -34,8 +36,8 @@ namespace dm {
 
 constexpr int kQryRows = 128;
 constexpr int kQrySoft = 256;
-constexpr int kQryThreads = kQrySoft + 64;
-constexpr int kQryLead = 2;        // an item's start and end in tiles (KeyWalk)
+constexpr int kQryThreads = kQrySoft + 96;
+constexpr int kQryLead = 6;        // an item's start and end in tiles (KeyWalk)
 constexpr float kQryLazy = 2.0f;
 constexpr float kQryBoost = 6.0f;  // weights enter as 2^6 w <= 256
 
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     uint8_t* sm = qry_smem + ((1024u - (smem_u32(qry_smem) & 1023u)) & 1023u);
     uint8_t* s_q = sm + SL * S::kTileBytes;
     __shared__ __align__(8) KeyRing<SL, false> ring;
-    __shared__ __align__(8) uint64_t s_full, s_free, p_ready[2], pv_done[2], q_ready, done_bar;
+    __shared__ __align__(8) uint64_t s_full, s_free, p_ready[2], pv_done[2], q_ready, done_bar[2];
     __shared__ float s_max[2][RB], s_l[2][RB];
     __shared__ long long s_sum[64];
     __shared__ KeyRange s_range;
@@ -88,7 +90,8 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
         mbar_init(&s_full, 1);
         mbar_init(&s_free, kQrySoft);
         mbar_init(&q_ready, kQrySoft);
-        mbar_init(&done_bar, 1);
+        mbar_init(&done_bar[0], 1);
+        mbar_init(&done_bar[1], 1);
         mbar_fence_init();
         s_abort = 0;
     }
@@ -102,78 +105,71 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     if (active && warp == W_LOAD) {
         key_produce<RB, kQryLead, D, SL, false>(a, &qa.map, sm, ring, s_range, abort_flag);
     } else if (active && warp == W_MMA) {
-        // ---------------- MMA ----------------
+        // ---------------- scores ----------------
         if (lane == 0) {
             bool ok = true;
-            const uint32_t i_s = f8_idesc(128, kKeyTile, false, false), i_o = f8_idesc(128, D, false, true);
+            const uint32_t i_s = f8_idesc(128, kKeyTile, false, false);
             const uint32_t sq = smem_u32(s_q);
-            // scores run one tile ahead of the O products, across items too
             KeyWalk<RB, kQryLead> w(a, s_range);
-            uint32_t x = 0, sx = 0, item = 0;
-            int left = 0;         // score tiles left of the walked item
-            unsigned firsts = 0;  // bit (x & 1): tile x is its item's first
-            bool first = false;   // the next score tile is its item's first
-            enum { kNone, kIssued, kLater };
-            // S of the next tile; kLater: its item's terms are not ready and `wait` is not set
-            auto next_scores = [&](bool wait) -> int {
-                while (left == 0) {
-                    if (w.unit >= w.end) return kNone;
-                    int begin, last, real;
-                    w.span(begin, last, real);
-                    left = max(0, last - begin);
-                    w.next();
-                    first = left > 0;
+            uint32_t x = 0, item = 0;
+            while (w.unit < w.end && ok) {
+                int begin, last, real;
+                w.span(begin, last, real);
+                if (last > begin) ok = mbar_wait_bounded(&q_ready, item++ & 1u, a.err, abort_flag);
+                for (; begin < last && ok; ++begin, ++x) {
+                    const uint32_t ld = ring.k_load(x);
+                    ok = ring.wait_full(ld, a.err, abort_flag) && mbar_wait_bounded(&s_free, (x & 1u) ^ 1u, a.err, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t k = smem_u32(sm + (ld % SL) * S::kTileBytes);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int c = 0; c < S::kChunks; ++c) {
+                            const uint64_t ad = f8_desc_k<CW>(sq + t * S::kTerm + c * (RB * CW));
+                            const uint64_t bd = f8_desc_k<CW>(k + c * (kKeyTile * CW));
+#pragma unroll
+                            for (int j = 0; j < CW / 32; ++j)
+                                f8_mma(tmem, ad + 2 * j, bd + 2 * j, i_s, t > 0 || c > 0 || j > 0);
+                        }
+                    tc_commit(&s_full);
+                    tc_commit(&ring.empty[ld % SL]);
                 }
-                if (first && !mbar_try_wait(&q_ready, item & 1u)) {
-                    if (!wait) return kLater;
-                    if (!(ok = mbar_wait_bounded(&q_ready, item & 1u, a.err, abort_flag))) return kNone;
-                }
-                const uint32_t ld = ring.k_load(sx);
-                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return kNone;
-                if (!(ok = mbar_wait_bounded(&s_free, (sx & 1u) ^ 1u, a.err, abort_flag))) return kNone;
-                tc_fence_after();
-                const uint32_t k = smem_u32(sm + (ld % SL) * S::kTileBytes);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int c = 0; c < S::kChunks; ++c) {
-                        const uint64_t ad = f8_desc_k<CW>(sq + t * S::kTerm + c * (RB * CW));
-                        const uint64_t bd = f8_desc_k<CW>(k + c * (kKeyTile * CW));
-#pragma unroll
-                        for (int j = 0; j < CW / 32; ++j)
-                            f8_mma(tmem, ad + 2 * j, bd + 2 * j, i_s, t > 0 || c > 0 || j > 0);
-                    }
-                tc_commit(&ring.empty[ld % SL]);
-                tc_commit(&s_full);
-                firsts = (firsts & ~(1u << (sx & 1u))) | ((first ? 1u : 0u) << (sx & 1u));
-                first = false;
-                ++sx;
-                if (--left == 0) ++item;
-                return kIssued;
-            };
-            int more = next_scores(true);
-            while (more == kIssued && ok) {
-                more = next_scores(false);
-                if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
-                const uint32_t ld = ring.v_load(x);
-                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) break;
-                tc_fence_after();
-                const bool fresh = (firsts >> (x & 1u)) & 1u;
-                const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), kKeyTile * CW);
-                const uint32_t p = tmem + kPw + (x & 1u) * 64;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < kKeyTile / 32; ++j)
-                        f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o,
-                                  !fresh || t > 0 || j > 0);
-                tc_commit(&ring.empty[ld % SL]);
-                tc_commit(&pv_done[x & 1u]);
-                ++x;
-                if (more == kLater) more = next_scores(true);
+                w.next();
             }
-            tc_commit(&done_bar);
-            mbar_wait_bounded(&done_bar, 0, a.err, nullptr);
+            tc_commit(&done_bar[0]);
+            mbar_wait_bounded(&done_bar[0], 0, a.err, nullptr);
+        }
+    } else if (active && warp == W_MMA + 1) {
+        // ---------------- O products ----------------
+        if (lane == 0) {
+            bool ok = true;
+            const uint32_t i_o = f8_idesc(128, D, false, true);
+            KeyWalk<RB, kQryLead> w(a, s_range);
+            uint32_t x = 0;
+            while (w.unit < w.end && ok) {
+                int begin, last, real;
+                w.span(begin, last, real);
+                for (int i = begin; i < last && ok; ++i, ++x) {
+                    const uint32_t ld = ring.v_load(x);
+                    ok = ring.wait_full(ld, a.err, abort_flag) &&
+                         mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), kKeyTile * CW);
+                    const uint32_t p = tmem + kPw + (x & 1u) * 64;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < kKeyTile / 32; ++j)
+                            f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o, i > begin || t > 0 || j > 0);
+                    tc_commit(&pv_done[x & 1u]);
+                    tc_commit(&ring.empty[ld % SL]);
+                }
+                w.next();
+            }
+            tc_commit(&done_bar[1]);
+            mbar_wait_bounded(&done_bar[1], 0, a.err, nullptr);
         }
     } else if (active) {
         // ---------------- Q terms, softmax, epilogue ----------------
