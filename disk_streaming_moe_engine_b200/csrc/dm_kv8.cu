@@ -57,9 +57,10 @@ int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "CONFIG_ERROR", stage, "head_dim %d: 64, 128 or 256", c->head_dim);
     if (c->num_kv_heads < 1 || c->num_kv_heads > 1024 || c->num_pages < 1 || c->num_pages > (1 << 27) - 1 ||
-        c->reserved != 0)
+        (static_cast<int64_t>(c->num_pages) + 1) * 4 * c->num_kv_heads > 0x7fffffffLL || c->reserved != 0)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "CONFIG_ERROR", stage,
-                       "need 1 <= num_kv_heads <= 1024, 1 <= num_pages < 2^27, reserved 0");
+                       "need 1 <= num_kv_heads <= 1024, 1 <= num_pages < 2^27, 4 num_kv_heads (num_pages + 1) < 2^31, "
+                       "reserved 0");
     if (reinterpret_cast<uintptr_t>(c->pages) % 16 != 0 || reinterpret_cast<uintptr_t>(c->scales) % 4 != 0)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", stage, "pages must be 16-byte aligned");
     return DM_OK;

@@ -48,14 +48,14 @@ struct KeyShape {
     static constexpr int kThreads = kSoft + 64;
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
-    static constexpr int kTileBytes = kKeyTile * D;   // K or V of a tile
     static constexpr int kQ = kN * D;
     static constexpr int kP = kN * kKeyTile;          // one of two buffers
     static constexpr int kFixed = kQ + 2 * kP + 1024;
     // a tile's chain of waits takes about 0.65 us whatever D is, its bytes from HBM 0.37 us at
     // D = 64 and 1.5 us at D = 256: the smaller heads take two CTAs per SM
     static constexpr int kCtas = D <= 128 && RB == 8 ? 2 : 1;
-    static constexpr int kSlot = 2 * kTileBytes;      // K and V of a tile
+    using Tile = KeyTile<D, true>;                    // K and V of a tile
+    static constexpr int kSlot = Tile::kSlot;
     static constexpr int kFit = (kKeySmem / kCtas - 6144 - kFixed) / kSlot;  // static arrays and 1 KB per CTA beside it
     static constexpr int kSlots = kFit > kKeyMaxSlots ? kKeyMaxSlots : kFit;
     static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kSlot + kFixed;
@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                 const uint32_t k = smem_u32(sm + (ld % SL) * S::kSlot);
 #pragma unroll
                 for (int c = 0; c < S::kChunks; ++c) {
-                    const uint64_t ad = f8_desc_k<CW>(k + c * (kKeyTile * CW)), bd = f8_desc_k<CW>(sq + c * (N * CW));
+                    const uint64_t ad = f8_desc_k<CW>(k + c * S::Tile::kChunk, S::Tile::kGroup);
+                    const uint64_t bd = f8_desc_k<CW>(sq + c * (N * CW), 8 * CW);
 #pragma unroll
                     for (int j = 0; j < CW / 32; ++j) f8_mma(tmem + (x & 1u) * N, ad + 2 * j, bd + 2 * j, i_s, c > 0 || j > 0);
                 }
@@ -153,14 +154,14 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                         if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
                         tc_fence_after();
                         const uint32_t ld = ring.v_load(x);
-                        const uint32_t v = smem_u32(sm + (ld % SL) * S::kSlot) + S::kTileBytes;
+                        const uint32_t v = smem_u32(sm + (ld % SL) * S::kSlot) + S::Tile::kV;
                         const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
-                            const uint64_t ad = f8_desc_m<CW>(v + c * (kKeyTile * CW), 0);  // 64 wide: M rows 64-127 repeat 0-63
+                            const uint64_t ad = f8_desc_m<CW>(v + c * S::Tile::kChunk, 0, S::Tile::kGroup);  // 64 wide: M rows 64-127 repeat 0-63
 #pragma unroll
                             for (int j = 0; j < kKeyTile / 32; ++j)
-                                f8_mma(tmem + (2 + c) * N, ad + j * (32 * CW / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
+                                f8_mma(tmem + (2 + c) * N, ad + j * (4 * S::Tile::kGroup / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
                         }
                         tc_commit(&ring.empty[ld % SL]);
                         tc_commit(&pv_done[x & 1u]);
@@ -334,18 +335,18 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     // becomes 0 and makes the sums of the rows that see it NaN
                     if (r0 == 0) {
                         ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
-                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kSlot + S::kTileBytes + tt * CW;
+                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kSlot + S::Tile::kV + S::Tile::row(tt);
                         bool nan = false;
                         if (key >= lim_max) {
 #pragma unroll
                             for (int c = 0; c < S::kChunks; ++c)
                                 for (int u = 0; u < CW / 16; ++u)
-                                    *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
+                                    *reinterpret_cast<uint4*>(v + c * S::Tile::kChunk + u * 16) = make_uint4(0, 0, 0, 0);
                         } else if (key >= lim_min) {
 #pragma unroll
                             for (int c = 0; c < S::kChunks; ++c)
                                 for (int u = 0; u < CW / 4; ++u) {
-                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
+                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * S::Tile::kChunk) + u;
                                     const uint32_t bad = e4m3_nan_mask(*p);
                                     if (bad) {
                                         *p &= ~bad;
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     }
 }
 
-bool kv8_encode_map(const dm_kv8_cache* c, CUtensorMap* map) {
+bool kv8_encode_map(const dm_kv8_cache* c, bool pair, CUtensorMap* map) {
     typedef CUresult (*Fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -537,11 +538,11 @@ bool kv8_encode_map(const dm_kv8_cache* c, CUtensorMap* map) {
     }();
     if (!fn) return false;
     const cuuint32_t cw = c->head_dim >= 128 ? 128 : 64;
-    const cuuint64_t rows = 2ull * c->num_kv_heads * kKv8Page;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c->head_dim), rows, static_cast<cuuint64_t>(c->num_pages)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c->head_dim), rows * c->head_dim};
-    const cuuint32_t box[3] = {cw, kKv8Page, 1}, estr[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c->pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t d = static_cast<cuuint64_t>(c->head_dim), chunks = d / cw, hkv = static_cast<cuuint64_t>(c->num_kv_heads);
+    const cuuint64_t dims[5] = {cw, 8, chunks, 2, 4 * hkv * static_cast<cuuint64_t>(c->num_pages)};
+    const cuuint64_t strides[4] = {d, cw, hkv * kKv8Page * d, 8 * d};
+    const cuuint32_t box[5] = {cw, 8, static_cast<cuuint32_t>(chunks), pair ? 2u : 1u, 2}, estr[5] = {1, 1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c->pages, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               cw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -571,7 +572,7 @@ static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev,
 // for 16 rows), else 8.
 cudaError_t launch_kv8_keys(const dm_kv8_cache* c, const Kv8AttnArgs& a, bool f32, int num_sms, int dev, cudaStream_t s) {
     KeyArgs ka{};
-    if (!kv8_encode_map(c, &ka.map)) return cudaErrorNotSupported;
+    if (!kv8_encode_map(c, true, &ka.map)) return cudaErrorNotSupported;
     ka.a = a;
     const bool wide = static_cast<int64_t>(a.max_q) * a.group > 8;
     ka.a.exact = kv8_exact(a, wide ? 16 : 8);

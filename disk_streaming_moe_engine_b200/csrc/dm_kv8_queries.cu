@@ -46,7 +46,8 @@ template <int D>
 struct QryShape {
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
-    static constexpr int kTileBytes = kKeyTile * D;
+    using Tile = KeyTile<D, false>;
+    static constexpr int kTileBytes = Tile::kSlot;
     static constexpr int kTerm = kQryRows * D;  // one term of Q
     static constexpr int kFixed = 2 * kTerm + 1024;
     static constexpr int kFit = (227 * 1024 - 6144 - kFixed) / kTileBytes;
@@ -127,8 +128,8 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
-                            const uint64_t ad = f8_desc_k<CW>(sq + t * S::kTerm + c * (RB * CW));
-                            const uint64_t bd = f8_desc_k<CW>(k + c * (kKeyTile * CW));
+                            const uint64_t ad = f8_desc_k<CW>(sq + t * S::kTerm + c * (RB * CW), 8 * CW);
+                            const uint64_t bd = f8_desc_k<CW>(k + c * S::Tile::kChunk, S::Tile::kGroup);
 #pragma unroll
                             for (int j = 0; j < CW / 32; ++j)
                                 f8_mma(tmem, ad + 2 * j, bd + 2 * j, i_s, t > 0 || c > 0 || j > 0);
@@ -157,13 +158,13 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                          mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), kKeyTile * CW);
+                    const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), S::Tile::kChunk, S::Tile::kGroup);
                     const uint32_t p = tmem + kPw + (x & 1u) * 64;
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int j = 0; j < kKeyTile / 32; ++j)
-                            f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (32 * CW / 16), i_o, i > begin || t > 0 || j > 0);
+                            f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (4 * S::Tile::kGroup / 16), i_o, i > begin || t > 0 || j > 0);
                     tc_commit(&pv_done[x & 1u]);
                     tc_commit(&ring.empty[ld % SL]);
                 }
@@ -477,19 +478,19 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     // becomes 0 and makes the sums of the rows that see it NaN
                     if (half == 0) {
                         ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
-                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kTileBytes + row * CW;
+                        uint8_t* v = sm + (ring.v_load(x) % SL) * S::kTileBytes + S::Tile::row(row);
                         const int key = tile0 + row;
                         bool nan = false;
                         if (key >= lim_max) {
 #pragma unroll
                             for (int c = 0; c < S::kChunks; ++c)
                                 for (int u = 0; u < CW / 16; ++u)
-                                    *reinterpret_cast<uint4*>(v + c * (kKeyTile * CW) + u * 16) = make_uint4(0, 0, 0, 0);
+                                    *reinterpret_cast<uint4*>(v + c * S::Tile::kChunk + u * 16) = make_uint4(0, 0, 0, 0);
                         } else if (key >= lim_min) {
 #pragma unroll
                             for (int c = 0; c < S::kChunks; ++c)
                                 for (int u = 0; u < CW / 4; ++u) {
-                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * (kKeyTile * CW)) + u;
+                                    uint32_t* p = reinterpret_cast<uint32_t*>(v + c * S::Tile::kChunk) + u;
                                     const uint32_t bad = e4m3_nan_mask(*p);
                                     if (bad) {
                                         *p &= ~bad;
@@ -553,7 +554,7 @@ static cudaError_t launch_queries(const QryArgs& qa, int num_sms, int dev, cudaS
 
 cudaError_t launch_kv8_queries(const dm_kv8_cache* c, const Kv8AttnArgs& a, int num_sms, int dev, cudaStream_t s) {
     QryArgs qa{};
-    if (!kv8_encode_map(c, &qa.map)) return cudaErrorNotSupported;
+    if (!kv8_encode_map(c, false, &qa.map)) return cudaErrorNotSupported;
     qa.a = a;
     qa.a.exact = kv8_exact(a, kQryRows);
     if (c->head_dim == 64) return launch_queries<64>(qa, num_sms, dev, s);

@@ -1,11 +1,10 @@
 // dm_kv8_tc.cuh — tcgen05 kind::f8f6f4 (e4m3 x e4m3 -> fp32) and TMA helpers of the 8-bit
 // cache attention kernels.
 //
-// Tiles of the cache in shared memory, as the TMA boxes of 16 token rows x CW bytes leave
-// them (CW = 128 with the 128-byte swizzle, or 64 with the 64-byte swizzle at head_dim 64):
-// token rows of CW bytes, 8-row groups of 8 CW bytes, the 16-byte units of a row permuted by
-// the row.  The same bytes serve two roles: K as a K-major operand (rows = M, the head's
-// elements = K) and V as an M-major operand (rows = K, the head's elements = M).
+// Operand tiles in shared memory: blocks of 8 rows by CW bytes (CW = 128 with the 128-byte
+// swizzle, or 64 with the 64-byte swizzle at head_dim 64), the 16-byte units of a row permuted by
+// the row.  The same cache bytes serve two roles: K as a K-major operand (rows = M, the head's
+// elements = K) and V as an M- or N-major operand (rows = K, the head's elements = M or N).
 #pragma once
 #include <cuda.h>
 #include <cuda_fp8.h>
@@ -17,19 +16,19 @@ namespace dm {
 
 constexpr uint64_t kDescVersion = 1ull << 46;
 
-// K-major operand of CW-byte rows: 8-row groups 8 CW bytes apart (stride byte offset); one
+// K-major operand of CW-byte rows: 8-row blocks `group` bytes apart (stride byte offset); one
 // K = 32 step of the tile advances the start address by 32 bytes.
 template <int CW>
-DM_DEV uint64_t f8_desc_k(uint32_t addr) {
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(8 * CW / 16) << 32) |
+DM_DEV uint64_t f8_desc_k(uint32_t addr, uint32_t group) {
+    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(group / 16) << 32) |
            kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
 }
-// M- or N-major operand: 8-token groups 8 CW bytes apart (stride byte offset), the next CW
+// M- or N-major operand: 8-token blocks `group` bytes apart (stride byte offset), the next CW
 // elements of M or N `chunk` bytes on (leading byte offset; 0 repeats the first CW elements).
 template <int CW>
-DM_DEV uint64_t f8_desc_m(uint32_t addr, uint32_t chunk) {
+DM_DEV uint64_t f8_desc_m(uint32_t addr, uint32_t chunk, uint32_t group) {
     return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(chunk / 16) << 16) |
-           (static_cast<uint64_t>(8 * CW / 16) << 32) | kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
+           (static_cast<uint64_t>(group / 16) << 32) | kDescVersion | (static_cast<uint64_t>(CW == 128 ? 2 : 4) << 61);
 }
 // N-major operand without swizzle: per 16 N columns a block of 16-byte rows, one per K;
 // 8-row groups 128 bytes apart (leading byte offset), blocks `block` bytes apart (stride).
@@ -65,11 +64,12 @@ DM_DEV void f8_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_
         : "memory");
 }
 
-DM_DEV void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+// A page's box: block coordinate `block`, from K (kv 0) or V (kv 1) on.
+DM_DEV void tma_load_page(uint32_t smem_dst, const CUtensorMap* map, int kv, int block, uint64_t* bar) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(smem_dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, "
+        "%4}], [%5];" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(kv), "r"(block), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -150,8 +150,10 @@ DM_DEV bool named_bar_or(int id, int count, bool v) {
     return r != 0;
 }
 
-// Tensor map of the cache: (head element, row of a page, page), boxes of 16 rows x CW bytes.
-// A page index of num_pages reads zeros.
-bool kv8_encode_map(const dm_kv8_cache* c, CUtensorMap* map);
+// Tensor map of the cache: (CW bytes, 8 rows, chunk of the head, K | V, 8-row block of the cache
+// counted over page, kv head and half page as if there were no K | V), boxes of a page's two
+// blocks with all chunks and K alone, V alone or, in pairs, both.  A block behind the last page
+// reads zeros.  One copy per page (8 KB in pairs at head_dim 256) instead of one per 2 KB.
+bool kv8_encode_map(const dm_kv8_cache* c, bool pair, CUtensorMap* map);
 
 }  // namespace dm

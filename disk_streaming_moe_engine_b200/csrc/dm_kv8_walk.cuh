@@ -305,13 +305,25 @@ struct KeyRing {
     }
 };
 
-// Producer (one warp): a tile's K or V as TMA boxes of 16 token rows by CW bytes, one lane per
-// page; page ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A
+// Where a tile's bytes lie in its slot: blocks of 8 tokens, in each K then V (in pairs), in each
+// the head's chunks of 8 rows x CW bytes.
+template <int D, bool PAIR>
+struct KeyTile {
+    static constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW;
+    static constexpr int kChunk = 8 * CW;                          // from chunk to chunk
+    static constexpr int kGroup = (PAIR ? 2 : 1) * kChunks * kChunk;  // from block to block
+    static constexpr int kV = PAIR ? kChunks * kChunk : 0;         // V behind K
+    static constexpr int kSlot = kKeyTile / 8 * kGroup;
+    static DM_DEV int row(int token) { return token / 8 * kGroup + token % 8 * CW; }  // chunk 0
+};
+
+// Producer (one warp): a tile's K or V (or both) in one TMA box per page, one lane per page; page ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A
 // page that is missing or holds no key of the item reads zeros.
 template <int RB, int LEAD, int D, int SL, bool PAIR>
 DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, KeyRing<SL, PAIR>& ring,
                         const KeyRange& range, volatile int* abort_flag) {
-    constexpr int CW = D >= 128 ? 128 : D, kChunks = D / CW, kSlot = (PAIR ? 2 : 1) * kKeyTile * D;
+    using Tile = KeyTile<D, PAIR>;
+    constexpr int kSlot = Tile::kSlot;
     const int lane = threadIdx.x & 31;
     bool ok = true;
     KeyWalk<RB, LEAD> w(a, range);
@@ -356,23 +368,17 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
         }
     };
     int last = -1;  // lane i: the last ring position loaded into slot i
-    // the tile with these pages into ring position `at`: rows from `row` on, in pairs V's behind K's
-    auto load = [&](uint32_t at, int id, int row) {
+    const int page_blocks = 4 * a.Hkv;  // K and V; a tensor-map block coordinate steps over 8 rows
+    // K (kv 0) or V (kv 1), or both in pairs, of the tile with these pages into ring position `at`
+    auto load = [&](uint32_t at, int id, int h, int kv) {
         const uint32_t si = at % SL;
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[si], ((at / SL) & 1u) ^ 1u, a.err, abort_flag))) return false;
         if (lane == 0) mbar_arrive_expect_tx(&ring.full[si], kSlot);
         if (lane == static_cast<int>(si)) last = static_cast<int>(at);
         __syncwarp();
         if (lane < kKeyPages) {
-            const uint32_t dst = smem_u32(sm + si * kSlot) + lane * (kKv8Page * CW);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                tma_load_3d(dst + c * (kKeyTile * CW), map, c * CW, row, id < 0 ? a.num_pages : id, &ring.full[si]);
-            if constexpr (PAIR)
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    tma_load_3d(dst + (kChunks + c) * (kKeyTile * CW), map, c * CW, row + a.Hkv * kKv8Page,
-                                id < 0 ? a.num_pages : id, &ring.full[si]);
+            tma_load_page(smem_u32(sm + si * kSlot) + lane * (2 * Tile::kGroup), map, kv,
+                          (id < 0 ? a.num_pages : id) * page_blocks + 2 * h, &ring.full[si]);
         }
         return true;
     };
@@ -391,18 +397,18 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
             int id = __shfl_sync(0xffffffffu, g0.id, from);
             if (id >= a.num_pages) id = -1;
             const float2 sc = make_float2(__shfl_sync(0xffffffffu, g0.sc.x, from), __shfl_sync(0xffffffffu, g0.sc.y, from));
-            if (!(ok = load(ring.k_load(x), id, h * kKv8Page))) break;
+            if (!(ok = load(ring.k_load(x), id, h, 0))) break;
             if (lane < kKeyPages) ring.meta[x % kKeyMeta][lane] = sc;
             __syncwarp();
             if (lane == 0) mbar_arrive(&ring.meta_full[x % kKeyMeta]);
-            if (!PAIR && x > 0) ok = load(ring.v_load(x - 1), prev_id, (a.Hkv + prev_h) * kKv8Page);
+            if (!PAIR && x > 0) ok = load(ring.v_load(x - 1), prev_id, prev_h, 1);
             prev_id = id;
             prev_h = h;
         }
         g0 = g1;
         g1 = g2;
     }
-    if (!PAIR && ok && x > 0) ok = load(ring.v_load(x - 1), prev_id, (a.Hkv + prev_h) * kKv8Page);
+    if (!PAIR && ok && x > 0) ok = load(ring.v_load(x - 1), prev_id, prev_h, 1);
     // no copy is left in flight, whoever gave up
     if (last >= 0) ring.wait_full(static_cast<uint32_t>(last), a.err, nullptr);
 }
