@@ -49,9 +49,10 @@ struct Kv8AttnArgs {
 };
 
 // Exact tile counts cost a pass over all row blocks in every CTA: taken where a warp goes through a
-// request's blocks (up to 64 requests) or no request has more than 8.
+// request's blocks (up to 64 requests) or no request has more than 8, and needless where every
+// block of a request sees the same keys.
 inline int kv8_exact(const Kv8AttnArgs& a, int rows_per_block) {
-    return a.n <= 64 || (static_cast<int64_t>(a.max_q) * a.group + rows_per_block - 1) / rows_per_block <= 8;
+    return a.max_q > 1 && (a.n <= 64 || (static_cast<int64_t>(a.max_q) * a.group + rows_per_block - 1) / rows_per_block <= 8);
 }
 
 // dm_kv8_keys.cu: any row count and type, one or two CTAs per SM.  Workspace: counters [2 num_sms], then

@@ -163,7 +163,30 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
             out->u1 = active ? total * (blockIdx.x + 1) / grid : 0;
         }
     };
-    if (a.n <= kKeyFew) {
+    if (a.n <= kKeyFew && !a.exact) {  // every warp for itself, two requests per lane
+        const KeyRaw w0 = key_raw(a, lane), w1 = key_raw(a, lane + 32);
+        auto units = [&](int i, const KeyRaw& w) {
+            const KeyReq r = key_req<RB>(a, w, report && warp == 0 && i < a.n);
+            return i < a.n ? static_cast<long long>(r.blocks) * a.Hkv * (r.tiles + LEAD) : 0;
+        };
+        const long long v0 = units(lane, w0), v1 = units(lane + 32, w1);
+        const long long e0 = warp_scan(v0), e1 = __shfl_sync(0xffffffffu, e0, 31) + warp_scan(v1);
+        total = __shfl_sync(0xffffffffu, e1, 31);
+        cut();
+        if (warp == 0) {
+            if (lane < a.n) out->raw[lane] = w0;
+            if (lane + 32 < a.n) out->raw[lane + 32] = w1;
+            const bool here0 = u0 >= e0 - v0 && u0 < e0, here1 = u0 >= e1 - v1 && u0 < e1;
+            if (active && (here0 || here1)) {
+                const long long rem = u0 - (here0 ? e0 - v0 : e1 - v1);
+                const KeyReq r = key_req<RB>(a, here0 ? w0 : w1, false);
+                const long long c = static_cast<long long>(r.tiles + LEAD) * a.Hkv;
+                out->req = here0 ? lane : lane + 32;
+                out->blk = r.blocks > 1 ? static_cast<int>(rem / c) : 0;
+                out->rem = rem - out->blk * c;
+            }
+        }
+    } else if (a.n <= kKeyFew) {
         if (tid < a.n) {
             out->raw[tid] = key_raw(a, tid);
             key_req<RB>(a, out->raw[tid], report);
@@ -172,10 +195,7 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
         for (int i = warp; i < a.n; i += NT / 32) {
             const KeyReq r = key_req<RB>(a, out->raw[i], false);
             long long sum = 0;
-            if (a.exact)
-                for (int b = lane; b < r.blocks; b += 32) sum += key_tiles<RB>(a, r, b) + LEAD;
-            else if (lane == 0)
-                sum = static_cast<long long>(r.blocks) * (r.tiles + LEAD);
+            for (int b = lane; b < r.blocks; b += 32) sum += key_tiles<RB>(a, r, b) + LEAD;
 #pragma unroll
             for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane == 0) s_sum[i] = sum * a.Hkv;
@@ -193,25 +213,19 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
             long long rem = u0 - (m0 ? __shfl_sync(0xffffffffu, e0 - v0, src) : __shfl_sync(0xffffffffu, e1 - v1, src));
             const KeyReq r = key_req<RB>(a, out->raw[req], false);
             int blk = 0;
-            if (a.exact) {  // 32 blocks at a time
-                for (;; blk += 32) {
-                    const long long c =
-                        blk + lane < r.blocks ? static_cast<long long>(key_tiles<RB>(a, r, blk + lane) + LEAD) * a.Hkv : 0;
-                    const long long e = warp_scan(c), all = __shfl_sync(0xffffffffu, e, 31);
-                    if (rem >= all && blk + 32 < r.blocks) {
-                        rem -= all;
-                        continue;
-                    }
-                    const unsigned m = __ballot_sync(0xffffffffu, rem < e);
-                    const int at = m ? __ffs(m) - 1 : 0;
-                    rem -= __shfl_sync(0xffffffffu, e - c, at);
-                    blk += at;
-                    break;
+            for (;; blk += 32) {  // 32 blocks at a time
+                const long long c =
+                    blk + lane < r.blocks ? static_cast<long long>(key_tiles<RB>(a, r, blk + lane) + LEAD) * a.Hkv : 0;
+                const long long e = warp_scan(c), all = __shfl_sync(0xffffffffu, e, 31);
+                if (rem >= all && blk + 32 < r.blocks) {
+                    rem -= all;
+                    continue;
                 }
-            } else {
-                const long long c = static_cast<long long>(r.tiles + LEAD) * a.Hkv;
-                blk = static_cast<int>(rem / c);
-                rem -= blk * c;
+                const unsigned m = __ballot_sync(0xffffffffu, rem < e);
+                const int at = m ? __ffs(m) - 1 : 0;
+                rem -= __shfl_sync(0xffffffffu, e - c, at);
+                blk += at;
+                break;
             }
             if (lane == 0) {
                 out->req = req;
