@@ -85,6 +85,9 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     __shared__ __align__(8) uint64_t s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
+    // elements of out and of lse of the item's rows, by the item's parity: some threads still write
+    // an item's results when others are at the next item's q
+    __shared__ int64_t s_off[2][RB], s_lse[2][RB];
     __shared__ float s_red[4][RB], s_fac[32][RB];
     __shared__ long long s_sum[64];
     __shared__ KeyRange s_range;
@@ -110,8 +113,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
     if (warp == W_MMA) tc_alloc(&s_tmem, S::kCols);
 
     tc_fence_before();
-    // two tiles per CTA at least: a part costs more to join than a second tile takes
-    const bool active = key_range<RB, kKeyLead, NT>(a, 2 + kKeyLead, s_sum, &s_range);
+    // one tile and its item cost per CTA at least
+    const bool active = key_range<RB, kKeyLead, NT>(a, 1 + kKeyLead, s_sum, &s_range);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
         const int tt = tid & 127, r0 = tid / 128 * 8, wq = warp & 3;  // token, first row, warp of the group
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + r0;
         uint32_t t = 0;
+        int item = 0;
         bool ok = true;
         KeyWalk<RB, kKeyLead> w(a, s_range);
         while (w.unit < w.end && ok) {
@@ -215,6 +219,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                 if (tid % 16 == 0) {
                     s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
                     s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
+                    s_off[item & 1][r] = static_cast<int64_t>(w.r.row0 + tok) * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
+                    s_lse[item & 1][r] = static_cast<int64_t>(w.r.row0 + tok) * a.Hq + head;
                 }
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[e] *= mul;
@@ -404,19 +410,13 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
 
             const long long item0 = w.tile0();  // the item's first tile in the sequence
             const bool whole = t_begin == 0 && nt == real;
-            const int c_first = key_owner(item0, s_range.total, s_range.grid), c_last = key_owner(item0 + real - 1, s_range.total, s_range.grid);
             constexpr int kSlot = (RB * (D + 2) + 3) / 4 * 4;
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
             auto put = [&](int r, int d, float o, float mm, float ll) {
                 if (r >= nrow) return;
-                const int f = w.block() * RB + r;
-                const int64_t row = w.r.row0 + f / a.group;
-                const int head = w.h * a.group + f % a.group;
                 // a row that saw no key keeps the reference -inf
-                static_cast<T*>(a.out)[row * a.o_rs + static_cast<int64_t>(head) * a.o_hs + d] =
-                    static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o / ll);
-                if (d == 0 && a.lse)
-                    a.lse[row * a.Hq + head] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+                static_cast<T*>(a.out)[s_off[item & 1][r] + d] = static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o / ll);
+                if (d == 0 && a.lse) a.lse[s_lse[item & 1][r]] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
             };
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c) {
@@ -448,6 +448,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                         slot[RB * D + RB + r0 + r] = l[r];
                     }
                 }
+                const int c_first = key_owner(item0, s_range.total, s_range.grid);
+                const int c_last = key_owner(item0 + real - 1, s_range.total, s_range.grid);
                 named_bar_sync(1, SOFT);
                 if (tid == 0) {
                     const unsigned parts = static_cast<unsigned>(c_last - c_first + 1);
@@ -513,6 +515,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     named_bar_sync(1, SOFT);  // s_red is free again
                 }
             }
+            ++item;
             w.next();
         }
     }

@@ -99,8 +99,9 @@ struct KeyWalk {
         r = key_req<RB>(a, range.request(a, req), false);
         ahead = range.request(a, req + 1);
         tiles = a.exact ? key_tiles<RB>(a, r, blk) : r.tiles;
-        pos = static_cast<int>(k.rem % (tiles + LEAD));
-        h = static_cast<int>(k.rem / (tiles + LEAD));
+        const unsigned per = tiles + LEAD;
+        h = k.rem >> 32 ? static_cast<int>(k.rem / per) : static_cast<int>(static_cast<unsigned>(k.rem) / per);
+        pos = static_cast<int>(k.rem - static_cast<long long>(h) * per);
     }
     DM_DEV int block() const { return a.exact ? blk : blk & 1 ? r.blocks - 1 - (blk >> 1) : blk >> 1; }
     DM_DEV int count() const { return static_cast<int>(min(static_cast<long long>(tiles + LEAD - pos), end - unit)); }
