@@ -1,5 +1,6 @@
 // dm_kv8.cu — slot planning, rotary positions and the quantising append of the 8-bit paged
 // KV cache (C entries dm_kv8_plan, dm_rope, dm_kv8_append, dm_kv8_status).
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -41,7 +42,13 @@ int Kv8Device::enter(const void* p, const char* stage, char* eb, uint64_t es) {
         if (e == cudaSuccess) prev = cur;
     }
     dev = at.device;
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev);
+    static std::atomic<int> sms[64];  // per device, once known
+    const bool known = dev < 64;
+    num_sms = known ? sms[dev].load(std::memory_order_relaxed) : 0;
+    if (e == cudaSuccess && num_sms == 0) {
+        e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess && known) sms[dev].store(num_sms, std::memory_order_relaxed);
+    }
     if (e != cudaSuccess)
         return kv8_err(eb, es, DM_ERR_CUDA, "CUDA_ERROR", stage, "%s", cudaGetErrorString(e));
     return DM_OK;
@@ -280,7 +287,7 @@ struct RopeArgs {
 };
 
 constexpr int kRopeTok = 8;    // tokens of a CTA at most
-constexpr int kRopeBatch = 4;  // tokens whose loads a thread has in flight
+constexpr int kRopeBatch = 2;  // tokens whose loads a thread has in flight
 
 // 16 bytes (VEC elements) or one element (VEC = 1) as loaded, and as floats
 template <typename T, int VEC>
@@ -330,7 +337,7 @@ struct RopeVec {
 // CTA computes the angles.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeArgs a) {
-    __shared__ float2 cs[kRopeTok][128];
+    __shared__ float2 cs[kRopeTok][128];  // pair unit * VEC + k at k * units + unit: no bank conflicts
     __shared__ int s_pos[kRopeTok];
     const int t0 = blockIdx.x * a.tok, nt = min(a.tok, a.n - t0);
     const int rot = a.plan.rotary_dim, half = rot / 2, D = a.plan.head_dim;
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
                     const float hi = static_cast<float>(red), lo = static_cast<float>(red - static_cast<double>(hi));
                     float s, c;
                     sincosf(hi, &s, &c);
-                    cs[t][j] = make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
+                    cs[t][j % VEC * pu + j / VEC] = make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
                 }
                 __syncthreads();
             }
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
                     if (!inter || VEC == 1) {
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) {
-                            const float2 f = cs[t][j0 + k];
+                            const float2 f = cs[t][k * pu + unit];
                             const float v = p[k], z = q[k];
                             p[k] = v * f.x - z * f.y;
                             q[k] = z * f.x + v * f.y;
@@ -396,7 +403,7 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
                     } else {
 #pragma unroll
                         for (int k = 0; k < VEC / 2; ++k) {
-                            const float2 f = cs[t][j0 + k], g = cs[t][j0 + VEC / 2 + k];
+                            const float2 f = cs[t][k * pu + unit], g = cs[t][(VEC / 2 + k) * pu + unit];
                             float v = p[2 * k], z = p[2 * k + 1];
                             p[2 * k] = v * f.x - z * f.y;
                             p[2 * k + 1] = z * f.x + v * f.y;

@@ -62,10 +62,13 @@ def _ints(device, names, *tensors):
 
 
 def _rows(name: str, t: torch.Tensor, heads, dim: int, device, dtype):
-    if (t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads) or t.device != device
-            or t.dtype != dtype or (t.numel() and t.stride(2) != 1)):
+    """Checks [rows][heads][dim] with contiguous heads; (address, row stride, head stride, rows, heads)."""
+    shape, stride = t.shape, t.stride()
+    if (len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads) or t.dtype is not dtype
+            or t.device != device or (stride[2] != 1 and t.numel())):
         _bad(f"{name} must be [rows][{'heads' if heads is None else heads}][{dim}] {dtype} on {device}, head elements "
-             f"contiguous (got {tuple(t.shape)} {t.dtype} on {t.device})")
+             f"contiguous (got {tuple(shape)} {t.dtype} on {t.device})")
+    return t.data_ptr(), stride[0], stride[1], shape[0], shape[1]
 
 
 def error_word(device="cuda") -> torch.Tensor:
@@ -132,7 +135,7 @@ def plan_slots(free_pages, free_state, block_table, ctx_lens, new_lens, max_toke
     dev = ctx_lens.device
     n = ctx_lens.numel()
     if out is None:
-        room = torch.empty(2 * n + 1 + 3 * max_tokens, dtype=torch.int32, device=dev)
+        room = ctx_lens.new_empty(2 * n + 1 + 3 * max_tokens)
         out = SlotPlan(*room.split_with_sizes((n, n + 1, max_tokens, max_tokens, max_tokens)))
     else:
         _ints(dev, "seq_lens cu_new slots positions requests", *out)
@@ -192,17 +195,18 @@ def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     k = q[:, :0] if k is None else k
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
-    for name, t, like in (("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)):
-        _rows(name, t, like.shape[1], D, dev, q.dtype)
-        if t.shape[0] != n:
-            _bad(f"{name} has {t.shape[0]} rows, positions {n}")
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    k_out = torch.empty_like(k) if k_out is None else k_out
+    q_ptr, q_rs, q_hs, q_rows, hq = _rows("q", q, None, D, dev, q.dtype)
+    k_ptr, k_rs, k_hs, k_rows, hk = _rows("k", k, None, D, dev, q.dtype)
+    qo_ptr, qo_rs, qo_hs, qo_rows, _ = _rows("q_out", q_out, hq, D, dev, q.dtype)
+    ko_ptr, ko_rs, ko_hs, ko_rows, _ = _rows("k_out", k_out, hk, D, dev, q.dtype)
+    if not n == q_rows == k_rows == qo_rows == ko_rows:
+        _bad(f"{n} positions, but q, k, q_out, k_out have {q_rows}, {k_rows}, {qo_rows}, {ko_rows} rows")
     buf = _buffer()
     rc = _lib.load().dm_rope(
-        plan._ref, _DTYPES[q.dtype], n, positions.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
-        q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.shape[1], k.data_ptr(), k.stride(0), k.stride(1),
-        k_out.data_ptr(), k_out.stride(0), k_out.stride(1), k.shape[1], _stream(dev, stream), buf, _ERR)
+        plan._ref, _DTYPES[q.dtype], n, positions.data_ptr(), q_ptr, q_rs, q_hs, qo_ptr, qo_rs, qo_hs, hq, k_ptr, k_rs,
+        k_hs, ko_ptr, ko_rs, ko_hs, hk, _stream(dev, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
     return q_out, k_out
@@ -213,15 +217,15 @@ def append(cache: Kv8Cache, k, v, slots, *, err=None, stream=None) -> None:
     n = slots.numel()
     if k.dtype not in _DTYPES:
         _bad(f"k is bf16 or fp32 (got {k.dtype})")
-    _rows("k", k, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
-    _rows("v", v, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
+    k_ptr, k_rs, k_hs, k_rows, _ = _rows("k", k, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
+    v_ptr, v_rs, v_hs, v_rows, _ = _rows("v", v, cache.num_kv_heads, cache.head_dim, cache.device, k.dtype)
     _ints(cache.device, "slots err", slots, err)
-    if k.shape[0] < n or v.shape[0] < n:
-        _bad(f"{n} slots, k has {k.shape[0]} rows, v {v.shape[0]}")
+    if k_rows < n or v_rows < n:
+        _bad(f"{n} slots, k has {k_rows} rows, v {v_rows}")
     buf = _buffer()
     rc = _lib.load().dm_kv8_append(
-        cache._ref, _DTYPES[k.dtype], n, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-        v.stride(1), slots.data_ptr(), None if err is None else err.data_ptr(), _stream(cache.device, stream), buf, _ERR)
+        cache._ref, _DTYPES[k.dtype], n, k_ptr, k_rs, k_hs, v_ptr, v_rs, v_hs, slots.data_ptr(),
+        None if err is None else err.data_ptr(), _stream(cache.device, stream), buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
 
@@ -246,14 +250,13 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
     n = seq_lens.numel()
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
-    _rows("q", q, None, D, dev, q.dtype)
+    q_ptr, q_rs, q_hs, rows, hq = _rows("q", q, None, D, dev, q.dtype)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _rows("out", out, q.shape[1], D, dev, q.dtype)
+        out = torch.empty_like(q)
+    out_ptr, out_rs, out_hs, out_rows, _ = _rows("out", out, hq, D, dev, q.dtype)
     _ints(dev, "block_table seq_lens cu_q err", block_table, seq_lens, cu_q, err)
     if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \
-            out.shape[0] < q.shape[0]:
+            out_rows < rows:
         _bad("need block_table [n][width], cu_q [n + 1] and out of q's shape")
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or
                             not lse.is_contiguous() or lse.device != dev):
@@ -261,9 +264,8 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
     if workspace.device != dev or not workspace.is_contiguous():
         _bad("the workspace must be a contiguous tensor on the cache's device")
     a = _lib.DmKv8AttnArgs(
-        _DTYPES[q.dtype], n, q.shape[1], max_q_len, q.shape[0], block_table.shape[1],
-        D ** -0.5 if sm_scale is None else sm_scale, 0, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-        out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), block_table.data_ptr(),
+        _DTYPES[q.dtype], n, hq, max_q_len, rows, block_table.shape[1], D ** -0.5 if sm_scale is None else sm_scale, 0,
+        q_ptr, q_rs, q_hs, out_ptr, out_rs, out_hs, None if lse is None else lse.data_ptr(), block_table.data_ptr(),
         seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), None if err is None else err.data_ptr())
     buf = _buffer()
