@@ -225,17 +225,16 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[e] *= mul;
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i)
+                for (int e = 0; e < E; e += 4) {
+                    uint32_t lo[TERMS], hi[TERMS];
+                    e4m3_split2<TERMS>(x[e], x[e + 1], lo);
+                    e4m3_split2<TERMS>(x[e + 2], x[e + 3], hi);
+                    const int d = e0 + e;
 #pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        float2 b0, b1;
-                        const uint32_t lo = e4m3_round2(x[e], x[e + 1], b0), hi = e4m3_round2(x[e + 2], x[e + 3], b1);
-                        const int d = e0 + e, n = i * RB + r;
-                        uint8_t* dst = s_q + (d / CW) * (N * CW) + f8_unit<CW>(n, (d % CW) / 16) + d % 16;
-                        *reinterpret_cast<uint32_t*>(dst) = lo | (hi << 16);
-                        x[e] = (x[e] - b0.x) * 16.0f, x[e + 1] = (x[e + 1] - b0.y) * 16.0f;
-                        x[e + 2] = (x[e + 2] - b1.x) * 16.0f, x[e + 3] = (x[e + 3] - b1.y) * 16.0f;
-                    }
+                    for (int i = 0; i < TERMS; ++i)
+                        *reinterpret_cast<uint32_t*>(s_q + (d / CW) * (N * CW) + f8_unit<CW>(i * RB + r, (d % CW) / 16) +
+                                                     d % 16) = lo[i] | (hi[i] << 16);
+                }
                 fence_proxy_async_smem();
                 mbar_arrive(&q_ready);
                 named_bar_sync(1, SOFT);
@@ -370,21 +369,14 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                     }
                 }
                 uint8_t* p = s_p + (x & 1u) * S::kP + tt * 16;
+                uint32_t code[4][TERMS];
+#pragma unroll
+                for (int r = 0; r < 8; r += 2) e4m3_split2<TERMS>(y[r], y[r + 1], code[r / 2]);
 #pragma unroll
                 for (int b = 0; b < TERMS; ++b) {
-                    uint32_t code[4];
-#pragma unroll
-                    for (int r = 0; r < 8; r += 2) {
-                        float2 back;
-                        code[r / 2] = e4m3_round2(y[r], y[r + 1], back);
-                        if (b + 1 < TERMS) {
-                            y[r] = (y[r] - back.x) * 16.0f;
-                            y[r + 1] = (y[r + 1] - back.y) * 16.0f;
-                        }
-                    }
                     const int n = b * RB + r0;
                     *reinterpret_cast<uint2*>(p + (n / 16) * (kKeyTile * 16) + n % 16) =
-                        make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
+                        make_uint2(code[0][b] | (code[1][b] << 16), code[2][b] | (code[3][b] << 16));
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();

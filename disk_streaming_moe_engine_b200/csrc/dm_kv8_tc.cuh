@@ -80,15 +80,33 @@ DM_DEV uint32_t f8_unit(int r, int u) {
     return static_cast<uint32_t>(r * CW + x * 16);
 }
 
-DM_DEV float e4m3_round(float x, uint32_t& code) {  // code of the nearest value, and that value
-    code = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
-}
-// codes of two values (a in the low byte), and the values they stand for
-DM_DEV uint32_t e4m3_round2(float a, float b, float2& back) {
-    const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), __NV_E4M3)));
+// Codes of two fp16 values (a in the low byte), and 16 times what they leave (exact).
+DM_DEV uint32_t e4m3_take2(__half2& h) {
+    const uint32_t c = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E4M3);
+    const __half2 back(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c), __NV_E4M3));
+    h = __hmul2(__hsub2(h, back), __float2half2_rn(16.0f));
     return c;
+}
+// e4m3 terms of two values of magnitude up to 448, term i scaled by 2^4i.  Two terms hold the 8
+// bits of the value as fp16; with five the first three take its 11 bits and the other two 8 bits
+// of the rest, 2^12 times of which is an fp16 value again: 2^-20 of the value, or 2^-26.
+template <int TERMS>
+DM_DEV void e4m3_split2(float a, float b, uint32_t (&t)[TERMS]) {
+    static_assert(TERMS == 2 || TERMS == 5, "terms");
+    __half2 h = __floats2half2_rn(a, b);
+    __half2 rest = h;
+    if constexpr (TERMS == 5) {
+        const float2 f = __half22float2(h);
+        rest = __floats2half2_rn((a - f.x) * 4096.0f, (b - f.y) * 4096.0f);
+    }
+    t[0] = e4m3_take2(h);
+    t[1] = e4m3_take2(h);
+    if constexpr (TERMS == 5) {
+        t[2] = e4m3_take2(h);
+        rest = __hadd2(rest, h);  // what small values still have left, at the same scale
+        t[3] = e4m3_take2(rest);
+        t[4] = e4m3_take2(rest);
+    }
 }
 // 0xff in the bytes of w that hold a NaN code
 DM_DEV uint32_t e4m3_nan_mask(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
