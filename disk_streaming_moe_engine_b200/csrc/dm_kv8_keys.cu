@@ -40,7 +40,7 @@ constexpr int kKeyLead = 1;                  // an item's start and end in tiles
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
 
-template <typename T, int D, int RB>
+template <typename T, int D, int RB, int CTAS>
 struct KeyShape {
     static constexpr int kTerms = sizeof(T) == 4 ? 5 : 2;
     static constexpr int kN = (RB * kTerms + 15) / 16 * 16;  // columns behind the terms are never read
@@ -51,9 +51,7 @@ struct KeyShape {
     static constexpr int kQ = kN * D;
     static constexpr int kP = kN * kKeyTile;          // one of two buffers
     static constexpr int kFixed = kQ + 2 * kP + 1024;
-    // a tile's chain of waits takes about 0.65 us whatever D is, its bytes from HBM 0.37 us at
-    // D = 64 and 1.5 us at D = 256: the smaller heads take two CTAs per SM
-    static constexpr int kCtas = D <= 128 && RB == 8 ? 2 : 1;
+    static constexpr int kCtas = CTAS;                       // per SM
     using Tile = KeyTile<D, true>;                    // K and V of a tile
     static constexpr int kSlot = Tile::kSlot;
     static constexpr int kFit = (kKeySmem / kCtas - 6144 - kFixed) / kSlot;  // static arrays and 1 KB per CTA beside it
@@ -70,10 +68,10 @@ struct KeyArgs {
     Kv8AttnArgs a;
 };
 
-template <typename T, int D, int RB>
-__global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, RB>::kCtas)
+template <typename T, int D, int RB, int CTAS>
+__global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T, D, RB, CTAS>::kCtas)
     kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
-    using S = KeyShape<T, D, RB>;
+    using S = KeyShape<T, D, RB, CTAS>;
     constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
@@ -258,7 +256,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB>::kThreads, KeyShape<T, D, R
                 }
                 __syncwarp();  // the loads below are the whole warp's
                 tc_fence_after();
-                const float2 sc = ring.meta[x % kKeyMeta][tt >> 4];
+                const float2 sc = ring.meta[x % ring.kMeta][tt >> 4];
                 const float vexp = static_cast<float>(((__float_as_int(sc.y) >> 23) & 0xff) - 127);
                 float y[8];
                 {
@@ -542,25 +540,32 @@ bool kv8_encode_map(const dm_kv8_cache* c, bool pair, CUtensorMap* map) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int RB>
+template <typename T, int D, int RB, int CTAS>
 static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStream_t s) {
-    using S = KeyShape<T, D, RB>;
+    using S = KeyShape<T, D, RB, CTAS>;
     static bool ready[64] = {};
     if (dev >= 64 || !ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_attn_keys_kernel<T, D, RB>,
+        const cudaError_t e = cudaFuncSetAttribute(kv8_attn_keys_kernel<T, D, RB, CTAS>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
         if (dev < 64) ready[dev] = true;
     }
-    kv8_attn_keys_kernel<T, D, RB><<<num_sms * S::kCtas, S::kThreads, S::kSmem, s>>>(ka);
+    kv8_attn_keys_kernel<T, D, RB, CTAS><<<num_sms * S::kCtas, S::kThreads, S::kSmem, s>>>(ka);
     return cudaGetLastError();
 }
 
+// CTAs per SM.  A tile's chain of waits takes 0.65 us and more whatever D is, its bytes from HBM
+// 0.37 us at D = 64 and 1.5 us at D = 256: two CTAs overlap their chains where they fit (D <= 128).
+// With 16 rows two leave each thread 96 registers, with some spills: fp32 chunks of 5 x 150 rows at
+// D = 128 take 365 us against 461 us with one, but one token of 16 heads (32 x 8000 keys) 48 us
+// against 45 us, so one token per request takes one CTA there.
 template <typename T, int RB>
 static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev, cudaStream_t s) {
-    if (D == 64) return launch_keys<T, 64, RB>(ka, num_sms, dev, s);
-    if (D == 128) return launch_keys<T, 128, RB>(ka, num_sms, dev, s);
-    return launch_keys<T, 256, RB>(ka, num_sms, dev, s);
+    if (D == 64) return launch_keys<T, 64, RB, 2>(ka, num_sms, dev, s);
+    if (D == 256) return launch_keys<T, 256, RB, 1>(ka, num_sms, dev, s);
+    if constexpr (RB == 16)
+        if (ka.a.max_q == 1) return launch_keys<T, 128, RB, 1>(ka, num_sms, dev, s);
+    return launch_keys<T, 128, RB, 2>(ka, num_sms, dev, s);
 }
 
 // Rows of an item: 16 when a request's rows fill more than 8 (the cache is then read once

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 const float base = mref == -INFINITY ? 0.0f : kQryBoost - mref;
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const float2 sc = ring.meta[x % kKeyMeta][half * 4 + p];
+                    const float2 sc = ring.meta[x % ring.kMeta][half * 4 + p];
                     const int ve = ((__float_as_int(sc.y) >> 23) & 0xff) - 127;
                     f[p] = frow * sc.x;
                     g[p] = sc.y < 0.0f ? -INFINITY : static_cast<float>(ve) + base;

@@ -294,13 +294,17 @@ DM_DEV int key_owner(long long u, long long total, long long grid) { return stat
 // holds what the next products need.  The query-side kernel is bound by its products and by how
 // early the next tile is there (4 x 8192 prompts 3.24 ms in pairs, 2.73 ms single); the key-side
 // one by the bytes (64 x 32768 384 us in pairs, 405 us single).
-constexpr int kKeyMeta = 8;      // tiles whose scales are kept (at least slots / 2 + 2)
 constexpr int kKeyMaxSlots = 12;
 
 template <int SL, bool PAIR>
 struct KeyRing {
-    uint64_t full[SL], empty[SL], meta_full[kKeyMeta];
-    float2 meta[kKeyMeta][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
+    // Tiles whose scales are kept.  Those of tile x + kMeta are written once its K has a slot, i.e.
+    // the K or O product of the tile SL positions before is done; by then every softmax thread has
+    // left tile x: in pairs that was the O product of tile x itself, else the scores of tile x + 2
+    // (issued after the weights of tile x) or a later O product.
+    static constexpr int kMeta = PAIR ? SL : SL / 2 + 2;
+    uint64_t full[SL], empty[SL], meta_full[kMeta];
+    float2 meta[kMeta][kKeyPages];  // (sK, sV) of the tile's pages; sV < 0: no such page
     static DM_DEV uint32_t k_load(uint32_t tile) { return PAIR ? tile : tile ? 2 * tile - 1 : 0; }
     static DM_DEV uint32_t v_load(uint32_t tile) { return PAIR ? tile : 2 * tile + 2; }
     DM_DEV void init() {               // one thread
@@ -308,15 +312,15 @@ struct KeyRing {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < kKeyMeta; ++i) mbar_init(&meta_full[i], 1);
+        for (int i = 0; i < kMeta; ++i) mbar_init(&meta_full[i], 1);
     }
     DM_DEV bool wait_full(uint32_t load, uint32_t* err, volatile int* abort_flag) {
         return mbar_wait_bounded(&full[load % SL], (load / SL) & 1u, err, abort_flag);
     }
     // scales of tile x: ready (or not yet)
-    DM_DEV bool try_meta(uint32_t x) { return mbar_try_wait(&meta_full[x % kKeyMeta], (x / kKeyMeta) & 1u); }
+    DM_DEV bool try_meta(uint32_t x) { return mbar_try_wait(&meta_full[x % kMeta], (x / kMeta) & 1u); }
     DM_DEV bool wait_meta(uint32_t x, uint32_t* err, volatile int* abort_flag) {
-        return mbar_wait_bounded(&meta_full[x % kKeyMeta], (x / kKeyMeta) & 1u, err, abort_flag);
+        return mbar_wait_bounded(&meta_full[x % kMeta], (x / kMeta) & 1u, err, abort_flag);
     }
 };
 
@@ -413,9 +417,9 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
             if (id >= a.num_pages) id = -1;
             const float2 sc = make_float2(__shfl_sync(0xffffffffu, g0.sc.x, from), __shfl_sync(0xffffffffu, g0.sc.y, from));
             if (!(ok = load(ring.k_load(x), id, h, 0))) break;
-            if (lane < kKeyPages) ring.meta[x % kKeyMeta][lane] = sc;
+            if (lane < kKeyPages) ring.meta[x % ring.kMeta][lane] = sc;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ring.meta_full[x % kKeyMeta]);
+            if (lane == 0) mbar_arrive(&ring.meta_full[x % ring.kMeta]);
             if (!PAIR && x > 0) ok = load(ring.v_load(x - 1), prev_id, prev_h, 1);
             prev_id = id;
             prev_h = h;

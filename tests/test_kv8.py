@@ -100,32 +100,41 @@ def plain_append(pages, scales, k, v, slots):
 
 def plain_attention(cache, q, table, lens, cu, scale):
     """64-bit results, their magnitudes (sum p |v|, and the row's largest p sV times the sum of
-    |codes|), the largest sum |q k| of every row, lse."""
-    pages, scales = cache.pages.cpu().numpy(), cache.scales.cpu().numpy().astype(np.float64)
-    q = q.double().cpu().numpy()
-    hk, d = pages.shape[2], pages.shape[4]
-    grp = q.shape[1] // hk
-    out, mag, small, sat = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q), np.zeros(q.shape[:2])
-    lse = np.full(q.shape[:2], -np.inf)
+    |codes|), the largest sum |q k| of every row, lse: elementary operations, one request at a
+    time."""
+    dev, f64 = cache.device, torch.float64
+    q = q.double()
+    grp = q.shape[1] // cache.num_kv_heads
+    value = torch.from_numpy(E4M3).to(dev)
+    out, mag, small = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    sat = torch.zeros(q.shape[:2], dtype=f64, device=dev)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=f64, device=dev)
     for i, n in enumerate(lens):
-        m = cu[i + 1] - cu[i]
-        ids = table[i, np.arange(n) // PAGE]
-        codes, sc = E4M3[pages[ids, :, :, np.arange(n) % PAGE]], scales[ids]
-        kv = codes * sc[..., None]  # [n][2][hk][d]
-        for j in range(m):
-            see = max(0, min(n, n - m + j + 1))
-            if see == 0:
-                continue
-            for h in range(q.shape[1]):
-                kk, vv, x = kv[:see, 0, h // grp], kv[:see, 1, h // grp], q[cu[i] + j, h]
-                s = kk @ x * scale
-                p = np.exp(s - s.max())
-                lse[cu[i] + j, h] = s.max() + math.log(p.sum())
-                p /= p.sum()
-                out[cu[i] + j, h], mag[cu[i] + j, h] = p @ vv, p @ np.abs(vv)
-                small[cu[i] + j, h] = (p * sc[:see, 1, h // grp]).max() * np.abs(codes[:see, 1, h // grp]).sum(0)
-                sat[cu[i] + j, h] = (np.abs(kk) @ np.abs(x)).max() * abs(scale)
-    return out, (mag, small), sat, lse
+        m = int(cu[i + 1] - cu[i])
+        if not m or not n:
+            continue
+        pos = torch.arange(n, device=dev)
+        ids = torch.from_numpy(np.asarray(table[i], np.int64)).to(dev)[pos // PAGE]
+        codes = value[cache.pages[ids, :, :, pos % PAGE].long()]  # [n][2][hk][d]
+        sc = cache.scales[ids].double()
+        see = pos[None, :] < (n - m + torch.arange(m, device=dev) + 1)[:, None]  # [m][n]
+        some = see.any(1)
+        rows = slice(int(cu[i]), int(cu[i + 1]))
+        for h in range(cache.num_kv_heads):
+            hs = slice(h * grp, (h + 1) * grp)
+            k, cv, sv = codes[:, 0, h] * sc[:, 0, h, None], codes[:, 1, h], sc[:, 1, h]
+            v = torch.where(see.any(0)[:, None], cv * sv[:, None], 0.0)
+            x = q[rows, hs]
+            s = torch.where(see[:, None], x @ k.T * scale, -math.inf)  # [m][grp][n]
+            top = s.amax(-1, keepdim=True).clamp(min=-1e300)
+            p = torch.exp(s - top)
+            total = p.sum(-1, keepdim=True)
+            p = p / total.clamp(min=1e-300)
+            lse[rows, hs] = torch.where(some[:, None], (top + torch.log(total))[..., 0], -math.inf)
+            out[rows, hs], mag[rows, hs] = p @ v, p @ v.abs()
+            small[rows, hs] = (p * sv).amax(-1, keepdim=True) * (see.double() @ cv.abs().nan_to_num())[:, None]
+            sat[rows, hs] = torch.where(see[:, None], x.abs() @ k.abs().T, 0.0).amax(-1) * abs(scale)
+    return out.cpu().numpy(), (mag.cpu().numpy(), small.cpu().numpy()), sat.cpu().numpy(), lse.cpu().numpy()
 
 
 def attention_tolerance(out, mag, sat, d, keys, dtype, rows=1):
@@ -150,9 +159,10 @@ def attention_tolerance(out, mag, sat, d, keys, dtype, rows=1):
 
 def make_cache(n_pages, hk, d, seed, lo=-9, hi=-5):
     g = np.random.default_rng(seed)
-    codes = to_e4m3(np.clip(g.standard_normal((n_pages, 2, hk, PAGE, d)) * 100, -448, 448))
+    x = torch.randn((n_pages, 2, hk, PAGE, d), generator=torch.Generator(DEV).manual_seed(seed), device=DEV)
+    codes = x.mul_(100).clamp_(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
     scales = np.exp2(g.integers(lo, hi + 1, (n_pages, 2, hk)).astype(np.float64)).astype(np.float32)
-    return kv8.Kv8Cache(torch.from_numpy(codes).to(DEV), torch.from_numpy(scales).to(DEV))
+    return kv8.Kv8Cache(codes, torch.from_numpy(scales).to(DEV))
 
 
 def make_table(lens, n_pages, seed, extra=0, width=None):
@@ -567,6 +577,17 @@ def test_attention_many_requests(lib, dtype, n, len_hi, q_hi):
     lens, rows = g.integers(0, len_hi + 1, n), g.integers(0, q_hi + 1, n)
     rows = np.minimum(rows, np.maximum(lens, 1))
     check_attention([int(x) for x in lens], [int(x) for x in rows], 1, 8, 64, dtype, seed=n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("grp,d,rows", [(16, 64, 1), (2, 64, 1), (9, 128, 1), (1, 256, 1), (8, 64, 4), (1, 128, 40)])
+def test_attention_many_tiles(lib, dtype, grp, d, rows):
+    """Enough keys that every CTA runs through its ring of tiles several times (148 SMs, two CTAs
+    each, 12 tiles of 128 keys in a ring: 2 * 148 * 24 * 128 keys)."""
+    n = 13
+    lens = [2 * 148 * 24 * 128 // n + 37 * i for i in range(n)]
+    check_attention(lens, [rows] * n, 1, grp, d, dtype, seed=8)
 
 
 @pytest.mark.gpu
