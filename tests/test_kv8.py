@@ -655,7 +655,7 @@ def test_attention_leaves_other_rows(lib, rows):
                       err=err)
         with pytest.raises(DmError):
             kv8.check(err)
-        assert (out[:rows + 1] == 3).all() and not (out[rows + 1:2 * rows] == 3).any()
+        assert (out[:rows + 1] == 3).all() and not (out[rows + 1:2 * rows] == 3).all(-1).any()  # every row written
     # a page out of range: its keys are left out (request 1's second page)
     bad = table.copy()
     bad[1, 1] = cache.num_pages
