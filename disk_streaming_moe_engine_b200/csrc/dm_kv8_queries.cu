@@ -401,20 +401,22 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 tc_fence_before();
                 mbar_arrive(&s_free);
                 const bool edge = tile0 + kKeyTile > lim_min;
-                float mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 64; ++c) {
-                    s[c] = fmaf(s[c], f[c / 16], g[c / 16]);
-                    if (g[c / 16] == -INFINITY) s[c] = -INFINITY;
-                }
-                if (edge) {
+                for (int c = 0; c < 64; ++c) s[c] = fmaf(s[c], f[c / 16], g[c / 16]);
+                // keys that the row does not see, or that lie on no page
+                const bool gone = g[0] == -INFINITY || g[1] == -INFINITY || g[2] == -INFINITY || g[3] == -INFINITY;
+                if (edge || gone) {
                     const int seen = lim - tile0 - half * 64;
 #pragma unroll
                     for (int c = 0; c < 64; ++c)
-                        if (c >= seen) s[c] = -INFINITY;
+                        if (c >= seen || g[c / 16] == -INFINITY) s[c] = -INFINITY;
                 }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 64; ++c) mx = fmaxf(mx, s[c]);
+                for (int c = 0; c < 64; c += 8)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) m4[j] = fmaxf(m4[j], fmaxf(s[c + j], s[c + 4 + j]));
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 const bool over = mref == -INFINITY ? mx > -INFINITY : mx > kQryBoost + kQryLazy;
                 if (named_bar_or(2 + wq, 64, over)) {
                     // the row's two threads agree on its reference; O of the raised rows follows
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 // weights, sums, terms: columns of P0 and P1 of this half's 64 keys
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    float sum = 0.0f;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     uint32_t p0[4], p1[4];
 #pragma unroll
                     for (int c = 0; c < 16; c += 4) {
@@ -462,14 +464,14 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             y[j] = ex2(y[j]);
-                            sum += y[j];
+                            sum[j] += y[j];
                         }
                         e4m3_terms2(y[0], y[1], a0, a1);
                         e4m3_terms2(y[2], y[3], b0, b1);
                         p0[c / 4] = a0 | (b0 << 16);
                         p1[c / 4] = a1 | (b1 << 16);
                     }
-                    l = fmaf(sum, vinv[p], l);
+                    l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), vinv[p], l);
                     tc_st4(lanes + pb + p * 4, p0);
                     tc_st4(lanes + pb + 32 + p * 4, p1);
                 }
