@@ -653,7 +653,8 @@ extern "C" int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t
     a.in_place = seq_lens == ctx_lens || free_state_out == free_state;
     const int work = max_tokens > n ? max_tokens : n;
     const int block = work <= 256 ? 256 : 1024;
-    int grid = (max_tokens + 1023) / 1024;
+    // CTAs by the entries to write: the tokens', and the pages that requests may give back
+    int grid = ((max_tokens > 4 * n ? max_tokens : 4 * n) + 1023) / 1024;
     if (grid > g.num_sms) grid = g.num_sms;
     const size_t smem = 3 * static_cast<size_t>(n + 1) * sizeof(unsigned);
     cudaError_t e = cudaSuccess;

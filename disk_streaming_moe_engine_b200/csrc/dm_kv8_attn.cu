@@ -43,8 +43,8 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
                        p->num_q_heads, c->num_kv_heads);
     if (!std::isfinite(p->sm_scale))
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "sm_scale is not finite");
-    if (p->table_width < 1 || p->table_width >= (1 << 27))
-        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "table_width %d", p->table_width);
+    if (p->table_width < 1 || p->table_width > (1 << 26))
+        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "table_width %d: 1 to 2^26", p->table_width);
     if (p->max_q_len < 1 || (!p->cu_q && (p->max_q_len != 1 || p->rows < p->n)))
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st,
                        "need max_q_len >= 1; without cu_q max_q_len is 1 and rows >= n");

@@ -8,17 +8,20 @@
 //   O^T [D x N]         += codeV^T [D x 128] . Pterms [128 x N]
 // N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
 // scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
-// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  The tensor time of
-// a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
-// below the time of the tile's bytes from HBM, which is what bounds the kernel.
+// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  The tensor
+// time of a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
+// below the time of the tile's bytes from HBM, which is what bounds long caches: 64 requests of
+// 32768 tokens (2 kv heads of 256, 8 query heads each) take 346 us, 6.21 TB/s, 0.96 of the measured
+// copy bandwidth.  Short ones are bound by the chain of waits of one tile (0.65 us and more) and of
+// an item's start, end and join (2 to 4 us): one request of 4096 tokens takes 18 us.
 //
 // Softmax in base 2: with a page's scales sK, sV = 2^v,
 //   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
 // M the row's reference for x + v: raised to the running maximum whenever some x + v exceeds
 // it by more than 2 (then O^T and the sums are rescaled), so w <= 4 and 64 w stays in e4m3's
-// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t of a group of 128 owns token t of the
-// tile for 8 of the rows: scores, weights, its share of the row sums; only the reference
-// crosses threads.
+// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t of
+// a group of 128 owns token t of the tile for 8 of the rows: scores, weights, its share of the row
+// sums; only the reference crosses threads.
 //
 // Split: all items' tiles in one sequence, cut into one contiguous range per CTA (one or two per
 // SM, persistent), so ragged lengths balance to a tile.  An item cut by a range boundary
@@ -26,9 +29,10 @@
 // range order: the result does not depend on timing.
 //
 // Roles: RB / 8 groups of 4 warps for softmax, epilogue and Q preparation; a producer warp
-// (groups of 4 tiles, a lane per page: page ids and scales fetched groups ahead, TMA boxes of 16
-// rows; a missing page reads zeros); an MMA warp (one thread).  All waits are bounded; after a timeout every role
-// leaves and copies and MMAs in flight are waited for.
+// (groups of 4 tiles, a lane per page: page ids and scales fetched groups ahead, one TMA box per
+// page; a missing page reads zeros); an MMA warp (one thread).  All waits are bounded; after a
+// timeout every role leaves and copies and MMAs in flight are waited for.
+#include <atomic>
 #include <cmath>
 
 #include "dm_kv8_walk.cuh"
@@ -159,7 +163,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                         const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
-                            const uint64_t ad = f8_desc_m<CW>(v + c * S::Tile::kChunk, 0, S::Tile::kGroup);  // 64 wide: M rows 64-127 repeat 0-63
+                            // 64 wide: M rows 64-127 repeat rows 0-63
+                            const uint64_t ad = f8_desc_m<CW>(v + c * S::Tile::kChunk, 0, S::Tile::kGroup);
 #pragma unroll
                             for (int j = 0; j < kKeyTile / 32; ++j)
                                 f8_mma(tmem + (2 + c) * N, ad + j * (4 * S::Tile::kGroup / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
@@ -180,9 +185,10 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + r0;
         uint32_t t = 0;
         int item = 0;
-        bool ok = true;
+        bool ok = true;     // of this thread; all leave together, after a barrier that ORs !ok
+        bool left = false;
         KeyWalk<RB, kKeyLead> w(a, s_range);
-        while (w.unit < w.end && ok) {
+        while (w.unit < w.end) {
             int lim_min, lim_max;
             key_limits<RB>(a, w.r, w.block(), lim_min, lim_max);
             int t_begin, t_end, real;
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 const bool t2 = mbar_try_wait(&s_full[x & 1u], (x >> 1) & 1u);
                 const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
                 if (!(t1 && t2 && t3)) {
-                    ok = ring.wait_meta(x, a.err, abort_flag) &&
+                    ok = ok && ring.wait_meta(x, a.err, abort_flag) &&
                          mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag) &&
                          (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
                 }
@@ -295,10 +301,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                         const float mx = warp_max(y[r]);
                         if (lane == 0) s_red[wq][r0 + r] = mx;
                     }
-                    if (named_bar_or(1, SOFT, !ok)) {
-                        ok = false;
-                        break;
-                    }
+                    if ((left = named_bar_or(1, SOFT, !ok))) break;
                     float fac[8];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 tc_fence_before();
                 mbar_arrive(&p_ready[x & 1u]);
             }
-            if (!ok) break;
+            if (left) break;
             t += nt;
             // the item's sums, then O
 #pragma unroll
@@ -388,11 +391,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 const float s = warp_sum(l[r]);
                 if (lane == 0) s_red[wq][r0 + r] = s;
             }
-            ok = mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
-            if (named_bar_or(1, SOFT, !ok)) {
-                ok = false;
-                break;
-            }
+            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
+            if (named_bar_or(1, SOFT, !ok)) break;
             tc_fence_after();
 #pragma unroll
             for (int r = 0; r < 8; ++r) l[r] = s_red[0][r0 + r] + s_red[1][r0 + r] + s_red[2][r0 + r] + s_red[3][r0 + r];
@@ -543,12 +543,12 @@ bool kv8_encode_map(const dm_kv8_cache* c, bool pair, CUtensorMap* map) {
 template <typename T, int D, int RB, int CTAS>
 static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStream_t s) {
     using S = KeyShape<T, D, RB, CTAS>;
-    static bool ready[64] = {};
-    if (dev >= 64 || !ready[dev]) {
+    static std::atomic<bool> ready[64];
+    if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
         const cudaError_t e = cudaFuncSetAttribute(kv8_attn_keys_kernel<T, D, RB, CTAS>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
-        if (dev < 64) ready[dev] = true;
+        if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
     kv8_attn_keys_kernel<T, D, RB, CTAS><<<num_sms * S::kCtas, S::kThreads, S::kSmem, s>>>(ka);
     return cudaGetLastError();

@@ -28,6 +28,7 @@
 // (128 columns), two buffers of weights (64), O (D).  Split of the work, joins and bounded waits
 // as in the key-side kernel; after a failed wait every thread runs through the remaining barriers
 // without work.
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -543,12 +544,12 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
 template <int D>
 static cudaError_t launch_queries(const QryArgs& qa, int num_sms, int dev, cudaStream_t s) {
     using S = QryShape<D>;
-    static bool ready[64] = {};
-    if (dev >= 64 || !ready[dev]) {
+    static std::atomic<bool> ready[64];
+    if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
         const cudaError_t e = cudaFuncSetAttribute(kv8_attn_queries_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(S::kSmem));
         if (e != cudaSuccess) return e;
-        if (dev < 64) ready[dev] = true;
+        if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
     }
     kv8_attn_queries_kernel<D><<<num_sms, kQryThreads, S::kSmem, s>>>(qa);
     return cudaGetLastError();

@@ -478,6 +478,7 @@ int32_t dm_moe_layer_noalloc(int32_t hidden_size, int32_t moe_intermediate_size,
  * head_dim in {64, 128, 256}; pages 16-byte aligned. */
 #define DM_KV8_PAGE_TOKENS 16
 #define DM_KV8_MAX_REQUESTS 8192
+#define DM_DEVERR_TIMEOUT 0x1u    /* a bounded wait inside a kernel ran out               */
 #define DM_DEVERR_NONFINITE 0x2u  /* NaN / Inf among the appended values                  */
 #define DM_DEVERR_CAPACITY 0x4u   /* pages, table width or token buffers do not suffice   */
 #define DM_DEVERR_PAGE 0x8u       /* a page id or slot outside the cache                  */
@@ -492,7 +493,8 @@ typedef struct dm_kv8_cache {
 } dm_kv8_cache;
 
 /* Waits for `stream`, reads and clears *err_dev and returns it as a status (DM_OK,
- * DM_ERR_CAPACITY, DM_ERR_INVALID_ARG for PAGE and RANGE, DM_ERR_NONFINITE). */
+ * DM_ERR_TIMEOUT, DM_ERR_CAPACITY, DM_ERR_INVALID_ARG for PAGE and RANGE,
+ * DM_ERR_NONFINITE, in this order).  Not inside a capture. */
 int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t err_buf_size);
 
 /* Plans one step of n requests (1 <= n <= DM_KV8_MAX_REQUESTS).  Request i holds ctx_lens[i]
@@ -589,8 +591,10 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * dtype (q and out) bf16 or fp32; scores, softmax and sums are fp32.
  * lse (may be NULL) [rows][Hq] receives ln sum exp of the scaled scores.
  * workspace: dm_kv8_attention_workspace bytes, 256-byte aligned, zeroed once before its
- * first use; every call leaves it ready for the next.  Calls that may overlap in time
- * (other streams, graphs) need workspaces of their own. */
+ * first use; every call leaves it ready for the next (after a DM_DEVERR_TIMEOUT it has to be
+ * zeroed again).  Calls that may overlap in time (other streams, graphs) need workspaces of
+ * their own; graphs and calls that run one after the other may share one.
+ * table_width <= 2^26. */
 typedef struct dm_kv8_attn_args {
     int32_t dtype, n, num_q_heads, max_q_len;
     int32_t rows;              /* rows of q and out                                       */

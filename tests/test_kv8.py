@@ -223,7 +223,8 @@ def _fake_cache(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(pages=None), dict(scales=None), dict(head_dim=96), dict(num_pages=0),
-                                dict(num_kv_heads=0), dict(pages=(1 << 20) + 8), dict(reserved=1)])
+                                dict(num_kv_heads=0), dict(pages=(1 << 20) + 8), dict(reserved=1),
+                                dict(num_pages=1 << 26, num_kv_heads=8)])
 def test_cache_refusals(lib, kw):
     c = _fake_cache(**kw)
     one = 1 << 22  # never dereferenced: the checks come first
@@ -235,7 +236,7 @@ def test_cache_refusals(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=2), dict(n=-1), dict(rows=-1), dict(num_q_heads=3), dict(num_q_heads=0),
-                                dict(sm_scale=float("nan")), dict(table_width=0), dict(max_q_len=0),
+                                dict(sm_scale=float("nan")), dict(table_width=0), dict(table_width=(1 << 26) + 1), dict(max_q_len=0),
                                 dict(max_q_len=2), dict(rows=3), dict(reserved=1), dict(q=None), dict(out=None),
                                 dict(block_table=None), dict(seq_lens=None), dict(workspace=None),
                                 dict(workspace=(1 << 22) + 16)])
@@ -709,6 +710,41 @@ def test_attention_strides_stream_and_repeats(lib):
             kv8.attention(cache, wide[:, ::2, 4:132], dev32(table), dev32(lens), out=out[:, 1:], workspace=ws)
     side.synchronize()
     assert torch.equal(out[:, 1:], want) and (out[:, 0] == 0).all()
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_a_workspace(lib):
+    """Two captured calls of different shapes on one workspace, replayed in turn on another
+    stream than they were captured on: the same bits as eager calls."""
+    cache, table, cu, q, want = check_attention([900, 2500, 40], [1, 1, 1], 2, 8, 64, torch.bfloat16, seed=3)
+    q2 = torch.randn(60, 16, 64, generator=torch.Generator().manual_seed(1)).to(DEV, torch.bfloat16)
+    t, n1, n2, cu2 = dev32(table), dev32([900, 2500, 40]), dev32([700, 30, 33]), dev32([0, 20, 40, 60])
+    ws = kv8.attention_workspace(cache)
+    want2 = kv8.attention(cache, q2, t, n2, cu2, 20, workspace=ws)
+    out, out2 = torch.empty_like(q), torch.empty_like(q2)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graphs[0]):
+        kv8.attention(cache, q, t, n1, out=out, workspace=ws)
+    with torch.cuda.graph(graphs[1]):
+        kv8.attention(cache, q2, t, n2, cu2, 20, out=out2, workspace=ws)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for i in range(6):
+            out.zero_(), out2.zero_()
+            graphs[i % 2].replay()
+            graphs[(i + 1) % 2].replay()
+            side.synchronize()
+            assert torch.equal(out, want) and torch.equal(out2, want2)
+
+
+@pytest.mark.gpu
+def test_attention_repeats_bit_for_bit(lib):
+    """Split requests are joined in a fixed order whatever the arrival order."""
+    cache, table, cu, q, want = check_attention([30000, 5, 17001], [1, 1, 1], 2, 4, 128, torch.float32, seed=6)
+    ws = kv8.attention_workspace(cache)
+    for _ in range(20):
+        assert torch.equal(kv8.attention(cache, q, dev32(table), dev32([30000, 5, 17001]), workspace=ws), want)
 
 
 # ---- GPU: the chain as a server runs it ---------------------------------------------------------------
