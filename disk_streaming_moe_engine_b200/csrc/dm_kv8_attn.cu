@@ -85,8 +85,15 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     a.q_vec = kv8_aligned(a.q, a.q_rs, a.q_hs, elem, 32);
     a.o_vec = kv8_aligned(a.out, a.o_rs, a.o_hs, elem, 32);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // many bf16 rows per request and kv head: queries on the M side
-    const bool many = !f32 && static_cast<int64_t>(a.max_q) * a.group >= 64;
+    // Many bf16 rows per request and kv head: queries on the M side, 128 rows at a time.  The
+    // key-side kernel goes over the cache once per 16 rows but joins small parts; with few items a
+    // query-side item is cut into many large ones.  us on the key side / the query side at D = 64
+    // and D = 256 (2 kv heads): 128 items (64 requests of 1000 keys) 32 rows 32/32 49/56, 48 rows
+    // 41/32 66/55; 16 items (8 of 4000) 64 rows 29/31 40/46, 128 rows 37/31 55/49; 4 items (2 of
+    // 30000) 128 rows 46/47 80/117.
+    const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
+    const int64_t items = (rows + 127) / 128 * a.n * a.Hkv;
+    const bool many = !f32 && rows >= (2 * items >= g.num_sms ? 40 : items >= 8 ? 96 : 192);
     const cudaError_t e = many ? launch_kv8_queries(c, a, g.num_sms, g.dev, s)
                                : launch_kv8_keys(c, a, f32, g.num_sms, g.dev, s);
     if (e != cudaSuccess)

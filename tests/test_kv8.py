@@ -145,13 +145,13 @@ def attention_tolerance(out, mag, sat, d, keys, dtype, rows=1):
     bf16 outputs carry weights of at least 8 bits and their own rounding.  The 8 bits are two
     e4m3 terms, the second scaled by 2^4, of 64 times the weight (relative to the row's
     largest, at least 2^-2 of it): its smallest step is 2^-9 / 2^4 / 2^6, so a weight is off by
-    2^-20 of the largest one's p sV at least, on a code of V.  From 64 query rows per request and
-    kv head on, the second term has the scale of the first: 2^-16."""
+    2^-20 of the largest one's p sV at least, on a code of V.  From 40 query rows per request and
+    kv head on, the second term may have the scale of the first: 2^-16."""
     mag, small = mag
     ds = sat[..., None] * (d / 16 + 1) * 2.0 ** -22
     tol = (2 * ds + (keys / PAGE + 4) * 2.0 ** -22 + 2.0 ** -20) * mag
     if dtype == torch.bfloat16:
-        tol = tol + BF16_STEP * np.abs(out) + (BF16_STEP + 2 * sat[..., None] * 2.0 ** -13) * mag + (2.0 ** -16 if rows >= 64 else 2.0 ** -18) * small
+        tol = tol + BF16_STEP * np.abs(out) + (BF16_STEP + 2 * sat[..., None] * 2.0 ** -13) * mag + (2.0 ** -16 if rows >= 40 else 2.0 ** -18) * small
     return tol + 1e-30
 
 
