@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <cuda_fp8.h>
 
 #include "dm_common.cuh"
@@ -458,27 +459,33 @@ DM_DEV float2 e4m3x2_to_float2(uint32_t two) {
     return __half22float2(__half2(h));
 }
 
-// 8 consecutive elements of a row as floats
+// 8 consecutive elements of a row as loaded (bf16 stays packed: half the registers), and as floats
 template <typename T>
-DM_DEV void load8(const T* p, int vec, float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Row8 {
+    uint4 u[sizeof(T) / 2];
+    DM_DEV void load(const T* p, int vec) {
+        if (vec) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = bf16lo(w[i]);
-                v[2 * i + 1] = bf16hi(w[i]);
-            }
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         } else {
-            const float4 f = *reinterpret_cast<const float4*>(p), g = *reinterpret_cast<const float4*>(p + 4);
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
-        }
-    } else {
+            T e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(p[i]);
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+            memcpy(u, e, sizeof e);
+        }
     }
-}
+    DM_DEV void get(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 2) v[2 * j] = bf16lo(w[j]), v[2 * j + 1] = bf16hi(w[j]);
+                else v[4 * i + j] = __uint_as_float(w[j]);
+            }
+        }
+    }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a) {
@@ -513,17 +520,24 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
             if (tid == 0) raise_error(a.err, DM_DEVERR_PAGE);
             continue;
         }
-        float v[kPasses][8];
+        Row8<T> rows[kPasses];
         float amax = 0.0f;
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const int r = i * kRows + row;
             if (r < len) {
-                load8<T>(x + static_cast<int64_t>(t0 + r) * a.rs[kv], a.vec, v[i]);
+                rows[i].load(x + static_cast<int64_t>(t0 + r) * a.rs[kv], a.vec);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            if (i * kRows + row < len) {
+                float f[8];
+                rows[i].get(f);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float m = fabsf(v[i][e]);
+                    const float m = fabsf(f[e]);
                     if (m <= 3.402823466e38f) amax = fmaxf(amax, m);
                     else odd = true;
                 }
@@ -562,7 +576,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid
         for (int i = 0; i < kPasses; ++i) {
             const int r = i * kRows + row;
             if (r < len) {
-                const float* f = v[i];
+                float f[8];
+                rows[i].get(f);
                 *reinterpret_cast<uint2*>(dst + (off + r) * D) =
                     make_uint2(e4m3x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
                                e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
