@@ -87,7 +87,10 @@ static int launch_status(cudaError_t e, const char* stage, char* eb, uint64_t es
 // second kernel.  Reads and writes of the step never meet: new table entries lie behind the
 // ones that are read, released pages land at or above the count that the pops read below.
 // Only in-place lengths or an in-place count have to wait until every CTA has read them; the
-// last CTA to arrive writes those.
+// last CTA to arrive writes those.  What bounds it is that chain (lengths, three scans, a binary
+// search per token, a dependent table or stack read, the store), not its bytes: 64 requests with a
+// token each 3.4 us, 512 requests with up to 1000 new tokens each 7.5 us in a graph; a
+// call from Python costs 17 us of host time, the caller's torch allocation among it.
 struct Kv8PlanArgs {
     const int* ctx;
     const int* add;
@@ -276,7 +279,11 @@ __global__ void __launch_bounds__(1024) kv8_plan_kernel(const __grid_constant__ 
 // The angle pos * f is reduced to [-pi, pi] in 64 bits (at position 10^6 an fp32 angle has
 // lost 4 decimal digits); the reduced angle goes to fp32 as hi + lo, sin and cos of hi by
 // sincosf and the lo part to first order, so both are within an fp32 rounding or two.  The
-// angles of a CTA's tokens are computed once and used by every head.
+// angles of a CTA's tokens are computed once and used by every head.  Bound by the bytes, each
+// read and written once: 32771 tokens of 32 + 8 heads of 128, all of a head turned, take 116 us or
+// 5.77 TB/s (0.89 of the measured copy bandwidth); 64 tokens of 16 + 2 heads 3.65 us, the chain of
+// position, angle, barrier, store.  Sixteen tokens per CTA, four tokens' loads in flight, loads and
+// stores marked streaming and smaller register budgets gave nothing or cost 1 to 4 us.
 struct RopeArgs {
     dm_rope_plan plan;
     const void* x[2];
@@ -380,7 +387,8 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
                     const float hi = static_cast<float>(red), lo = static_cast<float>(red - static_cast<double>(hi));
                     float s, c;
                     sincosf(hi, &s, &c);
-                    cs[t][j % VEC * pu + j / VEC] = make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
+                    cs[t][j % VEC * pu + j / VEC] =
+                        make_float2((c - s * lo) * a.plan.mscale, (s + c * lo) * a.plan.mscale);
                 }
                 __syncthreads();
             }
@@ -426,7 +434,11 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
 // ---- quantising append ----------------------------------------------------------------------
 // A run is the rows of one call that fall into one page.  One CTA quantises a run of one kv
 // head's K or V: all its rows in registers, the largest magnitude over the CTA, then the
-// codes; the page's older codes are touched only when the scale grows.
+// codes; the page's older codes are touched only when the scale grows.  Bound by the bytes for
+// prompts, read once (bf16 rows stay packed, 48 registers at D = 256 where fp32 copies took 64 and
+// 20.5 us): 17.5 k tokens of 2 heads of 256 take 15.9 us, 12.3 us with the rows in L2, against 8.3 us
+// for the bytes; the difference is the launch and one chain of slot, load, maximum, barrier, store.
+// 64 single tokens take 2.3 us in a graph, that chain alone.
 struct Kv8AppendArgs {
     uint8_t* pages;
     float* scales;
@@ -466,7 +478,8 @@ struct Row8 {
     DM_DEV void load(const T* p, int vec) {
         if (vec) {
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+                u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         } else {
             T e[8];
 #pragma unroll
@@ -671,6 +684,8 @@ extern "C" int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t
     // CTAs by the entries to write: the tokens', and the pages that requests may give back
     int grid = ((max_tokens > 4 * n ? max_tokens : 4 * n) + 1023) / 1024;
     if (grid > g.num_sms) grid = g.num_sms;
+    // lengths in place, the count not: no word of free_state_out is known to be zero, so one CTA
+    if (seq_lens == ctx_lens && free_state_out != free_state) grid = 1;
     const size_t smem = 3 * static_cast<size_t>(n + 1) * sizeof(unsigned);
     cudaError_t e = cudaSuccess;
     if (smem > 40 * 1024)
@@ -737,8 +752,8 @@ extern "C" int32_t dm_rope(const dm_rope_plan* plan, int32_t dtype, int32_t n, c
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "no plan of dm_rope_plan_init");
     if (dtype != DM_DTYPE_BF16 && dtype != DM_DTYPE_F32)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "dtype is bf16 or fp32");
-    if (n < 0 || Hq < 0 || Hk < 0 || Hq > 65536 || Hk > 65536)
-        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "negative (or absurd) n or head count");
+    if (n < 0 || n > (1 << 30) || Hq < 0 || Hk < 0 || Hq > 65536 || Hk > 65536)
+        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "n: 0 to 2^30, head counts: 0 to 65536");
     if (n == 0 || Hq + Hk == 0) return DM_OK;
     if (!positions || (Hq && (!q || !qo)) || (Hk && (!k || !ko)))
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "null pointer");
@@ -760,10 +775,11 @@ extern "C" int32_t dm_rope(const dm_rope_plan* plan, int32_t dtype, int32_t n, c
                 return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "in place needs the same strides");
             a.inplace[i] = 1;
         }
-        vec = vec && kv8_aligned(a.x[i], a.x_rs[i], a.x_hs[i], elem, 16) && kv8_aligned(a.y[i], a.y_rs[i], a.y_hs[i], elem, 16);
+        vec = vec && kv8_aligned(a.x[i], a.x_rs[i], a.x_hs[i], elem, 16) &&
+              kv8_aligned(a.y[i], a.y_rs[i], a.y_hs[i], elem, 16);
     }
     // few tokens: a CTA each, for the shortest wait; many: 8, whose angles are then computed by
-    // the CTA's threads in one round (32771 tokens of 40 heads: see the figures above)
+    // the CTA's threads in one round
     a.tok = n <= 8 * g.num_sms ? 1 : kRopeTok;
     const int grid = (n + a.tok - 1) / a.tok;
     // threads: the units of a token in equal rounds

@@ -7,7 +7,9 @@
 namespace dm {
 
 // Workspace: a counter per CTA, two per SM at most (zero between calls), then the partial results.
-static size_t counter_bytes(int num_sms) { return (static_cast<size_t>(2 * num_sms) * sizeof(unsigned) + 255) / 256 * 256; }
+static size_t counter_bytes(int num_sms) {
+    return (static_cast<size_t>(2 * num_sms) * sizeof(unsigned) + 255) / 256 * 256;
+}
 static size_t workspace_bytes(int D, int num_sms) {
     const size_t k = kv8_keys_part_floats(D, num_sms), q = kv8_queries_part_floats(D, num_sms);
     return counter_bytes(num_sms) + (k > q ? k : q) * sizeof(float);
@@ -48,6 +50,8 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     if (p->max_q_len < 1 || (!p->cu_q && (p->max_q_len != 1 || p->rows < p->n)))
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st,
                        "need max_q_len >= 1; without cu_q max_q_len is 1 and rows >= n");
+    if (static_cast<int64_t>(p->rows) * p->num_q_heads > 0x7fffffffLL)
+        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "rows * num_q_heads must be below 2^31");
     if (p->n == 0 || p->rows == 0) return DM_OK;
     if (!p->q || !p->out || !p->block_table || !p->seq_lens || !p->workspace)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "null pointer");

@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 named_bar_sync(1, SOFT);
                 if (s_last) {
                     // the parts' references and sums to factors, 32 parts at a time, then O: every
-                    // thread sums its float4s over the parts, four parts' loads in flight
+                    // thread sums its float4s over the parts, eight parts' loads in flight
                     auto part_of = [&](int c) {
                         return a.part + (static_cast<size_t>(c) * 2 + (c == c_first ? 1 : 0)) * kSlot;
                     };

@@ -336,8 +336,9 @@ struct KeyTile {
     static DM_DEV int row(int token) { return token / 8 * kGroup + token % 8 * CW; }  // chunk 0
 };
 
-// Producer (one warp): a tile's K or V (or both) in one TMA box per page, one lane per page; page ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A
-// page that is missing or holds no key of the item reads zeros.
+// Producer (one warp): a tile's K or V (or both) in one TMA box per page, one lane per page; page
+// ids fetched two groups of 4 tiles ahead of their use, scales one group ahead.  A page that is
+// missing or holds no key of the item reads zeros.
 template <int RB, int LEAD, int D, int SL, bool PAIR>
 DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* sm, KeyRing<SL, PAIR>& ring,
                         const KeyRange& range, volatile int* abort_flag) {
@@ -391,7 +392,8 @@ DM_DEV void key_produce(const Kv8AttnArgs& a, const CUtensorMap* map, uint8_t* s
     // K (kv 0) or V (kv 1), or both in pairs, of the tile with these pages into ring position `at`
     auto load = [&](uint32_t at, int id, int h, int kv) {
         const uint32_t si = at % SL;
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[si], ((at / SL) & 1u) ^ 1u, a.err, abort_flag))) return false;
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ring.empty[si], ((at / SL) & 1u) ^ 1u, a.err, abort_flag)))
+            return false;
         if (lane == 0) mbar_arrive_expect_tx(&ring.full[si], kSlot);
         if (lane == static_cast<int>(si)) last = static_cast<int>(at);
         __syncwarp();

@@ -4,6 +4,8 @@
         --layer 0 --iters 20
     python -m disk_streaming_moe_engine_b200.kernel_bench --preset layer --kernel battn \
         --batch 16 --ctx 8192 --iters 5
+    python -m disk_streaming_moe_engine_b200.kernel_bench --kernel kv8_attn --batch 16 \
+        --ctx 16384 --new 1 --iters 5
 
 The model is synthesised on the device; with --warm the layer first runs one real token
 (so router ids, activations and the KV position are those of a real step).  Prints one
@@ -31,6 +33,7 @@ Q4_SLOTS = 2 * Q4_MAX_CTAS + 40
 # kernels of the batched step (--batch N): layer is the preset's attention or GDN layer
 BKERNELS = {"battn": _lib.DM_BKERNEL_ATTN, "bgdn": _lib.DM_BKERNEL_GDN_REC, "bexperts": _lib.DM_BKERNEL_EXPERTS,
             "brouter": _lib.DM_BKERNEL_ROUTER, "bgemm": _lib.DM_BKERNEL_GEMM_IN}
+KV8_OPS = ["kv8_append", "kv8_attn", "kv8_plan", "kv8_rope"]  # --batch N --ctx C --new M
 
 
 def batched(a, cfg):
@@ -83,11 +86,60 @@ def batched(a, cfg):
                           "bytes": nbytes, "GBps": nbytes / (ms * 1e-3) / 1e9, "pipeline_us": pipe}))
 
 
+def kv8_op(a, cfg):
+    """One operator of the 8-bit paged cache at the preset's attention shape: --batch requests of
+    --ctx tokens, the last --new of them the step's (bf16; a shuffled page pool)."""
+    import torch
+
+    from . import kv8
+    torch.manual_seed(a.seed)
+    n, rows, hk, hq, d = a.batch, a.batch * a.new, cfg.num_key_value_heads, cfg.num_attention_heads, cfg.head_dim
+    if not 1 <= a.new <= a.ctx:
+        raise SystemExit("need 1 <= --new <= --ctx")
+    width = (a.ctx + 15) // 16
+    cache = kv8.Kv8Cache.empty(n * width, hk, d)
+    cache.scales.fill_(2.0 ** -6)
+    cache.pages.copy_(torch.randint(0, 120, (n * width, 2, hk, 16, 1), dtype=torch.uint8, device="cuda"))
+    cache.pages[..., 1::2] ^= 0x80
+    table = torch.randperm(n * width, device="cuda").int().view(n, width)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    lens, ctx, new, err = ints(*[a.ctx] * n), ints(*[a.ctx - a.new] * n), ints(*[a.new] * n), kv8.error_word()
+    held = (a.ctx - a.new + 15) // 16
+    free, state, left = table[:, held:].flatten(), ints(n * (width - held), 0), ints(0, 0)
+    free = torch.cat([free, ints(0)])  # never empty
+    plan = kv8.plan_slots(free, state, table.clone(), ctx, new, rows, state_out=left, err=err)
+    cu = ints(*range(0, rows + 1, a.new))
+    q, out = torch.randn(rows, hq, d, device="cuda").bfloat16(), torch.empty(rows, hq, d, device="cuda").bfloat16()
+    k, v = torch.randn(rows, hk, d, device="cuda").bfloat16(), torch.randn(rows, hk, d, device="cuda").bfloat16()
+    rope, ws = kv8.RopePlan(d, cfg.rotary_dim), kv8.attention_workspace(cache)
+    kv, qo = 2 * hk * d, hq * d
+    run, nbytes = {
+        "kv8_plan": (lambda: kv8.plan_slots(free, state, table, ctx, new, rows, state_out=left, out=plan, err=err),
+                     12 * rows + 16 * n + 8 * n * (width - held)),
+        "kv8_rope": (lambda: kv8.rope(rope, q, k, plan.positions, q_out=out, k_out=v), 4 * rows * (hq + hk) * d),
+        "kv8_append": (lambda: kv8.append(cache, k, v, plan.slots, err=err), 3 * rows * kv),
+        "kv8_attn": (lambda: kv8.attention(cache, q, table, lens, cu, a.new, out=out, workspace=ws, err=err),
+                     n * a.ctx * kv + 4 * rows * qo),
+    }[a.kernel]
+    for _ in range(3):
+        run()
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record()
+    for _ in range(a.iters):
+        run()
+    t1.record()
+    kv8.check(err)
+    us = t0.elapsed_time(t1) / a.iters * 1e3
+    print(json.dumps({"kernel": a.kernel, "batch": n, "ctx": a.ctx, "new": a.new, "us": us, "bytes": nbytes,
+                      "GBps": nbytes / us / 1e3}))
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--preset", default="layer")
-    ap.add_argument("--kernel", default="in_proj", choices=sorted(KERNELS) + sorted(BKERNELS))
-    ap.add_argument("--batch", type=int, default=0, help="batched-step kernels: sequences per step")
+    ap.add_argument("--kernel", default="in_proj", choices=sorted(KERNELS) + sorted(BKERNELS) + KV8_OPS)
+    ap.add_argument("--batch", type=int, default=0, help="batched-step kernels and 8-bit cache operators: sequences")
+    ap.add_argument("--new", type=int, default=1, help="8-bit cache operators: the step's tokens per sequence")
     ap.add_argument("--layer", type=int, default=0)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--ctx", type=int, default=0, help="tokens already in the KV cache / GDN state")
@@ -103,6 +155,10 @@ def main():
         if a.batch <= 0:
             raise SystemExit("--batch N is required for the batched kernels")
         return batched(a, cfg)
+    if a.kernel in KV8_OPS:
+        if a.batch <= 0:
+            raise SystemExit("--batch N is required for the 8-bit cache operators")
+        return kv8_op(a, cfg)
     with Engine(cfg, RuntimeConfig.for_context(a.ctx + 64)) as eng:
         eng.synth_on_device(a.seed)
         eng.seq_reset(0)

@@ -10,11 +10,14 @@ A host runtime that keeps its own paged cache runs, per step,
 
 Every call runs on torch's current stream (or `stream`, a cudaStream_t) of the tensors' device
 and returns without waiting, so a step may be captured into a CUDA graph (with the outputs
-given).  Arguments are checked on the host and raise DmError; what only the device can see
-goes into the error word of `error_word()` and is raised by `check()`.
+given).  Outputs that are not given are allocated on the stream of the call.  The operators serve:
+they have no gradients and refuse tensors that ask for one.  Arguments are checked on the host
+and raise DmError; what only the device can see goes into the error word of `error_word()` and is
+raised by `check()`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from typing import NamedTuple
@@ -45,11 +48,19 @@ def _raise(rc: int, buf):
 
 
 def _bad(detail: str):
-    raise _lib.DmError(_lib.DM_ERR_INVALID_ARG, '{"error_type":"INVALID_ARG","detail":"%s","stage":"kv8","layer":-1}' % detail)
+    raise _lib.DmError(_lib.DM_ERR_INVALID_ARG,
+                       '{"error_type":"INVALID_ARG","detail":"%s","stage":"kv8","layer":-1}' % detail)
 
 
 def _stream(device, stream) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream
+
+
+def _allocating(device, stream):
+    """Where a call's outputs are allocated: torch reuses memory in the order of one stream."""
+    if stream is None or device.type != "cuda":
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device))
 
 
 def _ints(device, names, *tensors):
@@ -68,6 +79,8 @@ def _rows(name: str, t: torch.Tensor, heads, dim: int, device, dtype):
             or t.device != device or (stride[2] != 1 and t.numel())):
         _bad(f"{name} must be [rows][{'heads' if heads is None else heads}][{dim}] {dtype} on {device}, head elements "
              f"contiguous (got {tuple(shape)} {t.dtype} on {t.device})")
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(f"{name} asks for a gradient; the operator has none (use torch.no_grad or detach)")
     return t.data_ptr(), stride[0], stride[1], shape[0], shape[1]
 
 
@@ -135,7 +148,8 @@ def plan_slots(free_pages, free_state, block_table, ctx_lens, new_lens, max_toke
     dev = ctx_lens.device
     n = ctx_lens.numel()
     if out is None:
-        room = ctx_lens.new_empty(2 * n + 1 + 3 * max_tokens)
+        with _allocating(dev, stream):
+            room = ctx_lens.new_empty(2 * n + 1 + 3 * max_tokens)
         out = SlotPlan(*room.split_with_sizes((n, n + 1, max_tokens, max_tokens, max_tokens)))
     else:
         _ints(dev, "seq_lens cu_new slots positions requests", *out)
@@ -195,8 +209,10 @@ def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     k = q[:, :0] if k is None else k
-    q_out = torch.empty_like(q) if q_out is None else q_out
-    k_out = torch.empty_like(k) if k_out is None else k_out
+    if q_out is None or k_out is None:
+        with _allocating(dev, stream):
+            q_out = torch.empty_like(q) if q_out is None else q_out
+            k_out = torch.empty_like(k) if k_out is None else k_out
     q_ptr, q_rs, q_hs, q_rows, hq = _rows("q", q, None, D, dev, q.dtype)
     k_ptr, k_rs, k_hs, k_rows, hk = _rows("k", k, None, D, dev, q.dtype)
     qo_ptr, qo_rs, qo_hs, qo_rows, _ = _rows("q_out", q_out, hq, D, dev, q.dtype)
@@ -252,7 +268,8 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     q_ptr, q_rs, q_hs, rows, hq = _rows("q", q, None, D, dev, q.dtype)
     if out is None:
-        out = torch.empty_like(q)
+        with _allocating(dev, stream):
+            out = torch.empty_like(q)
     out_ptr, out_rs, out_hs, out_rows, _ = _rows("out", out, hq, D, dev, q.dtype)
     _ints(dev, "block_table seq_lens cu_q err", block_table, seq_lens, cu_q, err)
     if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \

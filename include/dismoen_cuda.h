@@ -506,7 +506,7 @@ int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t e
  *     The j-th new page (in request, then page order) is the j-th from the top of
  *     free_pages[0 .. count) followed by the released pages (same order).
  *   free_state int32[2] {count, 0}; free_state_out receives {count after, 0} and may be the
- *     same array (its second word is the library's, zero between calls).
+ *     same array (whose second word is the library's, zero between calls).
  *   seq_lens [n] lengths after the step (may be ctx_lens itself), cu_new [n + 1] prefix sums
  *     of the new tokens, and per new token (request, then position order) slots[t] =
  *     page * 16 + position % 16, positions[t], requests[t]; entries [total, max_tokens)
@@ -514,7 +514,7 @@ int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t e
  * All or nothing: when pages, the table's width, max_tokens or free_capacity do not suffice
  * (DM_DEVERR_CAPACITY) or a length is negative (DM_DEVERR_RANGE), no page moves, the
  * lengths stay ctx_lens, cu_new is all 0 and the token arrays all -1.
- * n * table_width <= 2^27, max_tokens <= 2^30. */
+ * n * table_width <= 2^27, max_tokens <= 2^30.  No overlap but the two named. */
 int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table,
                     int32_t table_width, int32_t* free_pages, int32_t free_capacity, const int32_t* free_state,
                     int32_t* free_state_out, int32_t* seq_lens, int32_t* cu_new, int32_t max_tokens, int32_t* slots,
@@ -594,7 +594,7 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * first use; every call leaves it ready for the next (after a DM_DEVERR_TIMEOUT it has to be
  * zeroed again).  Calls that may overlap in time (other streams, graphs) need workspaces of
  * their own; graphs and calls that run one after the other may share one.
- * table_width <= 2^26. */
+ * table_width <= 2^26, rows * num_q_heads < 2^31; out overlaps no input. */
 typedef struct dm_kv8_attn_args {
     int32_t dtype, n, num_q_heads, max_q_len;
     int32_t rows;              /* rows of q and out                                       */

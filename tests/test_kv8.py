@@ -251,6 +251,20 @@ def test_attention_refusals(lib, kw):
     assert rc == _lib.DM_ERR_INVALID_ARG
 
 
+def test_size_refusals(lib):
+    """Counts whose products would pass 32 bits in the kernels."""
+    c, one = _fake_cache(), 1 << 22
+    a = _lib.DmKv8AttnArgs(dtype=0, n=1, num_q_heads=1 << 11, max_q_len=1, rows=1 << 20, table_width=1, sm_scale=0.1,
+                           q=one, out=one, block_table=one, seq_lens=one, workspace=one, workspace_bytes=1 << 40)
+    rc, err = _call(lib, "dm_kv8_attention", C.addressof(c), C.addressof(a), None)
+    assert rc == _lib.DM_ERR_INVALID_ARG and "2^31" in err["detail"]
+    plan = kv8.RopePlan(64)
+    for n, hq in (((1 << 30) + 1, 1), (1, 65537), (-1, 1)):
+        rc, err = _call(lib, "dm_rope", plan._ref, 0, n, one, one, 64, 64, one, 64, 64, hq, None, 0, 0, None, 0, 0, 0,
+                        None)
+        assert rc == _lib.DM_ERR_INVALID_ARG and "2^30" in err["detail"]
+
+
 def test_empty_calls_need_no_device(lib):
     c, one = _fake_cache(), 1 << 22
     assert _call(lib, "dm_kv8_append", C.addressof(c), 0, 0, one, 0, 0, one, 0, 0, one, None, None)[0] == 0
@@ -390,6 +404,35 @@ def test_plan(lib, n, ctx_hi, new_hi, release, pad, seed, in_place):
 @pytest.mark.parametrize("in_place", [False, True])
 def test_plan_all_or_nothing(lib, ctx, new, width, cap, used, tokens, in_place):
     assert run_plan(ctx, new, width, cap, used, tokens, 1, in_place)[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("own_lens,own_state", [(True, False), (False, True), (False, False)])
+def test_plan_partly_in_place(lib, own_lens, own_state):
+    """Only the lengths, or only the state, in place, over many CTAs; a separate state's memory
+    holds anything before the call."""
+    n, new = 40, 700
+    cap = n * 47
+    free, state = kv8.free_list(cap)
+    table = torch.zeros((n, 48), dtype=torch.int32, device=DEV)
+    lens = dev32([30] * n)
+    tok = torch.zeros((3, n * new), dtype=torch.int32, device=DEV)
+    held = kv8.plan_slots(free, state, table, dev32([0] * n), lens, 30 * n)  # pages of the old tokens
+    count = int(state[0])
+    pages, old = free.cpu().numpy().copy(), table.cpu().numpy().copy()
+    out = kv8.SlotPlan(lens if own_lens else torch.zeros_like(lens), torch.zeros(n + 1, dtype=torch.int32, device=DEV),
+                       tok[0], tok[1], tok[2])
+    state_out = None if own_state else dev32([-7, 1234567])
+    err = kv8.error_word()
+    p = kv8.plan_slots(free, state, table, lens, dev32([new] * n), n * new, state_out=state_out, out=out, err=err)
+    kv8.check(err)
+    refused, want_lens, cu, slots, pos, req, want_table, _, left = plain_plan(pages, count, old, [30] * n, [new] * n,
+                                                                              n * new)
+    assert not refused and held.seq_lens.tolist() == [30] * n
+    for got, ref in zip(p, (want_lens, cu, slots, pos, req)):
+        np.testing.assert_array_equal(got.cpu().numpy(), np.asarray(ref, np.int32))
+    np.testing.assert_array_equal(table.cpu().numpy(), want_table)
+    assert (state if own_state else state_out).tolist() == [left, 0]
 
 
 # ---- GPU: rope ----------------------------------------------------------------------------------
@@ -745,6 +788,52 @@ def test_attention_repeats_bit_for_bit(lib):
     ws = kv8.attention_workspace(cache)
     for _ in range(20):
         assert torch.equal(kv8.attention(cache, q, dev32(table), dev32([30000, 5, 17001]), workspace=ws), want)
+
+
+@pytest.mark.gpu
+def test_outputs_follow_the_given_stream(lib):
+    """Outputs that a call with `stream` allocates belong to that stream: memory that the current
+    stream still uses is not handed out."""
+    side = torch.cuda.Stream()
+    plan, pos = kv8.RopePlan(64), dev32(range(512))
+    q = torch.randn(512, 8, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    want, _ = kv8.rope(plan, q, None, pos)
+    torch.cuda.synchronize()
+    for s in (side.cuda_stream, 0):
+        busy = torch.empty_like(q)
+        for _ in range(50):
+            busy.fill_(1.0)
+        del busy  # its memory is free for the current stream alone
+        got, _ = kv8.rope(plan, q, None, pos, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused(lib):
+    cache = kv8.Kv8Cache.empty(4, 2, 64)
+    q = torch.zeros(1, 4, 64, device=DEV, requires_grad=True)
+    k = torch.zeros(1, 2, 64, device=DEV)
+    ws, one = kv8.attention_workspace(cache), dev32([1])
+    for call in (lambda: kv8.rope(kv8.RopePlan(64), q, None, one),
+                 lambda: kv8.append(cache, k, q[:, :2], dev32([0])),
+                 lambda: kv8.attention(cache, q, dev32([[0]]), one, workspace=ws)):
+        with pytest.raises(DmError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", ["kv8_append", "kv8_attn", "kv8_plan", "kv8_rope"])
+@pytest.mark.parametrize("batch,ctx,new", [(2, 100, 1), (3, 70, 33), (1, 16, 16)])
+def test_kernel_bench_runs(lib, capsys, monkeypatch, kernel, batch, ctx, new):
+    from disk_streaming_moe_engine_b200 import kernel_bench
+    monkeypatch.setattr("sys.argv", ["kernel_bench", "--preset", "mini", "--kernel", kernel, "--batch", str(batch),
+                                     "--ctx", str(ctx), "--new", str(new), "--iters", "2"])
+    kernel_bench.main()
+    line = json.loads(capsys.readouterr().out)
+    assert line["kernel"] == kernel and line["us"] > 0 and line["bytes"] > 0
 
 
 # ---- GPU: the chain as a server runs it ---------------------------------------------------------------
