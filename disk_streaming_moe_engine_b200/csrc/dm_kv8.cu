@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
 // head's K or V: all its rows in registers, the largest magnitude over the CTA, then the
 // codes; the page's older codes are touched only when the scale grows.  Bound by the bytes for
 // prompts, read once (bf16 rows stay packed, 48 registers at D = 256 where fp32 copies took 64 and
-// 20.5 us): 17.5 k tokens of 2 heads of 256 take 15.9 us, 12.3 us with the rows in L2, against 8.3 us
+// 20.5 us): 17.5 k tokens of 2 heads of 256 take 14.4 us, 12.3 us with the rows in L2, against 8.3 us
 // for the bytes; the difference is the launch and one chain of slot, load, maximum, barrier, store.
 // 64 single tokens take 2.3 us in a graph, that chain alone.
 struct Kv8AppendArgs {

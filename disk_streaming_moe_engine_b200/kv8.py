@@ -17,7 +17,6 @@ raised by `check()`.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import threading
 from typing import NamedTuple
@@ -56,11 +55,12 @@ def _stream(device, stream) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream
 
 
-def _allocating(device, stream):
-    """Where a call's outputs are allocated: torch reuses memory in the order of one stream."""
+def _allocate(device, stream, make, *args):
+    """A call's output, on the stream of the call: torch reuses memory in the order of one stream."""
     if stream is None or device.type != "cuda":
-        return contextlib.nullcontext()
-    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device))
+        return make(*args)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)):
+        return make(*args)
 
 
 def _ints(device, names, *tensors):
@@ -148,8 +148,7 @@ def plan_slots(free_pages, free_state, block_table, ctx_lens, new_lens, max_toke
     dev = ctx_lens.device
     n = ctx_lens.numel()
     if out is None:
-        with _allocating(dev, stream):
-            room = ctx_lens.new_empty(2 * n + 1 + 3 * max_tokens)
+        room = _allocate(dev, stream, ctx_lens.new_empty, 2 * n + 1 + 3 * max_tokens)
         out = SlotPlan(*room.split_with_sizes((n, n + 1, max_tokens, max_tokens, max_tokens)))
     else:
         _ints(dev, "seq_lens cu_new slots positions requests", *out)
@@ -209,10 +208,8 @@ def rope(plan: RopePlan, q, k, positions, *, q_out=None, k_out=None, stream=None
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     k = q[:, :0] if k is None else k
-    if q_out is None or k_out is None:
-        with _allocating(dev, stream):
-            q_out = torch.empty_like(q) if q_out is None else q_out
-            k_out = torch.empty_like(k) if k_out is None else k_out
+    q_out = _allocate(dev, stream, torch.empty_like, q) if q_out is None else q_out
+    k_out = _allocate(dev, stream, torch.empty_like, k) if k_out is None else k_out
     q_ptr, q_rs, q_hs, q_rows, hq = _rows("q", q, None, D, dev, q.dtype)
     k_ptr, k_rs, k_hs, k_rows, hk = _rows("k", k, None, D, dev, q.dtype)
     qo_ptr, qo_rs, qo_hs, qo_rows, _ = _rows("q_out", q_out, hq, D, dev, q.dtype)
@@ -268,8 +265,7 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     q_ptr, q_rs, q_hs, rows, hq = _rows("q", q, None, D, dev, q.dtype)
     if out is None:
-        with _allocating(dev, stream):
-            out = torch.empty_like(q)
+        out = _allocate(dev, stream, torch.empty_like, q)
     out_ptr, out_rs, out_hs, out_rows, _ = _rows("out", out, hq, D, dev, q.dtype)
     _ints(dev, "block_table seq_lens cu_q err", block_table, seq_lens, cu_q, err)
     if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \
