@@ -313,9 +313,9 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     }
                     if (i > 0) {
                         tc_fence_after();
-#pragma unroll
+#pragma unroll 1  // rare: little code
                         for (int c = 0; c < S::kChunks; ++c)
-#pragma unroll
+#pragma unroll(TERMS == 2 ? 2 : 1)
                             for (int b = 0; b < TERMS; ++b) {
                                 float o[8];
                                 tc_ld8(lanes + (2 + c) * N + b * RB, o);
@@ -402,13 +402,19 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
             const bool whole = t_begin == 0 && nt == real;
             constexpr int kSlot = (RB * (D + 2) + 3) / 4 * 4;
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (t_begin == 0 ? 1 : 0)) * kSlot;
+            // o is the result already; a row that saw no key keeps the reference -inf
             auto put = [&](int r, int d, float o, float mm, float ll) {
                 if (r >= nrow) return;
-                // a row that saw no key keeps the reference -inf
-                static_cast<T*>(a.out)[s_off[item & 1][r] + d] = static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o / ll);
+                static_cast<T*>(a.out)[s_off[item & 1][r] + d] = static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o);
                 if (d == 0 && a.lse) a.lse[s_lse[item & 1][r]] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
             };
+            // Runs once per item, mostly from a cold instruction cache: one reciprocal per row (to 2
+            // units of fp32 for bf16 results) and one chunk's code.
+            auto reciprocal = [](float ll) { return sizeof(T) == 2 ? __fdividef(1.0f, ll) : __frcp_rn(ll); };
+            float scale[8];
 #pragma unroll
+            for (int r = 0; r < 8; ++r) scale[r] = reciprocal(l[r]);
+#pragma unroll 1
             for (int c = 0; c < S::kChunks; ++c) {
                 float o[8], v[TERMS][8];
 #pragma unroll
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 if (tt < CW) {
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
-                        if (whole) put(r0 + r, c * CW + tt, o[r], mref[r], l[r]);
+                        if (whole) put(r0 + r, c * CW + tt, o[r] * scale[r], mref[r], l[r]);
                         else slot[(r0 + r) * D + c * CW + tt] = o[r];
                     }
                 }
@@ -496,11 +502,11 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll
                     for (int j = 0; j < kVec; ++j) {
                         const int e = (j * SOFT + tid) * 4, row = e / D, d = e % D;
-                        const float m2 = s_red[0][row], l2 = s_red[1][row];
-                        put(row, d, o[j].x, m2, l2);
-                        put(row, d + 1, o[j].y, m2, l2);
-                        put(row, d + 2, o[j].z, m2, l2);
-                        put(row, d + 3, o[j].w, m2, l2);
+                        const float m2 = s_red[0][row], l2 = s_red[1][row], inv = reciprocal(l2);
+                        put(row, d, o[j].x * inv, m2, l2);
+                        put(row, d + 1, o[j].y * inv, m2, l2);
+                        put(row, d + 2, o[j].z * inv, m2, l2);
+                        put(row, d + 3, o[j].w * inv, m2, l2);
                     }
                     named_bar_sync(1, SOFT);  // s_red is free again
                 }
@@ -557,7 +563,7 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
 // CTAs per SM.  A tile's chain of waits takes 0.65 us and more whatever D is, its bytes from HBM
 // 0.37 us at D = 64 and 1.5 us at D = 256: two CTAs overlap their chains where they fit (D <= 128).
 // With 16 rows two leave each thread 96 registers, with some spills: fp32 chunks of 5 x 150 rows at
-// D = 128 take 365 us against 461 us with one, but one token of 16 heads (32 x 8000 keys) 48 us
+// D = 128 took 365 us against 461 us with one (326 us since the code run once per item is small), but one token of 16 heads (32 x 8000 keys) 48 us
 // against 45 us, so one token per request takes one CTA there.
 template <typename T, int RB>
 static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev, cudaStream_t s) {
