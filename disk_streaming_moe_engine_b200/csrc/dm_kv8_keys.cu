@@ -563,8 +563,9 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
 // CTAs per SM.  A tile's chain of waits takes 0.65 us and more whatever D is, its bytes from HBM
 // 0.37 us at D = 64 and 1.5 us at D = 256: two CTAs overlap their chains where they fit (D <= 128).
 // With 16 rows two leave each thread 96 registers, with some spills: fp32 chunks of 5 x 150 rows at
-// D = 128 took 365 us against 461 us with one (326 us since the code run once per item is small), but one token of 16 heads (32 x 8000 keys) 48 us
-// against 45 us, so one token per request takes one CTA there.
+// D = 128 took 365 us against 461 us with one (326 us now that an item's end is little code), but
+// one token of 16 heads (32 x 8000 keys) 48 us against 45 us, so one token per request takes one
+// CTA there.
 template <typename T, int RB>
 static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev, cudaStream_t s) {
     if (D == 64) return launch_keys<T, 64, RB, 2>(ka, num_sms, dev, s);
