@@ -5,10 +5,13 @@
 // and kv head; its keys come in tiles of 128 tokens (8 pages).  Per tile, on tcgen05 with
 // e4m3 operands straight from the cache's bytes (no conversion of the cache at all):
 //   S^T [128 tokens x N] = codeK [128 x D] . Qterms^T [D x N]
-//   O^T [D x N]         += codeV^T [D x 128] . Pterms [128 x N]
+//   O^T [D x NP]        += codeV^T [D x 128] . Pterms [128 x NP]
 // N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
 // scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
-// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  The tensor
+// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  Weights need
+// range as well: thousands of keys may lie many nats below one whose V is small.  So NP = 2 N: a
+// weight below 2^-12 of the reference enters 2^14 times larger in columns of its own, the others'
+// columns hold zero there (one group of columns lost all below 2^-19).  The tensor
 // time of a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
 // below the time of the tile's bytes from HBM, which is what bounds long caches: 64 requests of
 // 32768 tokens (2 kv heads of 256, 8 query heads each) take 346 us, 6.21 TB/s, 0.96 of the measured
@@ -19,7 +22,8 @@
 //   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
 // M the row's reference for x + v: raised to the running maximum whenever some x + v exceeds
 // it by more than 2 (then O^T and the sums are rescaled), so w <= 4 and 64 w stays in e4m3's
-// range whatever the scales are; two terms leave an error of at most 2^-8 w or 2^-20.  Thread t of
+// range whatever the scales are; two terms leave an error of at most 2^-8 w down to w = 2^-26, below
+// that 2^-34 (five: 2^-20 w, 2^-46).  Thread t of
 // a group of 128 owns token t of the tile for 8 of the rows: scores, weights, its share of the row
 // sums; only the reference crosses threads.
 //
@@ -43,6 +47,8 @@ constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its C
 constexpr int kKeyLead = 1;                  // an item's start and end in tiles (KeyWalk)
 constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
+constexpr float kKeySmall = 1.0f / 4096;     // those below it in the second group of columns,
+constexpr float kKeyGroup = 16384.0f;        // times 2^14
 
 template <typename T, int D, int RB, int CTAS>
 struct KeyShape {
@@ -52,18 +58,23 @@ struct KeyShape {
     static constexpr int kThreads = kSoft + 64;
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
+    static constexpr int kNP = 2 * RB * kTerms;              // column (2 i + group) RB + row: term i
+    // buffers of the scores and of the weights: two, so that no role waits; one where the fp32 terms'
+    // columns and bytes would cost the second CTA (16 rows) or the third slot of the ring (D = 256:
+    // 32 requests of 8000 keys 82 us with two buffers and two slots)
+    static constexpr int kBufs = sizeof(T) == 4 && (RB == 16 || D == 256) ? 1 : 2;
     static constexpr int kQ = kN * D;
-    static constexpr int kP = kN * kKeyTile;          // one of two buffers
-    static constexpr int kFixed = kQ + 2 * kP + 1024;
+    static constexpr int kP = kNP * kKeyTile;                // one buffer
+    static constexpr int kFixed = kQ + kBufs * kP + 1024;
     static constexpr int kCtas = CTAS;                       // per SM
     using Tile = KeyTile<D, true>;                    // K and V of a tile
     static constexpr int kSlot = Tile::kSlot;
     static constexpr int kFit = (kKeySmem / kCtas - 6144 - kFixed) / kSlot;  // static arrays and 1 KB per CTA beside it
     static constexpr int kSlots = kFit > kKeyMaxSlots ? kKeyMaxSlots : kFit;
     static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kSlot + kFixed;
-    static constexpr int kColsUsed = (2 + kChunks) * kN;
+    static constexpr int kColsUsed = kBufs * kN + kChunks * kNP;
     static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
-    static_assert(kSlots >= 2 && kN % 16 == 0 && kColsUsed <= 512, "shape");
+    static_assert(kSlots >= 2 && kN % 16 == 0 && kNP % 16 == 0 && kColsUsed * kCtas <= 512, "shape");
     static_assert(kQ % 1024 == 0 && kP % 1024 == 0, "tiles start at the swizzle's 1024 bytes");
 };
 
@@ -76,7 +87,8 @@ template <typename T, int D, int RB, int CTAS>
 __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T, D, RB, CTAS>::kCtas)
     kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB, CTAS>;
-    constexpr int N = S::kN, TERMS = S::kTerms, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
+    constexpr int N = S::kN, NP = S::kNP, TERMS = S::kTerms, BUFS = S::kBufs, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
+    constexpr uint32_t kO = BUFS * N;  // tensor memory columns: scores, O
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
     extern __shared__ __align__(1024) uint8_t key_smem[];
@@ -84,7 +96,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
     uint8_t* s_q = sm + SL * S::kSlot;
     uint8_t* s_p = s_q + S::kQ;
     __shared__ __align__(8) KeyRing<SL, true> ring;
-    __shared__ __align__(8) uint64_t s_full[2], p_ready[2], pv_done[2], q_ready, done_bar;
+    __shared__ __align__(8) uint64_t s_full[BUFS], s_free, p_ready[BUFS], pv_done[BUFS], q_ready, done_bar;
     __shared__ float s_frow[RB];
     __shared__ int s_lim[RB];
     // elements of out and of lse of the item's rows, by the item's parity: some threads still write
@@ -102,11 +114,12 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 
     if (tid == 0) {
         ring.init();
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < BUFS; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], SOFT);
             mbar_init(&pv_done[i], 1);
         }
+        mbar_init(&s_free, SOFT);
         mbar_init(&q_ready, SOFT);
         mbar_init(&done_bar, 1);
         mbar_fence_init();
@@ -119,6 +132,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
     const bool active = key_range<RB, kKeyLead, NT>(a, 1 + kKeyLead, s_sum, &s_range);
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    // tile x has buffer x % BUFS, in the phase of this parity
+    auto phase = [](uint32_t x) { return x / BUFS & 1u; };
 
     if (active && warp == W_LOAD) {
         key_produce<RB, kKeyLead, D, SL, true>(a, &ka.map, sm, ring, s_range, abort_flag);
@@ -127,11 +142,13 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
         if (lane == 0) {
             uint32_t t = 0, item = 0;
             bool ok = true;
-            const uint32_t i_s = f8_idesc(128, N, false, false), i_o = f8_idesc(128, N, true, true);
+            const uint32_t i_s = f8_idesc(128, N, false, false), i_o = f8_idesc(128, NP, true, true);
             const uint32_t sq = smem_u32(s_q), sp = smem_u32(s_p);
             auto scores = [&](uint32_t x) {  // S^T of tile x into its buffer
                 const uint32_t ld = ring.k_load(x);
-                if (!(ok = ring.wait_full(ld, a.err, abort_flag))) return;
+                ok = ring.wait_full(ld, a.err, abort_flag) &&
+                     (BUFS == 2 || x == 0 || mbar_wait_bounded(&s_free, (x - 1) & 1u, a.err, abort_flag));
+                if (!ok) return;
                 tc_fence_after();
                 const uint32_t k = smem_u32(sm + (ld % SL) * S::kSlot);
 #pragma unroll
@@ -139,9 +156,9 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     const uint64_t ad = f8_desc_k<CW>(k + c * S::Tile::kChunk, S::Tile::kGroup);
                     const uint64_t bd = f8_desc_k<CW>(sq + c * (N * CW), 8 * CW);
 #pragma unroll
-                    for (int j = 0; j < CW / 32; ++j) f8_mma(tmem + (x & 1u) * N, ad + 2 * j, bd + 2 * j, i_s, c > 0 || j > 0);
+                    for (int j = 0; j < CW / 32; ++j) f8_mma(tmem + x % BUFS * N, ad + 2 * j, bd + 2 * j, i_s, c > 0 || j > 0);
                 }
-                tc_commit(&s_full[x & 1u]);
+                tc_commit(&s_full[x % BUFS]);
             };
             KeyWalk<RB, kKeyLead> w(a, s_range);
             while (w.unit < w.end && ok) {
@@ -156,21 +173,21 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     for (int i = 0; i < nt && ok; ++i) {
                         const uint32_t x = t + i;
                         if (i + 1 < nt) scores(x + 1);
-                        if (!ok || !(ok = mbar_wait_bounded(&p_ready[x & 1u], (x >> 1) & 1u, a.err, abort_flag))) break;
+                        if (!ok || !(ok = mbar_wait_bounded(&p_ready[x % BUFS], phase(x), a.err, abort_flag))) break;
                         tc_fence_after();
                         const uint32_t ld = ring.v_load(x);
                         const uint32_t v = smem_u32(sm + (ld % SL) * S::kSlot) + S::Tile::kV;
-                        const uint64_t bd = f8_desc_n16(sp + (x & 1u) * S::kP, kKeyTile * 16);
+                        const uint64_t bd = f8_desc_n16(sp + x % BUFS * S::kP, kKeyTile * 16);
 #pragma unroll
                         for (int c = 0; c < S::kChunks; ++c) {
                             // 64 wide: M rows 64-127 repeat rows 0-63
                             const uint64_t ad = f8_desc_m<CW>(v + c * S::Tile::kChunk, 0, S::Tile::kGroup);
 #pragma unroll
                             for (int j = 0; j < kKeyTile / 32; ++j)
-                                f8_mma(tmem + (2 + c) * N, ad + j * (4 * S::Tile::kGroup / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
+                                f8_mma(tmem + kO + c * NP, ad + j * (4 * S::Tile::kGroup / 16), bd + j * (32 * 16 / 16), i_o, i > 0 || j > 0);
                         }
                         tc_commit(&ring.empty[ld % SL]);
-                        tc_commit(&pv_done[x & 1u]);
+                        tc_commit(&pv_done[x % BUFS]);
                     }
                     t += nt;
                 }
@@ -250,15 +267,15 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
             for (int i = 0; i < nt; ++i) {
                 const uint32_t x = t + i;
                 const int key = (t_begin + i) * kKeyTile + tt;
-                // the tile's scales, its scores, and (from the third tile on) the P buffer,
-                // tried together since they are mostly there
+                // the tile's scales, its scores, and (of two buffers, from the third tile on) the P
+                // buffer, tried together since they are mostly there
                 const bool t1 = ring.try_meta(x);
-                const bool t2 = mbar_try_wait(&s_full[x & 1u], (x >> 1) & 1u);
-                const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
+                const bool t2 = mbar_try_wait(&s_full[x % BUFS], phase(x));
+                const bool t3 = BUFS == 1 || i < 2 || mbar_try_wait(&pv_done[x % BUFS], phase(x - 2));
                 if (!(t1 && t2 && t3)) {
                     ok = ok && ring.wait_meta(x, a.err, abort_flag) &&
-                         mbar_wait_bounded(&s_full[x & 1u], (x >> 1) & 1u, a.err, abort_flag) &&
-                         (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
+                         mbar_wait_bounded(&s_full[x % BUFS], phase(x), a.err, abort_flag) &&
+                         (BUFS == 1 || i < 2 || mbar_wait_bounded(&pv_done[x % BUFS], phase(x - 2), a.err, abort_flag));
                 }
                 __syncwarp();  // the loads below are the whole warp's
                 tc_fence_after();
@@ -268,8 +285,12 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 {
                     float c[TERMS][8];
 #pragma unroll
-                    for (int b = 0; b < TERMS; ++b) tc_ld8(lanes + (x & 1u) * N + b * RB, c[b]);
+                    for (int b = 0; b < TERMS; ++b) tc_ld8(lanes + x % BUFS * N + b * RB, c[b]);
                     tc_wait_ld();
+                    if constexpr (BUFS == 1) {
+                        tc_fence_before();
+                        mbar_arrive(&s_free);
+                    }
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
                         y[r] = c[0][r];
@@ -295,7 +316,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     // raise the references to the maximum of this tile and rescale; after a failed
                     // wait all threads leave together here
                     if (ok && i > 0)
-                        ok = mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
+                        ok = mbar_wait_bounded(&pv_done[(x - 1) % BUFS], phase(x - 1), a.err, abort_flag);
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
                         const float mx = warp_max(y[r]);
@@ -316,13 +337,13 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll 1  // rare: little code
                         for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll(TERMS == 2 ? 2 : 1)
-                            for (int b = 0; b < TERMS; ++b) {
+                            for (int b = 0; b < 2 * TERMS; ++b) {
                                 float o[8];
-                                tc_ld8(lanes + (2 + c) * N + b * RB, o);
+                                tc_ld8(lanes + kO + c * NP + b * RB, o);
                                 tc_wait_ld();
 #pragma unroll
                                 for (int r = 0; r < 8; ++r) o[r] *= fac[r];
-                                tc_st8(lanes + (2 + c) * N + b * RB, o);
+                                tc_st8(lanes + kO + c * NP + b * RB, o);
                             }
                         tc_wait_st();
                     }
@@ -330,11 +351,13 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 }
                 // weights, row sums, e4m3 terms
                 const float vinv = __int_as_float((127 - static_cast<int>(vexp)) << 23);
+                uint32_t below[8];  // sign bit: in the second group
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const float wgt = ex2(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
                     l[r] = fmaf(wgt, vinv, l[r]);
-                    y[r] = wgt * kKeyBoost;
+                    below[r] = __float_as_uint(wgt - kKeySmall);
+                    y[r] = wgt * (wgt < kKeySmall ? kKeyBoost * kKeyGroup : kKeyBoost);
                 }
                 if (edge) {
                     // V rows behind the last key become zeros; a NaN code that not every row sees
@@ -369,19 +392,28 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                             if (key < s_lim[r0 + r]) l[r] = __int_as_float(0x7fc00000);
                     }
                 }
-                uint8_t* p = s_p + (x & 1u) * S::kP + tt * 16;
+                uint8_t* p = s_p + x % BUFS * S::kP + tt * 16;
                 uint32_t code[4][TERMS];
 #pragma unroll
                 for (int r = 0; r < 8; r += 2) e4m3_split2<TERMS>(y[r], y[r + 1], code[r / 2]);
+                const uint32_t m0 = sign_bytes(below[0], below[1], below[2], below[3]);
+                const uint32_t m1 = sign_bytes(below[4], below[5], below[6], below[7]);
+                if (BUFS == 1 && i > 0 && !mbar_try_wait(&pv_done[0], phase(x - 1)))
+                    ok = ok && mbar_wait_bounded(&pv_done[0], phase(x - 1), a.err, abort_flag);
 #pragma unroll
                 for (int b = 0; b < TERMS; ++b) {
-                    const int n = b * RB + r0;
-                    *reinterpret_cast<uint2*>(p + (n / 16) * (kKeyTile * 16) + n % 16) =
-                        make_uint2(code[0][b] | (code[1][b] << 16), code[2][b] | (code[3][b] << 16));
+                    const uint32_t c0 = code[0][b] | (code[1][b] << 16), c1 = code[2][b] | (code[3][b] << 16);
+                    uint8_t* at = p + 2 * b * RB / 16 * (kKeyTile * 16);
+                    if constexpr (RB == 8) {
+                        *reinterpret_cast<uint4*>(at) = make_uint4(c0 & ~m0, c1 & ~m1, c0 & m0, c1 & m1);
+                    } else {
+                        *reinterpret_cast<uint2*>(at + r0) = make_uint2(c0 & ~m0, c1 & ~m1);
+                        *reinterpret_cast<uint2*>(at + kKeyTile * 16 + r0) = make_uint2(c0 & m0, c1 & m1);
+                    }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
-                mbar_arrive(&p_ready[x & 1u]);
+                mbar_arrive(&p_ready[x % BUFS]);
             }
             if (left) break;
             t += nt;
@@ -391,7 +423,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 const float s = warp_sum(l[r]);
                 if (lane == 0) s_red[wq][r0 + r] = s;
             }
-            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) & 1u], ((t - 1) >> 1) & 1u, a.err, abort_flag);
+            ok = ok && mbar_wait_bounded(&pv_done[(t - 1) % BUFS], phase(t - 1), a.err, abort_flag);
             if (named_bar_or(1, SOFT, !ok)) break;
             tc_fence_after();
 #pragma unroll
@@ -416,16 +448,19 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
             for (int r = 0; r < 8; ++r) scale[r] = reciprocal(l[r]);
 #pragma unroll 1
             for (int c = 0; c < S::kChunks; ++c) {
-                float o[8], v[TERMS][8];
+                float o[8];
 #pragma unroll
-                for (int b = 0; b < TERMS; ++b) tc_ld8(lanes + (2 + c) * N + b * RB, v[b]);
-                tc_wait_ld();
+                for (int r = 0; r < 8; ++r) o[r] = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    o[r] = v[0][r] * (1.0f / kKeyBoost);
+                for (int b = 0; b < TERMS; ++b) {
+                    float v[2][8];
+                    tc_ld8(lanes + kO + c * NP + 2 * b * RB, v[0]);
+                    tc_ld8(lanes + kO + c * NP + (2 * b + 1) * RB, v[1]);
+                    tc_wait_ld();
 #pragma unroll
-                    for (int b = 1; b < TERMS; ++b)
-                        o[r] = fmaf(v[b][r], 1.0f / (static_cast<float>(1 << (4 * b)) * kKeyBoost), o[r]);
+                    for (int r = 0; r < 8; ++r)
+                        o[r] = fmaf(fmaf(v[1][r], 1.0f / kKeyGroup, v[0][r]),
+                                    1.0f / (static_cast<float>(1 << (4 * b)) * kKeyBoost), o[r]);
                 }
                 if (tt < CW) {
 #pragma unroll

@@ -108,6 +108,13 @@ DM_DEV void e4m3_split2(float a, float b, uint32_t (&t)[TERMS]) {
         t[4] = e4m3_take2(rest);
     }
 }
+// 0xff in byte i where value i has its sign bit set
+DM_DEV uint32_t sign_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    uint32_t lo, hi;
+    asm("prmt.b32 %0, %1, %2, 0xFB;" : "=r"(lo) : "r"(a), "r"(b));  // 8 + i: the sign of byte i
+    asm("prmt.b32 %0, %1, %2, 0xFB;" : "=r"(hi) : "r"(c), "r"(d));
+    return __byte_perm(lo, hi, 0x5410);
+}
 // 0xff in the bytes of w that hold a NaN code
 DM_DEV uint32_t e4m3_nan_mask(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 

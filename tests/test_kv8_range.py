@@ -1,0 +1,103 @@
+"""The 8-bit cache operators at the ends of what their contract allows: softmax weights far below
+the largest, page scales far apart, queries of extreme size, codes that are NaN, rows that no
+request covers, calls from several threads."""
+import math
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from disk_streaming_moe_engine_b200 import DmError, _lib, kv8
+from test_kv8 import BF16_STEP, DEV, E4M3, F32_STEP, PAGE, dev32, make_cache, make_table, plain_attention, plain_freq, plain_rope
+
+F16_STEP = 2.0 ** -11  # largest relative rounding of fp16
+
+
+def query_side(n, max_q, group, hk, dtype):
+    """The rule between the two attention kernels: True where 128 query rows go on the M side."""
+    rows = max_q * group
+    items = -(-rows // 128) * n * hk
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return dtype == torch.bfloat16 and rows >= (40 if 2 * items >= sms else 96 if items >= 8 else 192)
+
+
+def tolerance(cache, q, scale, ref, keys, on_query_side):
+    """Per output.  A score's error e changes an output by at most 2 e sum p |v|.  e: products and
+    sums in fp32 (D / 16 + 1 chained sums, 2^-22 of the magnitudes each), and q as e4m3 terms: bf16
+    on the query side off by 2^-17 of the row's largest element, on the key side by 2^-21 of it;
+    fp32 by 2^-20 of the element or 2^-26 of 2^8, the largest being at least 2^7.  Weights, sums in
+    fp32: on the query side fp16 values 2^13 w, off by 2^-11 of themselves or 2^-38 (half of 2^-24 /
+    2^13).  On the key side e4m3 terms of 64 w, or of 2^20 w for w < 2^-12, each term off by 2^-4 of
+    itself and the next one holding 16 times that: two terms 2^-8 (and 2^-11 on the way through
+    fp16) or 2^-34 (half of 2^-9 / 16 / 2^20), five 2^-20 or 2^-46.  What is absolute is relative to
+    a reference that the row's largest p sV is never below; times 4 for two groups of terms and
+    the rounding on the way.  bf16 results are rounded once."""
+    out, (mag, small), sat, _ = ref
+    d, bf16 = q.shape[-1], q.dtype == torch.bfloat16
+    k = torch.from_numpy(E4M3).to(DEV)[cache.pages[:, 0].long()].nan_to_num() * cache.scales[:, 0, :, None, None].double()
+    size = (q.double().abs().amax(-1) * k.abs().sum(-1).max() * abs(scale)).cpu().numpy()
+    e = sat * (d / 16 + 1) * 2.0 ** -22 + size * ((2.0 ** -17 if on_query_side else 2.0 ** -21) if bf16 else 2.0 ** -25)
+    if not bf16:
+        e = e + sat * 2.0 ** -20
+    rel, low = (F16_STEP, 2.0 ** -36) if on_query_side else (2.0 ** -8 + F16_STEP, 2.0 ** -32) if bf16 else (2.0 ** -20, 2.0 ** -44)
+    tol = (2 * e[..., None] + (keys / PAGE + 4) * 2.0 ** -22 + rel) * mag + low * small
+    return tol + (BF16_STEP * np.abs(out) if bf16 else 0) + 1e-30, e
+
+
+def check_against_64_bits(cache, q, table, lens, rows, scale, max_q=None):
+    """attention() over all rows against the plain form; (results, lse, reference)."""
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    max_q = max_q or max(rows)
+    err = kv8.error_word()
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    got = kv8.attention(cache, q, dev32(table), dev32(lens), dev32(cu), max_q, sm_scale=scale, lse=lse,
+                        workspace=kv8.attention_workspace(cache), err=err)
+    kv8.check(err)
+    ref = plain_attention(cache, q, table, lens, cu, scale)
+    side = query_side(len(lens), max_q, q.shape[1] // cache.num_kv_heads, cache.num_kv_heads, q.dtype)
+    tol, e = tolerance(cache, q, scale, ref, max(lens), side)
+    diff = np.abs(got.double().cpu().numpy() - ref[0])
+    assert (diff <= tol).all(), (np.nanmax(diff / tol), np.isnan(diff).any())
+    want = ref[3]
+    at = np.isfinite(want)
+    sums = lse.double().cpu().numpy()
+    assert (np.isneginf(sums) == ~at).all()
+    assert (np.abs(sums - want)[at] <= (e + np.abs(want) * 2.0 ** -22 + 2.0 ** -18)[at]).all()
+    return got, lse, ref
+
+
+# ---- softmax weights far below the largest ------------------------------------------------------------
+
+def peaked(d, hk, grp, keys, rows, nats, at, seed):
+    """One key whose score is `nats` above the others' mean (their spread about 1/2), with V = 0
+    there: the result is the other keys' alone, whose weights are e^-nats and less."""
+    g = torch.Generator().manual_seed(seed)
+    cache = make_cache(-(-keys // PAGE) + 2, hk, d, seed)
+    u = torch.randint(0, 2, (d,), generator=g) * 2.0 - 1
+    c = nats / (2 * math.sqrt(d))
+    tail = (torch.randn(cache.num_pages, hk, PAGE, d, generator=g) * (math.sqrt(d) / nats)).to(torch.float8_e4m3fn)
+    cache.pages[:, 0] = tail.view(torch.uint8).to(DEV)
+    cache.scales[:, 0] = 1.0
+    cache.scales[:, 1] = 2.0 ** -7
+    table = make_table([keys], cache.num_pages, seed)
+    page, off = int(table[0, at // PAGE]), at % PAGE
+    cache.pages[page, 0, :, off] = (2 * u).to(torch.float8_e4m3fn).view(torch.uint8).to(DEV)
+    cache.pages[page, 1, :, off] = 0
+    q = u * c * (1 + 0.05 * torch.rand(rows, hk * grp, 1, generator=g)) + 0.01 * torch.randn(rows, hk * grp, d, generator=g)
+    return cache, table, q
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,grp", [(1, 8), (1, 11)])
+@pytest.mark.parametrize("keys,nats,at", [(8192, 11, 0), (8192, 14, 4000), (32768, 12, 5), (8192, 19, 8100), (130, 14, 64)])
+def test_small_weights_count(lib, dtype, d, rows, grp, keys, nats, at):
+    """The key side: thousands of keys
+    11 to 19 nats below one that adds nothing, or a few in its own tile."""
+    cache, table, q = peaked(d, 1, grp, keys, rows, nats, at, seed=keys + nats)
+    q = q.to(DEV, dtype)
+    assert query_side(1, rows, grp, 1, dtype) == (rows == 48 and dtype == torch.bfloat16)
+    got, _, ref = check_against_64_bits(cache, q, table, [keys], [rows], d ** -0.5)
+    assert np.abs(ref[0]).max() > 0 and (got != 0).any()
