@@ -4,15 +4,20 @@
 // Work: an item is 128 query rows (a row = one query token and one query head; the heads of a
 // group share their keys, so a group's rows go together) of one request and kv head; its keys
 // come in tiles of 128 tokens.  Per tile, on tcgen05 with e4m3 operands straight from the cache:
-//   S [128 x 128] = (Q0 + Q1) [128 x D] . codeK^T,   O [128 x D] += (P0 + P1) [128 x 128] . codeV
-// q and the weights are sums of two e4m3 terms of one scale, so both products of a pair add into
-// one accumulator at the cost of one bf16 product (e4m3 runs at twice its rate), and the cache
-// needs no conversion.  bf16's 8 bits fit two terms: q, scaled to a largest magnitude in
-// [2^7, 2^8) per row, is exact down to 2^-10 of it and off by 2^-18 of it at most; a weight is
-// off by 2^-8 of itself or 2^-16 of the row's largest.
+//   S [128 x 128] = (Q0 + Q1) [128 x D] . codeK^T,   O [128 x D] += (P0 + P1 + P2) [128 x 128] . codeV
+// q and the weights are sums of 8-bit terms of one scale, so all products of a sum add into one
+// accumulator at half the cost of a bf16 product each, and the cache needs no conversion.  bf16's 8
+// bits fit two e4m3 terms: q, scaled to a largest magnitude in [2^7, 2^8) per row, is exact down to
+// 2^-10 of it and off by 2^-17 of it at most.  The weights need range as well, for thousands of keys
+// may lie many nats below one whose V is small: three e5m2 terms of 2^11 w (A and B need not be of
+// one 8-bit type) are off by 2^-9 w down to w = 2^-19 of the reference, by 2^-28 of it below.  Two
+// e4m3 terms of 2^6 w lost all below 2^-16.  fp16 weights were slower, for V's codes have to become
+// fp16 too and that copy takes as much of shared memory's bandwidth as the products' operands: one
+// prompt of 8192 (16 query heads on 2, D = 64 / 128 / 256) 416 / 479 / 598 us with V converted by the
+// softmax warps, 368 / 473 / 681 by four more, 376 / 394 / 529 this way.
 //
 // Softmax as in the key-side kernel: y = x + v - M in log2 units with the page's sV = 2^v folded
-// in, M raised when some y exceeds 2, o = sum w codeV / sum w 2^-v.  A row belongs to two
+// in, M raised when some y exceeds 4, o = sum w codeV / sum w 2^-v.  A row belongs to two
 // threads, 64 keys of the tile each, that meet at a 64-thread barrier to agree on M; O is
 // rescaled only by warps with a raised row.
 //
@@ -25,7 +30,8 @@
 // warps turn the next item's q rows into terms while the last O product runs, then write the
 // item's O while the next scores run (two separate warps for the terms were slower: the
 // conversions are ALU work that all four schedulers have to share).  Tensor memory: the scores
-// (128 columns), two buffers of weights (64), O (D).  Split of the work, joins and bounded waits
+// (128 columns), two buffers of weights (96 each; at D = 256 one, written once the O product before
+// is done, which it mostly is by then), O (D).  Split of the work, joins and bounded waits
 // as in the key-side kernel; after a failed wait every thread runs through the remaining barriers
 // without work.
 //
@@ -48,8 +54,12 @@ constexpr int kQryThreads = kQrySoft + 128;
 // an item's start and end in tiles (KeyWalk): q rows to terms and the first scores before, O after,
 // which cost this kernel as much as 6 tiles do; ranges cut by tiles alone end up to that much apart
 constexpr int kQryLead = 6;
-constexpr float kQryLazy = 2.0f;
-constexpr float kQryBoost = 6.0f;  // weights enter as 2^6 w <= 256
+// log2 units a weight may exceed the reference by: a raise makes the row wait for the O product before
+// and holds up the tile (2: 426 / 432 / 577 us for the three prompts above, 3: 380 / 401 / 534, 4: 376 /
+// 394 / 529, 5 the same)
+constexpr float kQryLazy = 4.0f;
+constexpr float kQryBoost = 11.0f;  // weights enter as 2^11 w <= 2^15
+constexpr int kQryTerms = 3;        // e5m2 terms of a weight, 32 columns of tensor memory each
 
 template <int D>
 struct QryShape {
@@ -74,7 +84,9 @@ template <int D>
 __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const __grid_constant__ QryArgs qa) {
     using S = QryShape<D>;
     constexpr int CW = S::CW, SL = S::kSlots, RB = kQryRows;
-    constexpr uint32_t kPw = 128, kO = 256;  // tensor memory columns: scores, weights (two buffers of 64), O
+    // tensor memory columns: scores, weights (two buffers, at D = 256 room for one), O
+    constexpr uint32_t PB = D == 256 ? 1 : 2, kPCols = 32 * kQryTerms, kPw = 128, kO = D == 256 ? 256 : kPw + PB * kPCols;
+    static_assert(kPw + PB * kPCols <= kO && kO + D <= 512, "tensor memory");
     const Kv8AttnArgs& a = qa.a;
     extern __shared__ __align__(1024) uint8_t qry_smem[];
     uint8_t* sm = qry_smem + ((1024u - (smem_u32(qry_smem) & 1023u)) & 1023u);
@@ -155,7 +167,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
         // ---------------- O products ----------------
         if (lane == 0) {
             bool ok = true;
-            const uint32_t i_o = f8_idesc(128, D, false, true);
+            const uint32_t i_o = f8_idesc(128, D, false, true) | (1u << 7);  // A e5m2
             KeyWalk<RB, kQryLead> w(a, s_range);
             uint32_t x = 0;
             while (w.unit < w.end && ok) {
@@ -168,9 +180,9 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = f8_desc_m<CW>(smem_u32(sm + (ld % SL) * S::kTileBytes), S::Tile::kChunk, S::Tile::kGroup);
-                    const uint32_t p = tmem + kPw + (x & 1u) * 64;
+                    const uint32_t p = tmem + kPw + x % PB * kPCols;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < kQryTerms; ++t)
 #pragma unroll
                         for (int j = 0; j < kKeyTile / 32; ++j)
                             f8_mma_ts(tmem + kO, p + t * 32 + j * 8, vd + j * (4 * S::Tile::kGroup / 16), i_o, i > begin || t > 0 || j > 0);
@@ -381,15 +393,15 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             bool nan_row = false;
 
             for (int i = 0; i < nt; ++i) {
-                const uint32_t x = t + i, pb = kPw + (x & 1u) * 64 + half * 16;
+                const uint32_t x = t + i, pb = kPw + x % PB * kPCols + half * 16;
                 const int tile0 = (t_begin + i) * kKeyTile;
                 const bool t1 = ring.try_meta(x);
                 const bool t2 = mbar_try_wait(&s_full, x & 1u);
-                const bool t3 = i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
+                const bool t3 = PB == 1 || i < 2 || mbar_try_wait(&pv_done[x & 1u], ((x - 2) >> 1) & 1u);
                 if (ok && !(t1 && t2 && t3))
                     ok = ring.wait_meta(x, a.err, abort_flag) &&
                          mbar_wait_bounded(&s_full, x & 1u, a.err, abort_flag) &&
-                         (i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
+                         (PB == 1 || i < 2 || mbar_wait_bounded(&pv_done[x & 1u], ((x - 2) >> 1) & 1u, a.err, abort_flag));
                 __syncwarp();
                 tc_fence_after();
                 float s[64];
@@ -461,28 +473,40 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                         tc_wait_st();
                     }
                 }
-                // weights, sums, terms: columns of P0 and P1 of this half's 64 keys
+                // weights, sums, terms: this half's 64 keys, columns of P0, P1 and P2
+                // (of one buffer: stored together once the O product of the tile before has read its own)
+                uint32_t pt[kQryTerms][PB == 1 ? 16 : 4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    uint32_t p0[4], p1[4];
 #pragma unroll
                     for (int c = 0; c < 16; c += 4) {
                         float* y = s + p * 16 + c;
-                        uint32_t a0, a1, b0, b1;
+                        uint32_t four[kQryTerms];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             y[j] = ex2(y[j]);
                             sum[j] += y[j];
                         }
-                        e4m3_terms2(y[0], y[1], a0, a1);
-                        e4m3_terms2(y[2], y[3], b0, b1);
-                        p0[c / 4] = a0 | (b0 << 16);
-                        p1[c / 4] = a1 | (b1 << 16);
+                        e5m2_terms3(y[0], y[1], y[2], y[3], four);
+#pragma unroll
+                        for (int t = 0; t < kQryTerms; ++t) pt[t][(PB == 1 ? p * 4 : 0) + c / 4] = four[t];
                     }
                     l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), vinv[p], l);
-                    tc_st4(lanes + pb + p * 4, p0);
-                    tc_st4(lanes + pb + 32 + p * 4, p1);
+                    if constexpr (PB == 2) {
+#pragma unroll
+                        for (int t = 0; t < kQryTerms; ++t) tc_st4(lanes + pb + t * 32 + p * 4, pt[t]);
+                    }
+                }
+                if constexpr (PB == 1) {
+                    if (i > 0) {
+                        if (ok && !mbar_try_wait(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u))
+                            ok = mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);
+                        __syncwarp();
+                        tc_fence_after();
+                    }
+#pragma unroll
+                    for (int t = 0; t < kQryTerms; ++t) tc_st16(lanes + pb + t * 32, pt[t]);
                 }
                 if (edge) {
                     // V rows behind the last key become zeros; a NaN code that not every row sees

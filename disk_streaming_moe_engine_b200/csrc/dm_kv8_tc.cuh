@@ -127,6 +127,27 @@ DM_DEV void e4m3_terms2(float a, float b, uint32_t& t0, uint32_t& t1) {
     t1 = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(__hsub2(h, back)), __NV_SATFINITE, __NV_E4M3);
 }
 
+// Three e5m2 terms of four values in [0, 2^15], all of one scale, a byte each.  An e5m2 code is the
+// upper byte of an fp16 value: three of its bits at a time stay with their exponent, what they leave
+// is exact, and the last term is rounded (conversion instructions took 40 % longer).
+DM_DEV void e5m2_terms3(float a, float b, float c, float d, uint32_t (&t)[3]) {
+    uint32_t x[2], top[2];
+    const __half2 h0 = __floats2half2_rn(a, b), h1 = __floats2half2_rn(c, d);
+    x[0] = *reinterpret_cast<const uint32_t*>(&h0);
+    x[1] = *reinterpret_cast<const uint32_t*>(&h1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            top[j] = x[j] & 0xff00ff00u;
+            const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&x[j]), *reinterpret_cast<const __half2*>(&top[j]));
+            x[j] = *reinterpret_cast<const uint32_t*>(&rest);
+        }
+        t[i] = __byte_perm(top[0], top[1], 0x7531);
+    }
+    t[2] = __byte_perm(x[0] + 0x00800080u, x[1] + 0x00800080u, 0x7531);
+}
+
 // 32 bytes of one thread (32-byte aligned): whole sectors where every lane has a row of its own
 DM_DEV void ldg_v8(uint32_t* v, const void* p) {
     asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"

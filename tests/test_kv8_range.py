@@ -27,12 +27,12 @@ def tolerance(cache, q, scale, ref, keys, on_query_side):
     sums in fp32 (D / 16 + 1 chained sums, 2^-22 of the magnitudes each), and q as e4m3 terms: bf16
     on the query side off by 2^-17 of the row's largest element, on the key side by 2^-21 of it;
     fp32 by 2^-20 of the element or 2^-26 of 2^8, the largest being at least 2^7.  Weights, sums in
-    fp32: on the query side fp16 values 2^13 w, off by 2^-11 of themselves or 2^-38 (half of 2^-24 /
-    2^13).  On the key side e4m3 terms of 64 w, or of 2^20 w for w < 2^-12, each term off by 2^-4 of
+    fp32: on the query side three e5m2 terms of 2^11 w, each holding the next 3 bits: off by 2^-9 of
+    themselves (and 2^-11 on the way through fp16) or 2^-28 (half of 2^-16 / 2^11).  On the key side e4m3 terms of 64 w, or of 2^20 w for w < 2^-12, each term off by 2^-4 of
     itself and the next one holding 16 times that: two terms 2^-8 (and 2^-11 on the way through
     fp16) or 2^-34 (half of 2^-9 / 16 / 2^20), five 2^-20 or 2^-46.  What is absolute is relative to
-    a reference that the row's largest p sV is never below; times 4 for two groups of terms and
-    the rounding on the way.  bf16 results are rounded once."""
+    a reference that the row's largest p sV is never below; doubled or
+    more for the rounding on the way.  bf16 results are rounded once."""
     out, (mag, small), sat, _ = ref
     d, bf16 = q.shape[-1], q.dtype == torch.bfloat16
     k = torch.from_numpy(E4M3).to(DEV)[cache.pages[:, 0].long()].nan_to_num() * cache.scales[:, 0, :, None, None].double()
@@ -40,7 +40,7 @@ def tolerance(cache, q, scale, ref, keys, on_query_side):
     e = sat * (d / 16 + 1) * 2.0 ** -22 + size * ((2.0 ** -17 if on_query_side else 2.0 ** -21) if bf16 else 2.0 ** -25)
     if not bf16:
         e = e + sat * 2.0 ** -20
-    rel, low = (F16_STEP, 2.0 ** -36) if on_query_side else (2.0 ** -8 + F16_STEP, 2.0 ** -32) if bf16 else (2.0 ** -20, 2.0 ** -44)
+    rel, low = (2.0 ** -9 + F16_STEP, 2.0 ** -27) if on_query_side else (2.0 ** -8 + F16_STEP, 2.0 ** -32) if bf16 else (2.0 ** -20, 2.0 ** -44)
     tol = (2 * e[..., None] + (keys / PAGE + 4) * 2.0 ** -22 + rel) * mag + low * small
     return tol + (BF16_STEP * np.abs(out) if bf16 else 0) + 1e-30, e
 
@@ -91,10 +91,10 @@ def peaked(d, hk, grp, keys, rows, nats, at, seed):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("rows,grp", [(1, 8), (1, 11)])
+@pytest.mark.parametrize("rows,grp", [(1, 8), (1, 11), (48, 4)])
 @pytest.mark.parametrize("keys,nats,at", [(8192, 11, 0), (8192, 14, 4000), (32768, 12, 5), (8192, 19, 8100), (130, 14, 64)])
 def test_small_weights_count(lib, dtype, d, rows, grp, keys, nats, at):
-    """The key side: thousands of keys
+    """The key side (one token) and the query side (48 tokens of 4 heads, bf16): thousands of keys
     11 to 19 nats below one that adds nothing, or a few in its own tile."""
     cache, table, q = peaked(d, 1, grp, keys, rows, nats, at, seed=keys + nats)
     q = q.to(DEV, dtype)
