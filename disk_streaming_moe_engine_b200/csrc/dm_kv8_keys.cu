@@ -21,7 +21,10 @@
 // Softmax in base 2: with a page's scales sK, sV = 2^v,
 //   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
 // M the row's reference for x + v: raised to the running maximum whenever some x + v exceeds
-// it by more than 2 (then O^T and the sums are rescaled), so w <= 4 and 64 w stays in e4m3's
+// it by more than 2 (then O^T and the sums are rescaled).  Scores and references are kept in halves of
+// log2 units: e = 2^((x + v - M) / 2) does not underflow where w = e e does, and a key whose w is far
+// below 2^-126 may well have its share (e 2^-v) e of the sum, as pages of zeros do (their scale is
+// 2^-100).  So w <= 4 and 64 w stays in e4m3's
 // range whatever the scales are; two terms leave an error of at most 2^-8 w down to w = 2^-26, below
 // that 2^-34 (five: 2^-20 w, 2^-46).  Thread t of
 // a group of 128 owns token t of the tile for 8 of the rows: scores, weights, its share of the row
@@ -45,9 +48,9 @@ namespace dm {
 
 constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its CTAs
 constexpr int kKeyLead = 1;                  // an item's start and end in tiles (KeyWalk)
-constexpr float kKeyLazy = 2.0f;             // log2 units a weight may exceed the reference by
+constexpr float kKeyLazy = 1.0f;             // what a half log2 weight may exceed its reference by
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
-constexpr float kKeySmall = 1.0f / 4096;     // those below it in the second group of columns,
+constexpr float kKeySmall = 1.0f / 64;       // e of those in the second group of columns, below 2^-12 and
 constexpr float kKeyGroup = 16384.0f;        // times 2^14
 
 template <typename T, int D, int RB, int CTAS>
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
                 const float mul = __int_as_float((127 - ex) << 23);
                 if (tid % 16 == 0) {
-                    s_frow[r] = a.scale_log2 * __int_as_float((127 + ex) << 23);
+                    s_frow[r] = 0.5f * a.scale_log2 * __int_as_float((127 + ex) << 23);
                     s_lim[r] = r < nrow ? min(w.r.len, max(0, w.r.full - w.r.m + tok + 1)) : 0;
                     s_off[item & 1][r] = static_cast<int64_t>(w.r.row0 + tok) * a.o_rs + static_cast<int64_t>(head) * a.o_hs;
                     s_lse[item & 1][r] = static_cast<int64_t>(w.r.row0 + tok) * a.Hq + head;
@@ -296,7 +299,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                         y[r] = c[0][r];
 #pragma unroll
                         for (int b = 1; b < TERMS; ++b) y[r] = fmaf(c[b][r], 1.0f / static_cast<float>(1 << (4 * b)), y[r]);
-                        y[r] = fmaf(y[r], frow[r] * sc.x, vexp);
+                        y[r] = fmaf(y[r], frow[r] * sc.x, 0.5f * vexp);
                     }
                 }
                 const bool edge = (t_begin + i + 1) * kKeyTile > lim_min;
@@ -328,9 +331,10 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     for (int r = 0; r < 8; ++r) {
                         const float mx = fmaxf(fmaxf(s_red[0][r0 + r], s_red[1][r0 + r]), fmaxf(s_red[2][r0 + r], s_red[3][r0 + r]));
                         const float nm = fmaxf(mref[r], mx);
-                        fac[r] = nm == mref[r] ? 1.0f : exp2f(mref[r] - nm);
+                        const float f = nm == mref[r] ? 1.0f : exp2f(mref[r] - nm);
                         mref[r] = nm;
-                        l[r] *= fac[r];
+                        l[r] = l[r] * f * f;
+                        fac[r] = f * f;
                     }
                     if (i > 0) {
                         tc_fence_after();
@@ -354,10 +358,10 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                 uint32_t below[8];  // sign bit: in the second group
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    const float wgt = ex2(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
-                    l[r] = fmaf(wgt, vinv, l[r]);
-                    below[r] = __float_as_uint(wgt - kKeySmall);
-                    y[r] = wgt * (wgt < kKeySmall ? kKeyBoost * kKeyGroup : kKeyBoost);
+                    const float e = ex2(y[r] - (mref[r] == -INFINITY ? 0.0f : mref[r]));
+                    l[r] = fmaf(e * vinv, e, l[r]);
+                    below[r] = __float_as_uint(e - kKeySmall);
+                    y[r] = e * (e < kKeySmall ? kKeyBoost * kKeyGroup : kKeyBoost) * e;
                 }
                 if (edge) {
                     // V rows behind the last key become zeros; a NaN code that not every row sees
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
             auto put = [&](int r, int d, float o, float mm, float ll) {
                 if (r >= nrow) return;
                 static_cast<T*>(a.out)[s_off[item & 1][r] + d] = static_cast<T>(mm == -INFINITY && ll == 0.0f ? 0.0f : o);
-                if (d == 0 && a.lse) a.lse[s_lse[item & 1][r]] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+                if (d == 0 && a.lse) a.lse[s_lse[item & 1][r]] = ll == 0.0f ? -INFINITY : (2.0f * mm + log2f(ll)) * 0.6931471805599453f;
             };
             // Runs once per item, mostly from a cold instruction cache: one reciprocal per row (to 2
             // units of fp32 for bf16 results) and one chunk's code.
@@ -510,8 +514,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                             const float* p = part_of(c_first + c0 + c) + RB * D;
                             const float mc = __ldcg(p + r);
                             const float f = mc == mm ? 1.0f : exp2f(mc - mm);
-                            s_fac[c][r] = f;
-                            ll = fmaf(__ldcg(p + RB + r), f, ll);
+                            s_fac[c][r] = f * f;
+                            ll = fmaf(__ldcg(p + RB + r) * f, f, ll);
                         }
                         named_bar_sync(1, SOFT);
 #pragma unroll 8

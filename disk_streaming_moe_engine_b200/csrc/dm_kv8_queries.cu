@@ -58,6 +58,8 @@ constexpr int kQryLead = 6;
 // and holds up the tile (2: 426 / 432 / 577 us for the three prompts above, 3: 380 / 401 / 534, 4: 376 /
 // 394 / 529, 5 the same)
 constexpr float kQryLazy = 4.0f;
+// log2 of what enters as a page's largest weight: below kQryTiny it is put to kQryZero, still a zero as fp16
+constexpr float kQryTiny = -60.0f, kQryZero = -26.0f;
 constexpr float kQryBoost = 11.0f;  // weights enter as 2^11 w <= 2^15
 constexpr int kQryTerms = 3;        // e5m2 terms of a weight, 32 columns of tensor memory each
 
@@ -308,8 +310,8 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                         for (int c = c_first; c <= c_last; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + RB * D + row));
                         for (int c = c_first; c <= c_last; ++c) {
                             const float* p = part_of(c) + RB * D + row;
-                            const float mc = __ldcg(p);
-                            ll = fmaf(__ldcg(p + RB), mc == mm ? 1.0f : exp2f(mc - mm), ll);
+                            const float mc = __ldcg(p), f = mc == mm ? 1.0f : exp2f(0.5f * (mc - mm));
+                            ll = fmaf(__ldcg(p + RB) * f, f, ll);
                         }
                         const float linv = 1.0f / ll;
 #pragma unroll 1
@@ -432,29 +434,52 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     for (int c = 0; c < 64; ++c)
                         if (c >= seen || g[c / 16] == -INFINITY) s[c] = -INFINITY;
                 }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of each page
 #pragma unroll
-                for (int c = 0; c < 64; c += 8)
+                for (int c = 0; c < 16; c += 2)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) m4[j] = fmaxf(m4[j], fmaxf(s[c + j], s[c + 4 + j]));
+                    for (int p = 0; p < 4; ++p) m4[p] = fmaxf(m4[p], fmaxf(s[p * 16 + c], s[p * 16 + c + 1]));
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                bool low = fminf(fminf(m4[0], m4[1]), fminf(m4[2], m4[3])) < kQryTiny;
+                if (edge || gone) {  // pages without a visible key are not meant
+                    low = false;
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) low = low || (m4[p] < kQryTiny && m4[p] > -INFINITY);
+                }
                 const bool over = mref == -INFINITY ? mx > -INFINITY : mx > kQryBoost + kQryLazy;
-                if (named_bar_or(2 + wq, 64, over)) {
+                if (named_bar_or(2 + wq, 64, over || low)) {
                     // the row's two threads agree on its reference; O of the raised rows follows
                     s_max[half][row] = mx;
                     named_bar_sync(2 + wq, 64);
                     const float both = fmaxf(s_max[0][row], s_max[1][row]);  // in units of the old reference
                     named_bar_sync(2 + wq, 64);
                     const bool raise = mref == -INFINITY ? both > -INFINITY : both > kQryBoost + kQryLazy;
-                    float fac = 1.0f;
+                    float fac = 1.0f, shift = 0.0f;
                     if (raise) {
                         const float nm = mref == -INFINITY ? both : both - kQryBoost + mref;
-                        const float shift = mref == -INFINITY ? kQryBoost - nm : mref - nm;
-                        fac = mref == -INFINITY ? 0.0f : exp2f(shift);
+                        shift = mref == -INFINITY ? kQryBoost - nm : mref - nm;
+                        // in two factors, for the sum holds 2^-v: it may have to go down by more than one reaches
+                        const float f = mref == -INFINITY ? 0.0f : exp2f(0.5f * shift);
                         mref = nm;
-                        l *= fac;
+                        l = l * f * f;
+                        fac = f * f;
+                    }
+                    if (raise || low) {
+                        // A page whose weights are all near or below ex2's last step may still have its share of
+                        // the sum, where V's scales are far apart, as pages of zeros do (their scale is 2^-100).
+                        // Its scores go up, to where the weights' terms are still zero, and its 2^-v goes down
 #pragma unroll
-                        for (int c = 0; c < 64; ++c) s[c] += shift;
+                        for (int p = 0; p < 4; ++p) {
+                            const float m = m4[p] + shift;
+                            float up = shift;
+                            if (m < kQryTiny && m > -INFINITY) {
+                                const float d = fminf(floorf(kQryZero - m), 226.0f);
+                                up += d;
+                                vinv[p] = __int_as_float(max(0, (__float_as_int(vinv[p]) >> 23) - static_cast<int>(d)) << 23);
+                            }
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) s[p * 16 + c] += up;
+                        }
                     }
                     if (__any_sync(0xffffffffu, raise) && i > 0) {
                         ok = ok && mbar_wait_bounded(&pv_done[(x - 1) & 1u], ((x - 1) >> 1) & 1u, a.err, abort_flag);

@@ -101,3 +101,29 @@ def test_small_weights_count(lib, dtype, d, rows, grp, keys, nats, at):
     assert query_side(1, rows, grp, 1, dtype) == (rows == 48 and dtype == torch.bfloat16)
     got, _, ref = check_against_64_bits(cache, q, table, [keys], [rows], d ** -0.5)
     assert np.abs(ref[0]).max() > 0 and (got != 0).any()
+
+
+# ---- V page scales far apart ------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,grp", [(1, 2), (48, 4)])
+@pytest.mark.parametrize("high,low,how", [(27, -100, "alternate"), (100, -100, "alternate"), (100, -100, "low first"),
+                                          (100, -100, "high first"), (0, -100, "low first"), (60, -60, "alternate"),
+                                          (-95, -100, "alternate")])
+def test_v_scales_far_apart(lib, dtype, rows, grp, high, low, how):
+    """A key's share of the softmax does not depend on its V: pages of all-zero V (scale 2^-100)
+    beside pages of huge V, in one tile and in different ones, in one CTA and in several."""
+    d, keys = 64, 3000
+    cache = make_cache(-(-keys // PAGE) + 1, 1, d, seed=3, lo=-8, hi=-8)
+    table = make_table([keys], cache.num_pages, 3)
+    n = table.shape[1]
+    is_low = {"alternate": np.arange(n) % 2 == 1, "low first": np.arange(n) < n // 2,
+              "high first": np.arange(n) >= n // 2}[how]
+    for page, lo in zip(table[0], is_low):
+        cache.scales[page, 1] = 2.0 ** (low if lo else high)
+        if lo and low == -100:
+            cache.pages[page, 1] = 0
+    q = torch.randn(rows, grp, d, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
+    check_against_64_bits(cache, q, table, [keys], [rows], d ** -0.5)
+    check_against_64_bits(cache, q, table[:, :8], [100], [rows], d ** -0.5)
