@@ -688,8 +688,15 @@ extern "C" int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t
     if (seq_lens == ctx_lens && free_state_out != free_state) grid = 1;
     const size_t smem = 3 * static_cast<size_t>(n + 1) * sizeof(unsigned);
     cudaError_t e = cudaSuccess;
-    if (smem > 40 * 1024)
-        e = cudaFuncSetAttribute(kv8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (smem > 40 * 1024) {
+        // once per device and for the largest plan: the limit is the function's, calls on other threads share it
+        static std::atomic<bool> ready[64];
+        if (g.dev >= 64 || !ready[g.dev].load(std::memory_order_relaxed)) {
+            e = cudaFuncSetAttribute(kv8_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     3 * (DM_KV8_MAX_REQUESTS + 1) * static_cast<int>(sizeof(unsigned)));
+            if (e == cudaSuccess && g.dev < 64) ready[g.dev].store(true, std::memory_order_relaxed);
+        }
+    }
     if (e == cudaSuccess) {
         kv8_plan_kernel<<<grid, block, smem, static_cast<cudaStream_t>(stream)>>>(a);
         e = cudaGetLastError();

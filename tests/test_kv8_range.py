@@ -127,3 +127,36 @@ def test_v_scales_far_apart(lib, dtype, rows, grp, high, low, how):
     q = torch.randn(rows, grp, d, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
     check_against_64_bits(cache, q, table, [keys], [rows], d ** -0.5)
     check_against_64_bits(cache, q, table[:, :8], [100], [rows], d ** -0.5)
+
+
+# ---- calls from several threads --------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_plans_of_different_sizes_from_several_threads(lib):
+    """The plan of many requests needs more shared memory than that of fewer: a call on another
+    thread does not take it away between the setting and the launch."""
+    import ctypes as C
+    failed = []
+
+    def work(n, stream):
+        ctx, new = dev32([0] * n), dev32([1] * n)
+        table = torch.zeros((n, 1), dtype=torch.int32, device=DEV)
+        free, state = kv8.free_list(n)
+        left, tok = dev32([0, 0]), torch.zeros((4, n + 1), dtype=torch.int32, device=DEV)
+        lens, buf = torch.zeros_like(ctx), C.create_string_buffer(512)
+        ptr = [C.c_void_p(t.data_ptr()) for t in (ctx, new, table, free, state, left, lens, *tok)]
+        args = (n, *ptr[:3], 1, ptr[3], n, *ptr[4:7], ptr[7], n, *ptr[8:], None, C.c_void_p(stream.cuda_stream), buf, 512)
+        torch.cuda.synchronize()
+        for _ in range(10000):
+            if lib.dm_kv8_plan(*args):
+                failed.append((n, buf.value.decode()))
+                break
+
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    threads = [threading.Thread(target=work, args=a) for a in zip((8192, 3500, 8000, 3600, 8100, 4000), streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
