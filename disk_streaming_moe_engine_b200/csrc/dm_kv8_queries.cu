@@ -21,13 +21,13 @@
 // threads, 64 keys of the tile each, that meet at a 64-thread barrier to agree on M; O is
 // rescaled only by warps with a raised row.
 //
-// Roles (384 threads): 8 softmax warps (two per quarter of the rows), a producer warp, a warp that
-// brings the next item's q rows into L2, one that issues the scores and one that issues the O
-// products (each is held up by the tensor cores' short queue and by its own waits; together they
-// keep the queue filled).  The scores of tile x + 1
-// follow as soon as those of tile x are in registers and mostly run before the O product of tile
-// x, so the softmax has the time of two products.  Between items the softmax
-// warps turn the next item's q rows into terms while the last O product runs, then write the
+// Roles (352 threads): 8 softmax warps (two per quarter of the rows), a producer warp, one that issues
+// the scores and one that issues the O products (each is held up by the tensor cores' short queue and
+// by its own waits; together they keep the queue filled).  The scores of tile x + 1 follow as soon as
+// those of tile x are in registers and mostly run before the O product of tile x, so the softmax has
+// the time of two products.  Between items the softmax warps turn the next item's q rows into terms
+// while the last O product runs (a warp that brought those rows into L2 before gained nothing: 2.07 ms
+// with it, 2.04 without for the prompts below), then write the
 // item's O while the next scores run (two separate warps for the terms were slower: the
 // conversions are ALU work that all four schedulers have to share).  Tensor memory: the scores
 // (128 columns), two buffers of weights (96 each; at D = 256 one, written once the O product before
@@ -50,7 +50,7 @@ namespace dm {
 
 constexpr int kQryRows = 128;
 constexpr int kQrySoft = 256;
-constexpr int kQryThreads = kQrySoft + 128;
+constexpr int kQryThreads = kQrySoft + 96;  // the softmax, then three warps
 // an item's start and end in tiles (KeyWalk): q rows to terms and the first scores before, O after,
 // which cost this kernel as much as 6 tiles do; ranges cut by tiles alone end up to that much apart
 constexpr int kQryLead = 6;
@@ -195,29 +195,6 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             }
             tc_commit(&done_bar[1]);
             mbar_wait_bounded(&done_bar[1], 0, a.err, nullptr);
-        }
-    } else if (active && warp == W_MMA + 2) {
-        // ---------------- q rows of the next item to L2 ----------------
-        KeyWalk<RB, kQryLead> w(a, s_range);
-        uint32_t item = 0;
-        while (w.unit < w.end) {
-            int begin, last, real;
-            w.span(begin, last, real);
-            if (last > begin) {
-                if (item > 0 &&
-                    !__all_sync(0xffffffffu, mbar_wait_bounded(&q_ready, (item - 1) & 1u, a.err, abort_flag)))
-                    break;
-                const int nrow = min(RB, w.r.m * a.group - w.block() * RB);
-                for (int i = lane; i < nrow * (D / 64); i += 32) {  // 128 bytes each
-                    const int f = w.block() * RB + i / (D / 64);
-                    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
-                                             static_cast<int64_t>(w.r.row0 + f / a.group) * a.q_rs +
-                                             static_cast<int64_t>(w.h * a.group + f % a.group) * a.q_hs + i % (D / 64) * 64;
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
-                }
-                ++item;
-            }
-            w.next();
         }
     } else if (active) {
         // ---------------- Q terms, softmax, epilogue ----------------

@@ -160,3 +160,25 @@ def test_plans_of_different_sizes_from_several_threads(lib):
         t.join()
     torch.cuda.synchronize()
     assert not failed, failed
+
+
+# ---- many short items ------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("empty", [0, 3, 40])
+def test_many_short_items_on_the_query_side(lib, empty):
+    """Items of one tile, requests without tokens between them: every warp of a CTA walks over many
+    items, and none may fall behind for good (the kernel's waits would run out)."""
+    hk, grp, d, n = 2, 8, 64, 400
+    lens = [0 if i % (empty + 1) else 60 for i in range(n)]
+    rows = [0 if i % (empty + 1) else 9 + i % 12 for i in range(n)]
+    cache = make_cache(n * 4 + 1, hk, d, 2)
+    table = make_table(lens, cache.num_pages, 2)
+    assert query_side(n, max(rows), grp, hk, torch.bfloat16)
+    q = torch.randn(sum(rows), hk * grp, d, generator=torch.Generator().manual_seed(4)).to(DEV, torch.bfloat16)
+    got, _, _ = check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+    cu, err, ws = dev32(np.concatenate([[0], np.cumsum(rows)])), kv8.error_word(), kv8.attention_workspace(cache)
+    for _ in range(50):
+        again = kv8.attention(cache, q, dev32(table), dev32(lens), cu, max(rows), workspace=ws, err=err)
+        assert torch.equal(again, got)
+    kv8.check(err)
