@@ -11,9 +11,9 @@ A host runtime that keeps its own paged cache runs, per step,
 Every call runs on torch's current stream (or `stream`, a cudaStream_t) of the tensors' device
 and returns without waiting, so a step may be captured into a CUDA graph (with the outputs
 given).  Outputs that are not given are allocated on the stream of the call.  The operators serve:
-they have no gradients and refuse tensors that ask for one.  Arguments are checked on the host
-and raise DmError; what only the device can see goes into the error word of `error_word()` and is
-raised by `check()`.
+they have no gradients and refuse tensors that ask for one or carry a forward-mode tangent.
+Arguments are checked on the host and raise DmError; what only the device can see goes into the
+error word of `error_word()` and is raised by `check()`.
 """
 from __future__ import annotations
 
@@ -22,6 +22,7 @@ import threading
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -81,6 +82,8 @@ def _rows(name: str, t: torch.Tensor, heads, dim: int, device, dtype):
              f"contiguous (got {tuple(shape)} {t.dtype} on {t.device})")
     if t.requires_grad and torch.is_grad_enabled():
         _bad(f"{name} asks for a gradient; the operator has none (use torch.no_grad or detach)")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _bad(f"{name} carries a forward-mode gradient; the operator has none (use forward_ad.unpack_dual)")
     return t.data_ptr(), stride[0], stride[1], shape[0], shape[1]
 
 

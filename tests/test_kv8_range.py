@@ -182,3 +182,22 @@ def test_many_short_items_on_the_query_side(lib, empty):
         again = kv8.attention(cache, q, dev32(table), dev32(lens), cu, max(rows), workspace=ws, err=err)
         assert torch.equal(again, got)
     kv8.check(err)
+
+
+# ---- what the operators refuse -----------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(lib):
+    """A dual tensor's tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+    cache = kv8.Kv8Cache.empty(4, 2, 64)
+    x, one = torch.zeros(1, 2, 64, device=DEV), dev32([1])
+    ws = kv8.attention_workspace(cache)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda t: kv8.rope(kv8.RopePlan(64), t, None, one),
+                     lambda t: kv8.append(cache, x, t, dev32([0])),
+                     lambda t: kv8.attention(cache, t, dev32([[0]]), one, workspace=ws)):
+            call(x)
+            with pytest.raises(DmError, match="gradient"):
+                call(dual)
