@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll
                 for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 // largest magnitude of the row to [2^7, 2^8)
-                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
+                const int ex = max(-120, min(120, (__float_as_int(amax) >> 23) - 127 - 7));
                 const float mul = __int_as_float((127 - ex) << 23);
                 if (tid % 16 == 0) {
                     s_frow[r] = 0.5f * a.scale_log2 * __int_as_float((127 + ex) << 23);

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 named_bar_sync(2 + wq, 64);
                 amax = fmaxf(s_max[0][row], s_max[1][row]);
                 named_bar_sync(2 + wq, 64);
-                const int ex = max(-100, min(100, (__float_as_int(amax) >> 23) - 127 - 7));
+                const int ex = max(-120, min(120, (__float_as_int(amax) >> 23) - 127 - 7));
                 frow = a.scale_log2 * __int_as_float((127 + ex) << 23);
                 // a row with NaN or Inf becomes NaN, a row behind the last zero
                 const float mul = row >= nrow ? 0.0f : amax == INFINITY ? __int_as_float(0x7fc00000) : __int_as_float((127 - ex) << 23);

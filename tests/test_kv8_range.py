@@ -201,3 +201,22 @@ def test_forward_mode_is_refused(lib):
             call(x)
             with pytest.raises(DmError, match="gradient"):
                 call(dual)
+
+
+# ---- queries of extreme size -----------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,grp", [(2, 4), (48, 4)])
+@pytest.mark.parametrize("power", [-112, -100, 0, 100, 112, 120])
+def test_q_of_extreme_size(lib, dtype, rows, grp, power):
+    """q times 2^power against keys times 2^-power (as far as the scales go, the softmax scale takes
+    the rest): ordinary scores."""
+    d, keys, k_power = 64, 500, max(-100, min(92, -power))
+    cache = make_cache(-(-keys // PAGE) + 1, 1, d, 8, lo=-8, hi=-8)
+    cache.scales[:, 0] = 2.0 ** (k_power - 8 if k_power > -92 else k_power)
+    q = torch.randn(rows, grp, d, generator=torch.Generator().manual_seed(3)).clamp_(-4, 4)
+    q = (q.double() * 2.0 ** power).to(DEV, dtype)
+    rest = power + math.log2(float(cache.scales[0, 0, 0]))
+    scale = d ** -0.5 * 2.0 ** (-rest - 8)
+    check_against_64_bits(cache, q, make_table([keys], cache.num_pages, 8), [keys], [rows], scale)
