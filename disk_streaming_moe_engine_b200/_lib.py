@@ -84,7 +84,7 @@ class DmKv8Cache(C.Structure):
 
 class DmKv8AttnArgs(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("n", C.c_int32), ("num_q_heads", C.c_int32), ("max_q_len", C.c_int32),
-                ("rows", C.c_int32), ("table_width", C.c_int32), ("sm_scale", C.c_float), ("reserved", C.c_int32),
+                ("rows", C.c_int32), ("table_width", C.c_int32), ("sm_scale", C.c_float), ("flags", C.c_int32),
                 ("q", C.c_void_p), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
                 ("out", C.c_void_p), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
                 ("lse", C.c_void_p), ("block_table", C.c_void_p), ("seq_lens", C.c_void_p), ("cu_q", C.c_void_p),

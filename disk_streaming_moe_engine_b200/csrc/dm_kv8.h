@@ -46,6 +46,7 @@ struct Kv8AttnArgs {
     int n, rows, Hq, Hkv, group, num_pages, width, max_q;
     int exact;            // the work is cut by exact tile counts (few requests, or few blocks in each)
     int q_vec, o_vec;     // q / out: pointer and strides are multiples of 32 bytes
+    int fill;             // zeros in the rows that no request writes
 };
 
 // Exact tile counts cost a pass over all row blocks in every CTA: taken where a warp goes through a

@@ -38,8 +38,8 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     if (!p) return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "null arguments");
     if (p->dtype != DM_DTYPE_BF16 && p->dtype != DM_DTYPE_F32)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "dtype is bf16 or fp32");
-    if (p->n < 0 || p->rows < 0 || p->reserved != 0)
-        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "negative n or rows, or reserved not 0");
+    if (p->n < 0 || p->rows < 0 || (p->flags & ~DM_KV8_FILL_ROWS) != 0)
+        return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "negative n or rows, or an unknown flag");
     if (p->num_q_heads < 1 || p->num_q_heads % c->num_kv_heads != 0)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "CONFIG_ERROR", st, "num_q_heads %d is no multiple of %d kv heads",
                        p->num_q_heads, c->num_kv_heads);
@@ -82,6 +82,7 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     a.num_pages = c->num_pages;
     a.width = p->table_width;
     a.max_q = static_cast<int>(p->max_q_len);
+    a.fill = (p->flags & DM_KV8_FILL_ROWS) != 0;
     a.counters = static_cast<unsigned*>(p->workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + counter_bytes(g.num_sms));
     const bool f32 = p->dtype == DM_DTYPE_F32;

@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
     // tile x has buffer x % BUFS, in the phase of this parity
     auto phase = [](uint32_t x) { return x / BUFS & 1u; };
 
-    if (active && warp == W_LOAD) {
-        key_produce<RB, kKeyLead, D, SL, true>(a, &ka.map, sm, ring, s_range, abort_flag);
+    if (warp == W_LOAD) {
+        if (active) key_produce<RB, kKeyLead, D, SL, true>(a, &ka.map, sm, ring, s_range, abort_flag);
+        if (a.fill) key_fill<T, D>(a);
     } else if (active && warp == W_MMA) {
         // ---------------- MMA ----------------
         if (lane == 0) {

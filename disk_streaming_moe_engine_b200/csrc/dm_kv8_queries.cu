@@ -127,8 +127,9 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    if (active && warp == W_LOAD) {
-        key_produce<RB, kQryLead, D, SL, false>(a, &qa.map, sm, ring, s_range, abort_flag);
+    if (warp == W_LOAD) {
+        if (active) key_produce<RB, kQryLead, D, SL, false>(a, &qa.map, sm, ring, s_range, abort_flag);
+        if (a.fill) key_fill<__nv_bfloat16, D>(a);
     } else if (active && warp == W_MMA) {
         // ---------------- scores ----------------
         if (lane == 0) {

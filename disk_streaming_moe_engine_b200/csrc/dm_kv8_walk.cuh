@@ -285,6 +285,43 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
     return active;
 }
 
+// DM_KV8_FILL_ROWS: zeros in the rows of `out` that no request writes: those before cu_q[0] and from
+// cu_q[n] on, and those of requests that are skipped.  By one warp of every CTA.
+template <typename T, int D>
+DM_DEV void key_fill(const Kv8AttnArgs& a) {
+    constexpr int EV = 16 / sizeof(T);  // elements of 16 bytes
+    const int lane = threadIdx.x & 31;
+    auto clip = [&](long long r) { return static_cast<int>(min(max(r, 0ll), static_cast<long long>(a.rows))); };
+    auto row = [&](int r) {
+        for (int i = lane; i < a.Hq * (D / EV); i += 32) {
+            T* o = static_cast<T*>(a.out) + static_cast<int64_t>(r) * a.o_rs + static_cast<int64_t>(i / (D / EV)) * a.o_hs + i % (D / EV) * EV;
+            if (a.o_vec) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
+            } else {
+                for (int e = 0; e < EV; ++e) o[e] = static_cast<T>(0.0f);
+            }
+        }
+    };
+    auto shared_rows = [&](long long lo, long long hi) {  // by all CTAs together
+        const int end = clip(hi);
+        for (long long r = clip(lo) + static_cast<long long>(blockIdx.x); r < end; r += gridDim.x) row(static_cast<int>(r));
+    };
+    if (a.cu_q) shared_rows(0, a.cu_q[0]);
+    shared_rows(a.cu_q ? a.cu_q[a.n] : a.n, a.rows);
+    for (long long base = static_cast<long long>(blockIdx.x) * 32; a.cu_q && base < a.n; base += static_cast<long long>(gridDim.x) * 32) {
+        const int i = static_cast<int>(min(base + lane, static_cast<long long>(a.n)));
+        long long c0 = 0, c1 = 0;
+        if (i < a.n) c0 = a.cu_q[i], c1 = a.cu_q[i + 1];
+        unsigned skipped = __ballot_sync(0xffffffffu, c1 > c0 && (c0 < 0 || c1 - c0 > a.max_q || c1 > a.rows));
+        while (skipped) {
+            const int l = __ffs(skipped) - 1;
+            skipped &= skipped - 1;
+            const int end = clip(__shfl_sync(0xffffffffu, c1, l));
+            for (int r = clip(__shfl_sync(0xffffffffu, c0, l)); r < end; ++r) row(r);
+        }
+    }
+}
+
 // The CTA whose range holds unit u.
 DM_DEV int key_owner(long long u, long long total, long long grid) { return static_cast<int>(((u + 1) * grid - 1) / total); }
 

@@ -28,6 +28,7 @@ from . import _lib
 
 PAGE_TOKENS = 16
 MAX_REQUESTS = 8192
+FILL_ROWS = 2
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 _DTYPES = {torch.bfloat16: _lib.DM_DTYPE_BF16, torch.float32: _lib.DM_DTYPE_F32}
@@ -261,14 +262,16 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
               lse=None, workspace, err=None, stream=None) -> torch.Tensor:
     """dm_kv8_attention: q [rows][Hq][D] against the cached tokens of each request; rows
     [cu_q[i], cu_q[i + 1]) belong to request i and are its last tokens (cu_q None: one row
-    per request).  Rows from cu_q[n] on are left as they were in `out`."""
+    per request).  Rows that no request writes (before cu_q[0], from cu_q[n] on, those of a request
+    that is skipped) are left as they were in `out`, and zeros if `out` is not given."""
     dev, D = cache.device, cache.head_dim
     n = seq_lens.numel()
     if q.dtype not in _DTYPES:
         _bad(f"q is bf16 or fp32 (got {q.dtype})")
     q_ptr, q_rs, q_hs, rows, hq = _rows("q", q, None, D, dev, q.dtype)
+    flags = 0
     if out is None:
-        out = _allocate(dev, stream, torch.empty_like, q)
+        out, flags = _allocate(dev, stream, torch.empty_like if n else torch.zeros_like, q), FILL_ROWS
     out_ptr, out_rs, out_hs, out_rows, _ = _rows("out", out, hq, D, dev, q.dtype)
     _ints(dev, "block_table seq_lens cu_q err", block_table, seq_lens, cu_q, err)
     if block_table.dim() != 2 or block_table.shape[0] < n or (cu_q is not None and cu_q.numel() < n + 1) or \
@@ -280,7 +283,7 @@ def attention(cache: Kv8Cache, q, block_table, seq_lens, cu_q=None, max_q_len: i
     if workspace.device != dev or not workspace.is_contiguous():
         _bad("the workspace must be a contiguous tensor on the cache's device")
     a = _lib.DmKv8AttnArgs(
-        _DTYPES[q.dtype], n, hq, max_q_len, rows, block_table.shape[1], D ** -0.5 if sm_scale is None else sm_scale, 0,
+        _DTYPES[q.dtype], n, hq, max_q_len, rows, block_table.shape[1], D ** -0.5 if sm_scale is None else sm_scale, flags,
         q_ptr, q_rs, q_hs, out_ptr, out_rs, out_hs, None if lse is None else lse.data_ptr(), block_table.data_ptr(),
         seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), None if err is None else err.data_ptr())

@@ -595,12 +595,13 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * zeroed again).  Calls that may overlap in time (other streams, graphs) need workspaces of
  * their own; graphs and calls that run one after the other may share one.
  * table_width <= 2^26, rows * num_q_heads < 2^31; out overlaps no input. */
+#define DM_KV8_FILL_ROWS 0x2  /* rows of out that no request writes, skipped requests' among them, become zeros (n > 0) */
 typedef struct dm_kv8_attn_args {
     int32_t dtype, n, num_q_heads, max_q_len;
     int32_t rows;              /* rows of q and out                                       */
     int32_t table_width;
     float sm_scale;
-    int32_t reserved;          /* 0 */
+    int32_t flags;             /* 0 or DM_KV8_FILL_ROWS                                   */
     const void* q;
     int64_t q_row_stride, q_head_stride;
     void* out;

@@ -220,3 +220,51 @@ def test_q_of_extreme_size(lib, dtype, rows, grp, power):
     rest = power + math.log2(float(cache.scales[0, 0, 0]))
     scale = d ** -0.5 * 2.0 ** (-rest - 8)
     check_against_64_bits(cache, q, make_table([keys], cache.num_pages, 8), [keys], [rows], scale)
+
+
+# ---- rows that no request covers ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,grp", [(torch.float32, 5, 4), (torch.bfloat16, 5, 4), (torch.bfloat16, 60, 8)])
+def test_allocated_outputs_have_no_stale_rows(lib, dtype, rows, grp):
+    """attention() without `out`: rows that belong to no request, or to one that is skipped, are
+    zeros, not what the memory held before."""
+    lens, d = [70, 90, 40], 64
+    cache = make_cache(20, 1, d, 1)
+    table, ws = make_table(lens, 20, 1), kv8.attention_workspace(cache)
+    total = 3 * rows + 7
+    q = torch.randn(total, grp, d, generator=torch.Generator().manual_seed(0)).to(DEV, dtype)
+
+    def written(got, a, b, length):
+        """Rows a to b of a request: those that see a key have results, the others zeros."""
+        sees = torch.arange(a, b, device=DEV) >= b - length
+        return bool(((got[a:b] != 0).any(-1) == sees[:, None]).all())
+
+    def run(cu, lengths, max_q=rows, rest=None):
+        err = kv8.error_word()
+        torch.cuda.synchronize()
+        stale = [torch.full_like(q, math.nan) for _ in range(4)]
+        del stale
+        got = kv8.attention(cache, q, dev32(table), dev32(lengths), None if cu is None else dev32(cu), max_q,
+                            workspace=ws, err=err)
+        if rest is None:
+            kv8.check(err)
+        else:
+            with pytest.raises(DmError):
+                kv8.check(err)
+        return got
+
+    got = run([2, 2 + rows, 2 + 2 * rows, 3 * rows], lens)
+    assert (got[:2] == 0).all() and (got[3 * rows:] == 0).all() and got[2:3 * rows].isfinite().all()
+    assert written(got, 2, 2 + rows, 70) and written(got, 2 + rows, 2 + 2 * rows, 90) and written(got, 2 + 2 * rows, 3 * rows, 40)
+    # request 1 has more rows than max_q_len
+    got = run([0, 2, 2 + rows + 1, 2 * rows], lens, rest=True)
+    assert (got[2:3 + rows] == 0).all() and (got[2 * rows:] == 0).all()
+    assert written(got, 0, 2, 70) and written(got, 3 + rows, 2 * rows, 40)
+    # row ranges outside q and backwards
+    got = run([0, 3, 2, total + 5], lens, rest=True)
+    assert (got[:2] != 0).any(-1).all() and (got[3:] == 0).all() and got.isfinite().all()
+    if rows == 5:  # one row per request, more rows than requests
+        got = run(None, lens, max_q=1)
+        assert (got[3:] == 0).all() and (got[:3] != 0).any(-1).all()
+        assert (run([0, 0, 0, 0], lens) == 0).all()
