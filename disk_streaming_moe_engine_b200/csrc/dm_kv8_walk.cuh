@@ -286,9 +286,10 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
 }
 
 // DM_KV8_FILL_ROWS: zeros in the rows of `out` that no request writes: those before cu_q[0] and from
-// cu_q[n] on, and those of requests that are skipped.  By one warp of every CTA.
+// cu_q[n] on, and those of requests that are skipped.  By one warp of every CTA; out of line, for the
+// instruction cache is what the prompts' kernel has least of (inlined: 4 x 8192 2.05 -> 2.20 ms).
 template <typename T, int D>
-DM_DEV void key_fill(const Kv8AttnArgs& a) {
+__device__ __noinline__ void key_fill(const Kv8AttnArgs& a) {
     constexpr int EV = 16 / sizeof(T);  // elements of 16 bytes
     const int lane = threadIdx.x & 31;
     auto clip = [&](long long r) { return static_cast<int>(min(max(r, 0ll), static_cast<long long>(a.rows))); };
