@@ -59,6 +59,22 @@ Kv8Device::~Kv8Device() {
     if (prev >= 0) cudaSetDevice(prev);
 }
 
+static __device__ uint32_t g_kv8_err;
+
+uint32_t* kv8_error_word(uint32_t* callers, int dev) {
+    if (callers) return callers;
+    static std::atomic<void*> at[64];  // per device, once known
+    void* p = dev < 64 ? at[dev].load(std::memory_order_relaxed) : nullptr;
+    if (!p) {
+        if (cudaGetSymbolAddress(&p, g_kv8_err) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        if (dev < 64) at[dev].store(p, std::memory_order_relaxed);
+    }
+    return static_cast<uint32_t*>(p);
+}
+
 int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t es) {
     if (!c || !c->pages || !c->scales)
         return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", stage, "null cache");
@@ -617,8 +633,12 @@ using namespace dm;
 extern "C" int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* eb, uint64_t es) {
     const char* st = "kv8_status";
     if (eb && es > 0) eb[0] = '\0';
-    if (!err_dev) return kv8_err(eb, es, DM_ERR_INVALID_ARG, "INVALID_ARG", st, "null error word");
     Kv8Device g;
+    if (!err_dev) {
+        int dev = -1;
+        if (cudaGetDevice(&dev) == cudaSuccess) err_dev = kv8_error_word(nullptr, dev);
+        if (!err_dev) return kv8_err(eb, es, DM_ERR_CUDA, "CUDA_ERROR", st, "no device");
+    }
     if (int rc = g.enter(err_dev, st, eb, es)) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -673,7 +693,7 @@ extern "C" int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t
     a.slots = slots;
     a.positions = positions;
     a.requests = requests;
-    a.err = err_dev;
+    a.err = kv8_error_word(err_dev, g.dev);
     a.n = n;
     a.width = table_width;
     a.cap = free_capacity;
@@ -825,7 +845,7 @@ extern "C" int32_t dm_kv8_append(const dm_kv8_cache* c, int32_t dtype, int32_t n
     a.x[0] = k, a.rs[0] = k_rs, a.hs[0] = k_hs;
     a.x[1] = v, a.rs[1] = v_rs, a.hs[1] = v_hs;
     a.slots = slots;
-    a.err = err_dev;
+    a.err = kv8_error_word(err_dev, g.dev);
     a.n = n;
     a.Hkv = c->num_kv_heads;
     a.num_pages = c->num_pages;

@@ -22,6 +22,10 @@ struct Kv8Device {
     ~Kv8Device();
 };
 
+// The device word that takes the error bits of a call: the caller's, or this library's own of the
+// current device (null only if CUDA cannot say where it is).
+uint32_t* kv8_error_word(uint32_t* callers, int dev);
+
 int kv8_check_cache(const dm_kv8_cache* c, const char* stage, char* eb, uint64_t es);
 
 inline bool kv8_aligned(const void* p, int64_t stride_a, int64_t stride_b, int elem, int to) {

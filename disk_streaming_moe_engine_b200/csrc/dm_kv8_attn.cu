@@ -73,7 +73,7 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     a.table = p->block_table;
     a.seq_lens = p->seq_lens;
     a.cu_q = p->cu_q;
-    a.err = p->err_dev;
+    a.err = kv8_error_word(p->err_dev, g.dev);
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
     a.n = p->n;
     a.rows = p->rows;

@@ -12,8 +12,8 @@ Every call runs on torch's current stream (or `stream`, a cudaStream_t) of the t
 and returns without waiting, so a step may be captured into a CUDA graph (with the outputs
 given).  Outputs that are not given are allocated on the stream of the call.  The operators serve:
 they have no gradients and refuse tensors that ask for one or carry a forward-mode tangent.
-Arguments are checked on the host and raise DmError; what only the device can see goes into the
-error word of `error_word()` and is raised by `check()`.
+Arguments are checked on the host and raise DmError; what only the device can see goes into an
+error word, the call's `err` or one of the device's own, and is raised by `check()`.
 """
 from __future__ import annotations
 
@@ -93,10 +93,16 @@ def error_word(device="cuda") -> torch.Tensor:
     return torch.zeros(1, dtype=torch.int32, device=device)
 
 
-def check(err: torch.Tensor, stream=None) -> None:
-    """Waits for the stream, clears the error word and raises DmError when a bit was set."""
+def check(err: torch.Tensor | None = None, stream=None, device=None) -> None:
+    """Waits for the stream, clears the error word and raises DmError when a bit was set.  Without
+    `err`: the word of the device (by default the current one) that all calls without `err` share."""
     buf = _buffer()
-    rc = _lib.load().dm_kv8_status(err.data_ptr(), _stream(err.device, stream), buf, _ERR)
+    if err is not None:
+        rc = _lib.load().dm_kv8_status(err.data_ptr(), _stream(err.device, stream), buf, _ERR)
+    else:
+        with torch.cuda.device(device):
+            rc = _lib.load().dm_kv8_status(
+                None, torch.cuda.current_stream().cuda_stream if stream is None else stream, buf, _ERR)
     if rc != _lib.DM_OK:
         _raise(rc, buf)
 

@@ -467,7 +467,8 @@ int32_t dm_moe_layer_noalloc(int32_t hidden_size, int32_t moe_intermediate_size,
  * as it was.  All pointers are device memory of that device unless marked _host.
  * Statuses and err_buf are as in dm_moe_layer_noalloc.  What only the device can see (a
  * page id out of range, lengths that do not fit) is OR-ed as DM_DEVERR_* bits into
- * *err_dev (one uint32, may be NULL) and the access is skipped; dm_kv8_status reads it.
+ * *err_dev (one uint32; NULL: the library's own word of the device) and the access is
+ * skipped; dm_kv8_status reads it.
  *
  * Cache layout (the engine's page layout, one byte per value):
  *   pages  uint8 [num_pages][K|V][Hkv][16][D]   e4m3 codes
@@ -492,7 +493,8 @@ typedef struct dm_kv8_cache {
     int32_t reserved;   /* 0 */
 } dm_kv8_cache;
 
-/* Waits for `stream`, reads and clears *err_dev and returns it as a status (DM_OK,
+/* Waits for `stream`, reads and clears *err_dev (NULL: the library's own word of the current
+ * device, which all calls without a word share) and returns it as a status (DM_OK,
  * DM_ERR_TIMEOUT, DM_ERR_CAPACITY, DM_ERR_INVALID_ARG for PAGE and RANGE,
  * DM_ERR_NONFINITE, in this order).  Not inside a capture. */
 int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t err_buf_size);

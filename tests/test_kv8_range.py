@@ -268,3 +268,61 @@ def test_allocated_outputs_have_no_stale_rows(lib, dtype, rows, grp):
         got = run(None, lens, max_q=1)
         assert (got[3:] == 0).all() and (got[:3] != 0).any(-1).all()
         assert (run([0, 0, 0, 0], lens) == 0).all()
+
+
+@pytest.mark.gpu
+def test_errors_without_a_word_are_kept(lib):
+    """Without `err` the device's own error word takes what only the device can see: a refused plan,
+    a slot behind the cache and a request with too many rows raise at the next check()."""
+    kv8.check()
+    cache = kv8.Kv8Cache.empty(4, 1, 64)
+    x, ws = torch.randn(3, 1, 64, device=DEV), kv8.attention_workspace(cache)
+    free, state = kv8.free_list(1)
+    kv8.plan_slots(free, state, torch.zeros((1, 4), dtype=torch.int32, device=DEV), dev32([0]), dev32([40]), 64)
+    with pytest.raises(DmError) as e:
+        kv8.check()
+    assert e.value.code == _lib.DM_ERR_CAPACITY
+    kv8.check()
+    kv8.append(cache, x, x, dev32([0, 1, 4000]))
+    with pytest.raises(DmError):
+        kv8.check()
+    kv8.attention(cache, x, dev32([[0]]), dev32([2]), dev32([0, 3]), 2, workspace=ws)
+    with pytest.raises(DmError):
+        kv8.check(device=x.device)
+    kv8.check()
+    graph, word, out = torch.cuda.CUDAGraph(), kv8.error_word(), torch.empty_like(x)
+    args = (cache, x, dev32([[0]]), dev32([2]), dev32([0, 3]), 2)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        kv8.attention(*args, out=out, workspace=ws)
+    kv8.check()
+    graph.replay()
+    kv8.check(word)  # a word of one's own stays clean
+    with pytest.raises(DmError):
+        kv8.check()
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_may_be_captured(lib):
+    """Nothing that a call needs is made in a way that a capture forbids."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from disk_streaming_moe_engine_b200 import DmError, kv8
+free, state = kv8.free_list(1)
+ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+table, ctx, new = torch.zeros((1, 4), dtype=torch.int32, device="cuda"), ints(0), ints(40)
+tok = torch.zeros((5, 64), dtype=torch.int32, device="cuda")
+out, graph = kv8.SlotPlan(*tok), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    kv8.plan_slots(free, state, table, ctx, new, 64, out=out)
+graph.replay()
+try:
+    kv8.check()
+except DmError as e:
+    print("refused", e.code)
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert out.stdout.strip() == f"refused {_lib.DM_ERR_CAPACITY}", out.stderr[-2000:]
