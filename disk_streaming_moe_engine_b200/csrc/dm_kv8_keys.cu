@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
     __shared__ KeyRange s_range;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ uint8_t s_nan[kKeyTile];
+    __shared__ int s_nan;  // a NaN code of V that not every row sees was left out of the item's O
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &s_abort;
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
         mbar_init(&done_bar, 1);
         mbar_fence_init();
         s_abort = 0;
+        s_nan = 0;
     }
     if (warp == W_MMA) tc_alloc(&s_tmem, S::kCols);
 
@@ -365,8 +366,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     y[r] = e * (e < kKeySmall ? kKeyBoost * kKeyGroup : kKeyBoost) * e;
                 }
                 if (edge) {
-                    // V rows behind the last key become zeros; a NaN code that not every row sees
-                    // becomes 0 and makes the sums of the rows that see it NaN
+                    // V rows behind the last key become zeros, and so does a NaN code that not every row sees
                     if (r0 == 0) {
                         ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
                         uint8_t* v = sm + (ring.v_load(x) % SL) * S::kSlot + S::Tile::kV + S::Tile::row(tt);
@@ -388,13 +388,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                                     }
                                 }
                         }
-                        s_nan[tt] = nan;
-                    }
-                    named_bar_sync(1, SOFT);
-                    if (s_nan[tt]) {
-#pragma unroll
-                        for (int r = 0; r < 8; ++r)
-                            if (key < s_lim[r0 + r]) l[r] = __int_as_float(0x7fc00000);
+                        if (nan) s_nan = 1;
                     }
                 }
                 uint8_t* p = s_p + x % BUFS * S::kP + tt * 16;
@@ -431,9 +425,11 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
             ok = ok && mbar_wait_bounded(&pv_done[(t - 1) % BUFS], phase(t - 1), a.err, abort_flag);
             if (named_bar_or(1, SOFT, !ok)) break;
             tc_fence_after();
+            const bool nan_left = s_nan;
 #pragma unroll
             for (int r = 0; r < 8; ++r) l[r] = s_red[0][r0 + r] + s_red[1][r0 + r] + s_red[2][r0 + r] + s_red[3][r0 + r];
             named_bar_sync(1, SOFT);  // s_red is free again
+            if (tid == 0) s_nan = 0;  // before the next item's barriers
 
             const long long item0 = w.tile0();  // the item's first tile in the sequence
             const bool whole = t_begin == 0 && nt == real;
@@ -466,6 +462,17 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     for (int r = 0; r < 8; ++r)
                         o[r] = fmaf(fmaf(v[1][r], 1.0f / kKeyGroup, v[0][r]),
                                     1.0f / (static_cast<float>(1 << (4 * b)) * kKeyBoost), o[r]);
+                }
+                if (nan_left && tt < CW) {  // the rows that see it have a NaN in its element
+                    const int d = c * CW + tt, lo = max(lim_min, t_begin * kKeyTile), hi = min(lim_max, (t_begin + nt) * kKeyTile);
+#pragma unroll 1
+                    for (int k = lo; k < hi; ++k)
+                        if (key_nan32(a, w.req, w.h, D, d & ~31, k, k + 1) >> (d & 31) & 1u) {
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                if (k < s_lim[r0 + r]) o[r] = __int_as_float(0x7fc00000);
+                        }
+                    __syncwarp();  // the loads are the whole warp's
                 }
                 if (tt < CW) {
 #pragma unroll

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
     __shared__ KeyRange s_range;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ uint8_t s_nan[kKeyTile];
+    __shared__ int4 s_nan[2];  // by the item's parity: request, kv head and keys whose NaN codes were left out of O
     __shared__ unsigned s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     volatile int* abort_flag = &s_abort;
@@ -202,12 +202,13 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
         const int row = tid & 127, half = tid >> 7, wq = warp & 3;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16);
         constexpr int H = D / 2;  // a thread's share of its row's q and O
-        uint32_t t = 0;
+        uint32_t t = 0, item = 0;
         bool ok = true;
         struct Done {  // an item whose O waits for its epilogue
             long long tile0;
             int64_t row;
-            int t_begin, nt, real, head, live;
+            int t_begin, nt, real, head, lim;  // lim: keys that the row sees; -1: no row
+            bool nan;
             float mref, l;
         } done;
         done.nt = 0;
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             const float mref = done.mref, l = done.l;
             constexpr int kSlot = RB * (D + 2);
             float* slot = a.part + (static_cast<size_t>(blockIdx.x) * 2 + (done.t_begin == 0 ? 1 : 0)) * kSlot;
-            const bool live = ok && done.live;
+            const bool live = ok && done.lim >= 0;
             __nv_bfloat16* out =
                 static_cast<__nv_bfloat16*>(a.out) + done.row * a.o_rs + static_cast<int64_t>(done.head) * a.o_hs;
             // 16 consecutive results of this row from element d on
@@ -252,6 +253,14 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                 float o[32];
                 tc_ld32(lanes + kO + d, o);
                 tc_wait_ld();
+                if (done.nan) {  // the rows that see one have a NaN in its element
+                    const int4 n = s_nan[(item - 1) & 1u];
+                    const uint32_t bits = key_nan32(a, n.x, n.y, D, d, n.z, min(n.w, done.lim));
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (bits >> j & 1u) o[j] = __int_as_float(0x7fc00000);
+                    __syncwarp();  // the loads are the whole warp's
+                }
                 if (whole) {
                     if (live) {
                         put16(o, d, inv, none);
@@ -512,8 +521,7 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                     for (int t = 0; t < kQryTerms; ++t) tc_st16(lanes + pb + t * 32, pt[t]);
                 }
                 if (edge) {
-                    // V rows behind the last key become zeros; a NaN code that not every row sees
-                    // becomes 0 and makes the sums of the rows that see it NaN
+                    // V rows behind the last key become zeros, and so does a NaN code that not every row sees
                     if (half == 0) {
                         ok = ok && ring.wait_full(ring.v_load(x), a.err, abort_flag);
                         uint8_t* v = sm + (ring.v_load(x) % SL) * S::kTileBytes + S::Tile::row(row);
@@ -536,17 +544,9 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
                                     }
                                 }
                         }
-                        s_nan[row] = nan;
                         fence_proxy_async_smem();
-                        nan_row = nan;
+                        nan_row = nan_row || nan;
                     }
-                    if (named_bar_or(1, kQrySoft, half == 0 && nan_row)) {
-                        nan_row = false;
-                        for (int k = 0; k < kKeyTile; ++k)
-                            if (s_nan[k] && tile0 + k < lim) l = __int_as_float(0x7fc00000);
-                        named_bar_sync(1, kQrySoft);
-                    }
-                    nan_row = false;
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -562,7 +562,14 @@ __global__ void __launch_bounds__(kQryThreads, 1) kv8_attn_queries_kernel(const 
             done.tile0 = w.tile0();
             done.row = w.r.row0 + tok;
             done.head = head;
-            done.live = row < nrow;
+            done.lim = row < nrow ? lim : -1;
+            done.nan = false;
+            if (t_end * kKeyTile > lim_min) {  // tiles that not every row sees
+                if (tid == 0)
+                    s_nan[item & 1u] = make_int4(w.req, w.h, max(lim_min, t_begin * kKeyTile), min(lim_max, t_end * kKeyTile));
+                done.nan = named_bar_or(1, kQrySoft, nan_row);
+            }
+            ++item;
             done.t_begin = t_begin, done.nt = nt, done.real = real;
             w.next();
         }

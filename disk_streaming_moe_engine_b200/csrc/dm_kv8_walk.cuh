@@ -285,6 +285,21 @@ DM_DEV bool key_range(const Kv8AttnArgs& a, int min_units, long long* s_sum, Key
     return active;
 }
 
+// Bits of which of 32 elements from d on have a NaN code in V of some key in [lo, hi).  For keys that
+// not every row of an item sees (their NaN codes are zeros in the product): read from the cache, out
+// of line, for it hardly ever runs.
+static __device__ __noinline__ uint32_t key_nan32(const Kv8AttnArgs& a, int req, int h, int D, int d, int lo, int hi) {
+    uint32_t bits = 0;
+    for (int key = lo; key < hi; ++key) {
+        const int id = a.table[static_cast<size_t>(req) * a.width + key / kKv8Page];
+        if (id < 0 || id >= a.num_pages) continue;
+        const size_t at = ((static_cast<size_t>(id) * 2 + 1) * a.Hkv + h) * (kKv8Page * D) + static_cast<size_t>(key % kKv8Page) * D + d;
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(a.pages + at);
+        for (int i = 0; i < 8; ++i) bits |= ((e4m3_nan_mask(p[i]) & 0x01010101u) * 0x01020408u >> 24) << (4 * i);
+    }
+    return bits;
+}
+
 // DM_KV8_FILL_ROWS: zeros in the rows of `out` that no request writes: those before cu_q[0] and from
 // cu_q[n] on, and those of requests that are skipped.  By one warp of every CTA; out of line, for the
 // instruction cache is what the prompts' kernel has least of (inlined: 4 x 8192 2.05 -> 2.20 ms).

@@ -589,7 +589,8 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * cu_q[n] on stay as they were.  max_q_len >= every request's query count (a request with
  * more is skipped, DM_DEVERR_RANGE); it also chooses the kernel.  A key on a page id out of
  * range is left out (DM_DEVERR_PAGE), and so are keys beyond the table's width
- * (DM_DEVERR_CAPACITY).  NaN codes of keys that a query does not see do not reach it.
+ * (DM_DEVERR_CAPACITY).  NaN codes of keys that a query does not see do not reach it; one in
+ * V that it sees makes that element NaN, one in K its whole row.
  * dtype (q and out) bf16 or fp32; scores, softmax and sums are fp32.
  * lse (may be NULL) [rows][Hq] receives ln sum exp of the scaled scores.
  * workspace: dm_kv8_attention_workspace bytes, 256-byte aligned, zeroed once before its

@@ -326,3 +326,41 @@ except DmError as e:
 """
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert out.stdout.strip() == f"refused {_lib.DM_ERR_CAPACITY}", out.stderr[-2000:]
+
+
+# ---- NaN codes of V ------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("keys,rows,grp,at", [(70, 50, 4, 40), (700, 60, 4, 655), (4000, 48, 4, 3960), (300, 1, 8, 299),
+                                              (9000, 60, 4, 8990), (300, 20, 4, 10)])
+def test_nan_of_v_reaches_its_element_alone(lib, dtype, d, keys, rows, grp, at):
+    """softmax(q K^T) V with one NaN in V: every row that sees the key has that element NaN and no
+    other, its lse is untouched; rows that do not see it are untouched."""
+    cache = make_cache(-(-keys // PAGE) + 2, 2, d, 5)
+    table = make_table([keys], cache.num_pages, 5)
+    q = torch.randn(rows, 2 * grp, d, generator=torch.Generator().manual_seed(2)).to(DEV, dtype)
+    ws, cu = kv8.attention_workspace(cache), [0, rows]
+
+    def run():
+        lse = torch.empty(q.shape[:2], device=DEV)
+        got = kv8.attention(cache, q, dev32(table), dev32([keys]), dev32(cu), rows, workspace=ws, lse=lse,
+                            out=torch.zeros_like(q))
+        return got.float().cpu().numpy(), lse.cpu().numpy()
+    want, want_lse = run()
+    page = int(table[0, at // PAGE])
+    cache.pages[page, 1, 0, at % PAGE, 3] = 0xff
+    cache.pages[page, 1, 1, at % PAGE, d - 2] = 0x7f
+    if at + 1 < keys:
+        cache.pages[int(table[0, (at + 1) // PAGE]), 1, 1, (at + 1) % PAGE, d // 2] = 0x7f
+    got, lse = run()
+    np.testing.assert_array_equal(lse, want_lse)
+    pos = np.arange(rows) + keys - rows
+    nan = np.zeros(got.shape, bool)
+    nan[pos >= at, :grp, 3] = True
+    nan[pos >= at, grp:, d - 2] = True
+    if at + 1 < keys:
+        nan[pos >= at + 1, grp:, d // 2] = True
+    assert (np.isnan(got) == nan).all()
+    np.testing.assert_array_equal(got[~nan], want[~nan])
