@@ -364,3 +364,134 @@ def test_nan_of_v_reaches_its_element_alone(lib, dtype, d, keys, rows, grp, at):
         nan[pos >= at + 1, grp:, d // 2] = True
     assert (np.isnan(got) == nan).all()
     np.testing.assert_array_equal(got[~nan], want[~nan])
+
+
+# ---- the query side at the sizes that the key side is tested at ------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,keys", [(64, 60000), (128, 50000), (256, 30000)])
+def test_query_side_many_tiles(lib, d, keys):
+    """Every CTA passes through its ring of slots and scales several times, items are joined from
+    many parts."""
+    lens, rows, grp = [keys, keys - 777, 40], [48, 50, 48], 4
+    assert query_side(3, 50, grp, 1, torch.bfloat16)
+    cache = make_cache(sum(-(-n // PAGE) for n in lens) + 1, 1, d, 4)
+    table = make_table(lens, cache.num_pages, 4)
+    q = torch.randn(sum(rows), grp, d, generator=torch.Generator().manual_seed(5)).to(DEV, torch.bfloat16)
+    check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,n,q_hi,grp", [(64, 66, 140, 8), (128, 70, 90, 12)])
+def test_query_side_many_requests_of_many_rows(lib, d, n, q_hi, grp):
+    """More than 64 requests of more than 1024 rows per kv head: blocks in pairs, not by exact tiles."""
+    g = np.random.default_rng(n)
+    rows = g.integers(0, q_hi + 1, n)
+    rows[3] = q_hi
+    lens = rows + g.integers(0, 200, n) * (g.random(n) < 0.7)
+    assert q_hi * grp > 1024 and query_side(n, q_hi, grp, 1, torch.bfloat16)
+    lens, rows = [int(x) for x in lens], [int(x) for x in rows]
+    cache = make_cache(sum(-(-x // PAGE) for x in lens) + 1, 1, d, 6)
+    table = make_table(lens, cache.num_pages, 6)
+    q = torch.randn(sum(rows), grp, d, generator=torch.Generator().manual_seed(6)).to(DEV, torch.bfloat16)
+    check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 256])
+def test_prompt_beside_single_tokens(lib, dtype, d):
+    """A server's step: one prompt and one chunk among requests with a token each, in one call."""
+    lens, rows, grp = [900] + [37 * i + 1 for i in range(40)] + [2000], [900] + [1] * 40 + [130], 4
+    assert query_side(42, 900, grp, 2, dtype) == (dtype == torch.bfloat16)
+    cache = make_cache(sum(-(-x // PAGE) for x in lens) + 1, 2, d, 7)
+    table = make_table(lens, cache.num_pages, 7)
+    q = torch.randn(sum(rows), 2 * grp, d, generator=torch.Generator().manual_seed(7)).to(DEV, dtype)
+    check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["strided", "odd"])
+def test_query_side_strides(lib, how):
+    """q and out as parts of larger tensors, at 32-byte boundaries and off them: the bits of the
+    contiguous call, and nothing beside them is touched."""
+    lens, rows, grp, d = [700, 333], [60, 50], 4, 128
+    assert query_side(2, 60, grp, 2, torch.bfloat16)
+    cache = make_cache(70, 2, d, 8)
+    table = make_table(lens, 70, 8)
+    q = torch.randn(110, 2 * grp, d, generator=torch.Generator().manual_seed(8)).to(DEV, torch.bfloat16)
+    want, _, _ = check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+    a, pad = (16, 32) if how == "strided" else (1, 7)
+    wide = torch.full((110, 2 * grp + 1, d + pad), 9.0, device=DEV, dtype=torch.bfloat16)
+    out = torch.full((110, 3 * grp, d + pad), 5.0, device=DEV, dtype=torch.bfloat16)
+    wide[:, 1:, a:a + d] = q
+    kv8.attention(cache, wide[:, 1:, a:a + d], dev32(table), dev32(lens), dev32([0, 60, 110]), 60,
+                  out=out[:, grp:, a:a + d], workspace=kv8.attention_workspace(cache))
+    assert torch.equal(out[:, grp:, a:a + d], want)
+    out[:, grp:, a:a + d] = 5.0
+    assert (out == 5).all()
+
+
+@pytest.mark.gpu
+def test_query_side_leaves_other_rows(lib):
+    """Rows behind the last request stay; a request with too many queries, a bad page and a length
+    beyond the table are reported and touch nothing else."""
+    lens, rows, grp, d = [260, 275], 100, 4, 64
+    assert query_side(2, rows, grp, 1, torch.bfloat16)
+    cache = make_cache(40, 1, d, 9)
+    table = make_table(lens, 40, 9)
+    q = torch.randn(2 * rows, grp, d, generator=torch.Generator().manual_seed(9)).to(DEV, torch.bfloat16)
+    want, _, _ = check_against_64_bits(cache, q, table, lens, [rows, rows], d ** -0.5)
+    ws, err, cu = kv8.attention_workspace(cache), kv8.error_word(), dev32([0, rows, 2 * rows])
+    pad = torch.cat([q, q])
+    out = torch.full(pad.shape, 3.0, dtype=q.dtype, device=DEV)
+    kv8.attention(cache, pad, dev32(table), dev32(lens), cu, rows, out=out, workspace=ws, err=err)
+    kv8.check(err)
+    assert torch.equal(out[:2 * rows], want) and (out[2 * rows:] == 3).all()
+    out.fill_(3.0)
+    kv8.attention(cache, q, dev32(table), dev32(lens), dev32([0, rows + 1, 2 * rows]), rows, out=out, workspace=ws, err=err)
+    with pytest.raises(DmError):
+        kv8.check(err)
+    assert (out[:rows + 1] == 3).all() and not (out[rows + 1:2 * rows] == 3).all(-1).any()
+    bad = table.copy()
+    bad[1, 1] = cache.num_pages
+    got = kv8.attention(cache, q, dev32(bad), dev32(lens), cu, rows, workspace=ws, err=err)
+    with pytest.raises(DmError):
+        kv8.check(err)
+    assert torch.equal(got[:rows], want[:rows]) and got.isfinite().all()
+    got = kv8.attention(cache, q, dev32(table), dev32([260, 16 * table.shape[1] + 1]), cu, rows, workspace=ws, err=err)
+    with pytest.raises(DmError) as e:
+        kv8.check(err)
+    assert e.value.code == _lib.DM_ERR_CAPACITY and torch.equal(got[:rows], want[:rows])
+
+
+@pytest.mark.gpu
+def test_calls_at_the_same_time(lib):
+    """Both kernels on two streams at once, a workspace each, eager and as captured graphs: the bits
+    of the calls alone."""
+    d, grp = 128, 4
+    cache = make_cache(900, 2, d, 10)
+    cases = []
+    for lens, rows, dtype in (([5000, 3000, 400], [1, 1, 1], torch.float32), ([2000, 900], [300, 64], torch.bfloat16)):
+        table = make_table(lens, 900, len(lens))
+        q = torch.randn(sum(rows), 2 * grp, d, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
+        want, _, _ = check_against_64_bits(cache, q, table, lens, rows, d ** -0.5)
+        args = (cache, q, dev32(table), dev32(lens), dev32(np.concatenate([[0], np.cumsum(rows)])), max(rows))
+        cases.append((args, want, torch.cuda.Stream(), kv8.attention_workspace(cache), torch.zeros_like(q), torch.cuda.CUDAGraph()))
+    torch.cuda.synchronize()
+    for args, _, stream, ws, out, graph in cases:
+        with torch.cuda.graph(graph, stream=stream):
+            kv8.attention(*args, out=out, workspace=ws)
+    err = kv8.error_word()
+    for i in range(20):
+        for args, _, stream, ws, out, graph in cases:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                if i % 2:
+                    graph.replay()
+                else:
+                    kv8.attention(*args, out=out, workspace=ws, err=err)
+        torch.cuda.synchronize()
+        for _, want, _, _, out, _ in cases:
+            assert torch.equal(out, want)
+    kv8.check(err)
