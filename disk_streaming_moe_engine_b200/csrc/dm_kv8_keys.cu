@@ -8,10 +8,11 @@
 //   O^T [D x NP]        += codeV^T [D x 128] . Pterms [128 x NP]
 // N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
 // scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
-// before it left) and costs only N: 2 terms give bf16's 8 bits, fp32 takes 5 (2^-20).  Weights need
-// range as well: thousands of keys may lie many nats below one whose V is small.  So NP = 2 N: a
-// weight below 2^-12 of the reference enters 2^14 times larger in columns of its own, the others'
-// columns hold zero there (one group of columns lost all below 2^-19).  The tensor
+// before it left) and costs only N: 2 terms hold bf16's 8 bits of q, its weights take 3 (2^-11, so
+// that the result is as good as its rounding; 2 were 2 to 4 % faster), fp32 5 for both (2^-20).
+// Weights need range as well: thousands of keys may lie many nats below one whose V is small.  So NP
+// is twice their terms: a weight below 2^-12 of the reference enters 2^14 times larger in columns of
+// its own, the others' columns hold zero there (one group of columns lost all below 2^-19).  The tensor
 // time of a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
 // below the time of the tile's bytes from HBM, which is what bounds long caches: 64 requests of
 // 32768 tokens (2 kv heads of 256, 8 query heads each) take 346 us, 6.21 TB/s, 0.96 of the measured
@@ -25,8 +26,8 @@
 // log2 units: e = 2^((x + v - M) / 2) does not underflow where w = e e does, and a key whose w is far
 // below 2^-126 may well have its share (e 2^-v) e of the sum, as pages of zeros do (their scale is
 // 2^-100).  So w <= 4 and 64 w stays in e4m3's
-// range whatever the scales are; two terms leave an error of at most 2^-8 w down to w = 2^-26, below
-// that 2^-34 (five: 2^-20 w, 2^-46).  Thread t of
+// range whatever the scales are; three terms leave an error of at most 2^-11 w down to w = 2^-26,
+// below that 2^-37 (five: 2^-20 w, 2^-46).  Thread t of
 // a group of 128 owns token t of the tile for 8 of the rows: scores, weights, its share of the row
 // sums; only the reference crosses threads.
 //
@@ -55,26 +56,30 @@ constexpr float kKeyGroup = 16384.0f;        // times 2^14
 
 template <typename T, int D, int RB, int CTAS>
 struct KeyShape {
-    static constexpr int kTerms = sizeof(T) == 4 ? 5 : 2;
+    static constexpr int kTerms = sizeof(T) == 4 ? 5 : 2;    // of q
+    static constexpr int kPTerms = sizeof(T) == 4 ? 5 : 3;   // of the weights
     static constexpr int kN = (RB * kTerms + 15) / 16 * 16;  // columns behind the terms are never read
     static constexpr int kSoft = RB * 16;                    // softmax threads
     static constexpr int kThreads = kSoft + 64;
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
-    static constexpr int kNP = 2 * RB * kTerms;              // column (2 i + group) RB + row: term i
-    // buffers of the scores and of the weights: two, so that no role waits; one where the fp32 terms'
-    // columns and bytes would cost the second CTA (16 rows) or the third slot of the ring (D = 256:
-    // 32 requests of 8000 keys 82 us with two buffers and two slots)
-    static constexpr int kBufs = sizeof(T) == 4 && (RB == 16 || D == 256) ? 1 : 2;
+    static constexpr int kNP = 2 * RB * kPTerms;             // column (2 i + group) RB + row: term i
     static constexpr int kQ = kN * D;
     static constexpr int kP = kNP * kKeyTile;                // one buffer
-    static constexpr int kFixed = kQ + kBufs * kP + 1024;
     static constexpr int kCtas = CTAS;                       // per SM
     using Tile = KeyTile<D, true>;                    // K and V of a tile
     static constexpr int kSlot = Tile::kSlot;
-    static constexpr int kFit = (kKeySmem / kCtas - 6144 - kFixed) / kSlot;  // static arrays and 1 KB per CTA beside it
-    static constexpr int kSlots = kFit > kKeyMaxSlots ? kKeyMaxSlots : kFit;
-    static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kSlot + kFixed;
+    static constexpr int fixed(int bufs) { return kQ + bufs * kP + 1024; }
+    static constexpr int slots(int bufs) {
+        const int fit = (kKeySmem / kCtas - 6144 - fixed(bufs)) / kSlot;  // static arrays and 1 KB per CTA beside it
+        return fit > kKeyMaxSlots ? kKeyMaxSlots : fit;
+    }
+    // Buffers of the scores and of the weights: two, so that no role waits, unless the second costs
+    // a slot of the ring (fp32 at D = 256: 32 requests of 8000 keys 82 us with two buffers and two
+    // slots, 67 with one and three) or does not fit tensor memory.
+    static constexpr int kBufs = slots(2) == slots(1) && (2 * kN + kChunks * kNP) * CTAS <= 512 ? 2 : 1;
+    static constexpr int kSlots = slots(kBufs);
+    static constexpr size_t kSmem = static_cast<size_t>(kSlots) * kSlot + fixed(kBufs);
     static constexpr int kColsUsed = kBufs * kN + kChunks * kNP;
     static constexpr int kCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
     static_assert(kSlots >= 2 && kN % 16 == 0 && kNP % 16 == 0 && kColsUsed * kCtas <= 512, "shape");
@@ -90,7 +95,7 @@ template <typename T, int D, int RB, int CTAS>
 __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T, D, RB, CTAS>::kCtas)
     kv8_attn_keys_kernel(const __grid_constant__ KeyArgs ka) {
     using S = KeyShape<T, D, RB, CTAS>;
-    constexpr int N = S::kN, NP = S::kNP, TERMS = S::kTerms, BUFS = S::kBufs, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
+    constexpr int N = S::kN, NP = S::kNP, TERMS = S::kTerms, PT = S::kPTerms, BUFS = S::kBufs, CW = S::CW, SL = S::kSlots, SOFT = S::kSoft;
     constexpr uint32_t kO = BUFS * N;  // tensor memory columns: scores, O
     constexpr int NT = S::kThreads, W_LOAD = SOFT / 32, W_MMA = W_LOAD + 1;
     const Kv8AttnArgs& a = ka.a;
@@ -342,8 +347,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                         tc_fence_after();
 #pragma unroll 1  // rare: little code
                         for (int c = 0; c < S::kChunks; ++c)
-#pragma unroll(TERMS == 2 ? 2 : 1)
-                            for (int b = 0; b < 2 * TERMS; ++b) {
+#pragma unroll(PT == 3 ? 2 : 1)
+                            for (int b = 0; b < 2 * PT; ++b) {
                                 float o[8];
                                 tc_ld8(lanes + kO + c * NP + b * RB, o);
                                 tc_wait_ld();
@@ -392,15 +397,15 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
                     }
                 }
                 uint8_t* p = s_p + x % BUFS * S::kP + tt * 16;
-                uint32_t code[4][TERMS];
+                uint32_t code[4][PT];
 #pragma unroll
-                for (int r = 0; r < 8; r += 2) e4m3_split2<TERMS>(y[r], y[r + 1], code[r / 2]);
+                for (int r = 0; r < 8; r += 2) e4m3_split2<PT>(y[r], y[r + 1], code[r / 2]);
                 const uint32_t m0 = sign_bytes(below[0], below[1], below[2], below[3]);
                 const uint32_t m1 = sign_bytes(below[4], below[5], below[6], below[7]);
                 if (BUFS == 1 && i > 0 && !mbar_try_wait(&pv_done[0], phase(x - 1)))
                     ok = ok && mbar_wait_bounded(&pv_done[0], phase(x - 1), a.err, abort_flag);
 #pragma unroll
-                for (int b = 0; b < TERMS; ++b) {
+                for (int b = 0; b < PT; ++b) {
                     const uint32_t c0 = code[0][b] | (code[1][b] << 16), c1 = code[2][b] | (code[3][b] << 16);
                     uint8_t* at = p + 2 * b * RB / 16 * (kKeyTile * 16);
                     if constexpr (RB == 8) {
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll
                 for (int r = 0; r < 8; ++r) o[r] = 0.0f;
 #pragma unroll
-                for (int b = 0; b < TERMS; ++b) {
+                for (int b = 0; b < PT; ++b) {
                     float v[2][8];
                     tc_ld8(lanes + kO + c * NP + 2 * b * RB, v[0]);
                     tc_ld8(lanes + kO + c * NP + (2 * b + 1) * RB, v[1]);

@@ -87,12 +87,12 @@ DM_DEV uint32_t e4m3_take2(__half2& h) {
     h = __hmul2(__hsub2(h, back), __float2half2_rn(16.0f));
     return c;
 }
-// e4m3 terms of two values of magnitude up to 448, term i scaled by 2^4i.  Two terms hold the 8
-// bits of the value as fp16; with five the first three take its 11 bits and the other two 8 bits
+// e4m3 terms of two values of magnitude up to 448, term i scaled by 2^4i.  Two terms hold 8 bits of
+// the value as fp16, three its 11; with five the first three take its 11 bits and the other two 8 bits
 // of the rest, 2^12 times of which is an fp16 value again: 2^-20 of the value, or 2^-26.
 template <int TERMS>
 DM_DEV void e4m3_split2(float a, float b, uint32_t (&t)[TERMS]) {
-    static_assert(TERMS == 2 || TERMS == 5, "terms");
+    static_assert(TERMS == 2 || TERMS == 3 || TERMS == 5, "terms");
     __half2 h = __floats2half2_rn(a, b);
     __half2 rest = h;
     if constexpr (TERMS == 5) {
@@ -101,8 +101,8 @@ DM_DEV void e4m3_split2(float a, float b, uint32_t (&t)[TERMS]) {
     }
     t[0] = e4m3_take2(h);
     t[1] = e4m3_take2(h);
+    if constexpr (TERMS > 2) t[2] = e4m3_take2(h);
     if constexpr (TERMS == 5) {
-        t[2] = e4m3_take2(h);
         rest = __hadd2(rest, h);  // what small values still have left, at the same scale
         t[3] = e4m3_take2(rest);
         t[4] = e4m3_take2(rest);

@@ -29,8 +29,8 @@ def tolerance(cache, q, scale, ref, keys, on_query_side):
     fp32 by 2^-20 of the element or 2^-26 of 2^8, the largest being at least 2^7.  Weights, sums in
     fp32: on the query side three e5m2 terms of 2^11 w, each holding the next 3 bits: off by 2^-9 of
     themselves (and 2^-11 on the way through fp16) or 2^-28 (half of 2^-16 / 2^11).  On the key side e4m3 terms of 64 w, or of 2^20 w for w < 2^-12, each term off by 2^-4 of
-    itself and the next one holding 16 times that: two terms 2^-8 (and 2^-11 on the way through
-    fp16) or 2^-34 (half of 2^-9 / 16 / 2^20), five 2^-20 or 2^-46.  What is absolute is relative to
+    itself and the next one holding 16 times that: three terms 2^-12 (and 2^-11 on the way through
+    fp16) or 2^-38 (half of 2^-9 / 256 / 2^20), five 2^-20 or 2^-46.  What is absolute is relative to
     a reference that the row's largest p sV is never below; doubled or
     more for the rounding on the way.  bf16 results are rounded once."""
     out, (mag, small), sat, _ = ref
@@ -40,7 +40,7 @@ def tolerance(cache, q, scale, ref, keys, on_query_side):
     e = sat * (d / 16 + 1) * 2.0 ** -22 + size * ((2.0 ** -17 if on_query_side else 2.0 ** -21) if bf16 else 2.0 ** -25)
     if not bf16:
         e = e + sat * 2.0 ** -20
-    rel, low = (2.0 ** -9 + F16_STEP, 2.0 ** -27) if on_query_side else (2.0 ** -8 + F16_STEP, 2.0 ** -32) if bf16 else (2.0 ** -20, 2.0 ** -44)
+    rel, low = (2.0 ** -9 + F16_STEP, 2.0 ** -27) if on_query_side else (2.0 ** -12 + F16_STEP, 2.0 ** -36) if bf16 else (2.0 ** -20, 2.0 ** -44)
     tol = (2 * e[..., None] + (keys / PAGE + 4) * 2.0 ** -22 + rel) * mag + low * small
     return tol + (BF16_STEP * np.abs(out) if bf16 else 0) + 1e-30, e
 
