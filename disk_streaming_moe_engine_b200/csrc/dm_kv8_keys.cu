@@ -63,7 +63,7 @@ struct KeyShape {
     static constexpr int kThreads = kSoft + 64;
     static constexpr int CW = D >= 128 ? 128 : D;
     static constexpr int kChunks = D / CW;
-    static constexpr int kNP = 2 * RB * kPTerms;             // column (2 i + group) RB + row: term i
+    static constexpr int kNP = 2 * RB * kPTerms;             // per term and 8 rows: 8 columns of each group
     static constexpr int kQ = kN * D;
     static constexpr int kP = kNP * kKeyTile;                // one buffer
     static constexpr int kCtas = CTAS;                       // per SM
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
         // ---------------- softmax, epilogue, Q ----------------
         const int tt = tid & 127, r0 = tid / 128 * 8, wq = warp & 3;  // token, first row, warp of the group
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + r0;
+        const uint32_t o_lanes = tmem + (static_cast<uint32_t>(32 * wq) << 16) + kO + 2 * r0;
         uint32_t t = 0;
         int item = 0;
         bool ok = true;     // of this thread; all leave together, after a barrier that ORs !ok
@@ -350,11 +351,12 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll(PT == 3 ? 2 : 1)
                             for (int b = 0; b < 2 * PT; ++b) {
                                 float o[8];
-                                tc_ld8(lanes + kO + c * NP + b * RB, o);
+                                const uint32_t at = o_lanes + c * NP + (b >> 1) * (2 * RB) + (b & 1) * 8;
+                                tc_ld8(at, o);
                                 tc_wait_ld();
 #pragma unroll
                                 for (int r = 0; r < 8; ++r) o[r] *= fac[r];
-                                tc_st8(lanes + kO + c * NP + b * RB, o);
+                                tc_st8(at, o);
                             }
                         tc_wait_st();
                     }
@@ -407,13 +409,7 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll
                 for (int b = 0; b < PT; ++b) {
                     const uint32_t c0 = code[0][b] | (code[1][b] << 16), c1 = code[2][b] | (code[3][b] << 16);
-                    uint8_t* at = p + 2 * b * RB / 16 * (kKeyTile * 16);
-                    if constexpr (RB == 8) {
-                        *reinterpret_cast<uint4*>(at) = make_uint4(c0 & ~m0, c1 & ~m1, c0 & m0, c1 & m1);
-                    } else {
-                        *reinterpret_cast<uint2*>(at + r0) = make_uint2(c0 & ~m0, c1 & ~m1);
-                        *reinterpret_cast<uint2*>(at + kKeyTile * 16 + r0) = make_uint2(c0 & m0, c1 & m1);
-                    }
+                    *reinterpret_cast<uint4*>(p + (b * RB + r0) / 8 * (kKeyTile * 16)) = make_uint4(c0 & ~m0, c1 & ~m1, c0 & m0, c1 & m1);
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
@@ -460,8 +456,8 @@ __global__ void __launch_bounds__(KeyShape<T, D, RB, CTAS>::kThreads, KeyShape<T
 #pragma unroll
                 for (int b = 0; b < PT; ++b) {
                     float v[2][8];
-                    tc_ld8(lanes + kO + c * NP + 2 * b * RB, v[0]);
-                    tc_ld8(lanes + kO + c * NP + (2 * b + 1) * RB, v[1]);
+                    tc_ld8(o_lanes + c * NP + 2 * b * RB, v[0]);
+                    tc_ld8(o_lanes + c * NP + 2 * b * RB + 8, v[1]);
                     tc_wait_ld();
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
