@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(512) rope_kernel(const __grid_constant__ RopeA
 // head's K or V: all its rows in registers, the largest magnitude over the CTA, then the
 // codes; the page's older codes are touched only when the scale grows.  Bound by the bytes for
 // prompts, read once (bf16 rows stay packed, 48 registers at D = 256 where fp32 copies took 64 and
-// 20.5 us): 17.5 k tokens of 2 heads of 256 take 14.4 us, 12.3 us with the rows in L2, against 8.3 us
-// for the bytes; the difference is the launch and one chain of slot, load, maximum, barrier, store.
+// 20.5 us): 17.5 k tokens of 2 heads of 256 take 15.5 us, 13.2 us with the rows partly in L2, against
+// 8.3 us for the bytes; the difference is the launch and one chain of slot, load, maximum, barrier, store.
 // 64 single tokens take 2.3 us in a graph, that chain alone.
 struct Kv8AppendArgs {
     uint8_t* pages;
@@ -850,7 +850,10 @@ extern "C" int32_t dm_kv8_append(const dm_kv8_cache* c, int32_t dtype, int32_t n
     a.Hkv = c->num_kv_heads;
     a.num_pages = c->num_pages;
     // rows of a CTA: one when the rows may all be in pages of their own (a decode step), more
-    // for prompts, where a CTA per row would mostly find that an earlier one has its page
+    // for prompts, where a CTA per row would mostly find that an earlier one has its page.  us with 1 /
+    // 4 / 16 rows, cold, 2 heads of 256 in bf16: 500 single tokens 8 / 10 / 23, 2000 16 / 16 / 24, 2000 of
+    // prompts 10 / 8 / 10; 3000 single 21 / 21 / 25, 8000 45 / 39 / 43, 7000 of prompts 23 / 12 / 14;
+    // 9000 27 / 14 / 14, 17000 42 / 23 / 18
     a.window = n <= 2048 ? 1 : n <= 8192 ? 4 : 16;
     a.vec = kv8_aligned(k, k_rs, k_hs, elem, 16) && kv8_aligned(v, v_rs, v_hs, elem, 16);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -93,9 +93,9 @@ extern "C" int32_t dm_kv8_attention(const dm_kv8_cache* c, const dm_kv8_attn_arg
     // Many bf16 rows per request and kv head: queries on the M side, 128 rows at a time.  The
     // key-side kernel goes over the cache once per 16 rows but joins small parts; with few items a
     // query-side item is cut into many large ones.  us on the key side / the query side at D = 64
-    // and D = 256 (2 kv heads): 128 items (64 requests of 1000 keys) 32 rows 32/32 49/56, 48 rows
-    // 41/32 66/55; 16 items (8 of 4000) 64 rows 29/31 40/46, 128 rows 37/31 55/49; 4 items (2 of
-    // 30000) 128 rows 46/47 80/117.
+    // and D = 256 (2 kv heads of 8 query heads): 128 items (64 requests of 1000 keys) 32 rows 34/33
+    // 52/53, 40 rows 44/33 69/54; 16 items (8 of 4000) 64 rows 31/30 43/48, 96 rows 36/31 51/49; 4 items
+    // (2 of 30000) 128 rows 52/51 91/118, 192 rows 68/52 120/115.
     const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
     const int64_t items = (rows + 127) / 128 * a.n * a.Hkv;
     const bool many = !f32 && rows >= (2 * items >= g.num_sms ? 40 : items >= 8 ? 96 : 192);

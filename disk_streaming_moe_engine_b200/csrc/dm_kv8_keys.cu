@@ -8,16 +8,17 @@
 //   O^T [D x NP]        += codeV^T [D x 128] . Pterms [128 x NP]
 // N = RB rows x TERMS columns: q and the softmax weights enter as sums of e4m3 terms, term i
 // scaled by 2^-4i in columns of its own, so a term adds 4 bits (at least 2^-4 of what the terms
-// before it left) and costs only N: 2 terms hold bf16's 8 bits of q, its weights take 3 (2^-11, so
+// before it left) and costs only N: 2 terms hold bf16's 8 bits of q, its weights take 3 (2^-10, so
 // that the result is as good as its rounding; 2 were 2 to 4 % faster), fp32 5 for both (2^-20).
 // Weights need range as well: thousands of keys may lie many nats below one whose V is small.  So NP
 // is twice their terms: a weight below 2^-12 of the reference enters 2^14 times larger in columns of
 // its own, the others' columns hold zero there (one group of columns lost all below 2^-19).  The tensor
 // time of a tile is that of reading 128 x 32 operand bytes per instruction whatever N <= 64 is, far
 // below the time of the tile's bytes from HBM, which is what bounds long caches: 64 requests of
-// 32768 tokens (2 kv heads of 256, 8 query heads each) take 346 us, 6.21 TB/s, 0.96 of the measured
-// copy bandwidth.  Short ones are bound by the chain of waits of one tile (0.65 us and more) and of
-// an item's start, end and join (2 to 4 us): one request of 4096 tokens takes 18 us.
+// 32768 tokens (2 kv heads of 256, 8 query heads each) take 348 us in a graph, 6.2 TB/s or 0.96 of the
+// measured copy bandwidth, 367 us called with cold inputs.  Short ones are bound by the chain of waits
+// of one tile (0.65 us and more) and of an item's start, end and join (2 to 4 us): one request of 4096
+// tokens takes 19 us.
 //
 // Softmax in base 2: with a page's scales sK, sV = 2^v,
 //   x = q . k (scaled, in log2 units),  w = 2^(x + v - M),  o = sum w codeV / sum w 2^-v,
@@ -26,7 +27,7 @@
 // log2 units: e = 2^((x + v - M) / 2) does not underflow where w = e e does, and a key whose w is far
 // below 2^-126 may well have its share (e 2^-v) e of the sum, as pages of zeros do (their scale is
 // 2^-100).  So w <= 4 and 64 w stays in e4m3's
-// range whatever the scales are; three terms leave an error of at most 2^-11 w down to w = 2^-26,
+// range whatever the scales are; three terms leave an error of at most 2^-10 w down to w = 2^-26,
 // below that 2^-37 (five: 2^-20 w, 2^-46).  Thread t of
 // a group of 128 owns token t of the tile for 8 of the rows: scores, weights, its share of the row
 // sums; only the reference crosses threads.
@@ -611,7 +612,7 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
 // CTAs per SM.  A tile's chain of waits takes 0.65 us and more whatever D is, its bytes from HBM
 // 0.37 us at D = 64 and 1.5 us at D = 256: two CTAs overlap their chains where they fit (D <= 128).
 // With 16 rows two leave each thread 96 registers, with some spills: fp32 chunks of 5 x 150 rows at
-// D = 128 took 365 us against 461 us with one (326 us now that an item's end is little code), but
+// D = 128 took 365 us against 461 us with one, at an earlier state (360 us now), but
 // one token of 16 heads (32 x 8000 keys) 48 us against 45 us, so one token per request takes one
 // CTA there.
 template <typename T, int RB>

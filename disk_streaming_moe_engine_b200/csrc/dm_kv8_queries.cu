@@ -36,10 +36,11 @@
 // without work.
 //
 // Bound by the softmax warps' instructions and the products together: 4 prompts of 8192 tokens,
-// 16 query heads on 2 kv heads of 256, take 1.95 ms, 1.13 PFLOP/s or 0.68 of the measured bf16 rate
-// (D = 128 1.49 ms for the same q).  Two prompts of 4096: tensor pipe busy 45 % of the cycles, ALU
-// 36 %, the exponential's unit 23 %.  Slower: a polynomial for every fourth exponential (2.30 ms),
-// four threads per row (D = 128 1.60 ms), 32 columns at a time in the join (prompts 2.03 ms).
+// 16 query heads on 2 kv heads of 256, take 2.05 ms in a graph of three, 1.07 PFLOP/s or 0.64 of the
+// measured bf16 rate, and 2.34 to 2.44 ms back to back under the power cap.  Two prompts of 4096: tensor
+// pipe busy 54 % of the cycles, ALU 33 %, the exponential's unit 22 %.  Slower, measured with two e4m3
+// terms per weight (1.95 ms): a polynomial for every fourth exponential (2.30 ms), four threads per row
+// (D = 128 1.49 -> 1.60 ms), 32 columns at a time in the join (2.03 ms).
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -52,7 +53,8 @@ constexpr int kQryRows = 128;
 constexpr int kQrySoft = 256;
 constexpr int kQryThreads = kQrySoft + 96;  // the softmax, then three warps
 // an item's start and end in tiles (KeyWalk): q rows to terms and the first scores before, O after,
-// which cost this kernel as much as 6 tiles do; ranges cut by tiles alone end up to that much apart
+// which cost this kernel as much as 6 tiles do; ranges cut by tiles alone end up to that much apart (one
+// prompt of 8192 at D = 64 / 128 / 256 with 3: 374 / 430 / 715 us, 6: 387 / 397 / 524, 9: 400 / 409 / 522)
 constexpr int kQryLead = 6;
 // log2 units a weight may exceed the reference by: a raise makes the row wait for the O product before
 // and holds up the tile (2: 426 / 432 / 577 us for the three prompts above, 3: 380 / 401 / 534, 4: 376 /

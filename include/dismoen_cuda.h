@@ -516,7 +516,8 @@ int32_t dm_kv8_status(uint32_t* err_dev, void* stream, char* err_buf, uint64_t e
  * All or nothing: when pages, the table's width, max_tokens or free_capacity do not suffice
  * (DM_DEVERR_CAPACITY) or a length is negative (DM_DEVERR_RANGE), no page moves, the
  * lengths stay ctx_lens, cu_new is all 0 and the token arrays all -1.
- * n * table_width <= 2^27, max_tokens <= 2^30.  No overlap but the two named. */
+ * n * table_width <= 2^27, 1 <= max_tokens <= 2^30 (a step without new tokens passes room for
+ * one).  No overlap but the two named. */
 int32_t dm_kv8_plan(int32_t n, const int32_t* ctx_lens, const int32_t* new_lens, int32_t* block_table,
                     int32_t table_width, int32_t* free_pages, int32_t free_capacity, const int32_t* free_state,
                     int32_t* free_state_out, int32_t* seq_lens, int32_t* cu_new, int32_t max_tokens, int32_t* slots,
@@ -591,7 +592,12 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * range is left out (DM_DEVERR_PAGE), and so are keys beyond the table's width
  * (DM_DEVERR_CAPACITY).  NaN codes of keys that a query does not see do not reach it; one in
  * V that it sees makes that element NaN, one in K its whole row.
- * dtype (q and out) bf16 or fp32; scores, softmax and sums are fp32.
+ * dtype (q and out) bf16 or fp32.  Scores, maxima, sums and O are fp32 (bf16 q exact to 2^-17
+ * of the row's largest element, fp32 q to 2^-20).  The weights in front of V are rounded, the
+ * sums that divide are not: fp32 to 2^-20 of themselves down to 2^-26 of the row's largest
+ * (times V's page scale) and by 2^-46 of it below; bf16 to 2^-10 and 2^-37, or, from 40 to
+ * 192 query rows per request and kv head on (by the number of requests), to 2^-8 down to
+ * 2^-19 and by 2^-28 below.  bf16 divides by a reciprocal of 2 units of fp32.
  * lse (may be NULL) [rows][Hq] receives ln sum exp of the scaled scores.
  * workspace: dm_kv8_attention_workspace bytes, 256-byte aligned, zeroed once before its
  * first use; every call leaves it ready for the next (after a DM_DEVERR_TIMEOUT it has to be
