@@ -50,7 +50,7 @@ namespace dm {
 
 constexpr int kKeySmem = 227 * 1024;         // shared memory of an SM for its CTAs
 constexpr int kKeyLead = 1;                  // an item's start and end in tiles (KeyWalk)
-constexpr float kKeyLazy = 1.0f;             // what a half log2 weight may exceed its reference by
+constexpr float kKeyLazy = 1.0f;             // what a weight may exceed the reference by, in halves of log2 units
 constexpr float kKeyBoost = 64.0f;           // weights enter as 64 w <= 256
 constexpr float kKeySmall = 1.0f / 64;       // e of those in the second group of columns, below 2^-12 and
 constexpr float kKeyGroup = 16384.0f;        // times 2^14
@@ -611,10 +611,11 @@ static cudaError_t launch_keys(const KeyArgs& ka, int num_sms, int dev, cudaStre
 
 // CTAs per SM.  A tile's chain of waits takes 0.65 us and more whatever D is, its bytes from HBM
 // 0.37 us at D = 64 and 1.5 us at D = 256: two CTAs overlap their chains where they fit (D <= 128).
-// With 16 rows two leave each thread 96 registers, with some spills: fp32 chunks of 5 x 150 rows at
-// D = 128 took 365 us against 461 us with one, at an earlier state (360 us now), but
-// one token of 16 heads (32 x 8000 keys) 48 us against 45 us, so one token per request takes one
-// CTA there.
+// With 16 rows two leave each thread 96 registers, with some spills.  us with two / with one, fp32 and
+// bf16: D = 64, 32 requests of 2000 to 8000 keys with 3 tokens 48/56 and 48/53, of 8000 keys with one
+// token of 16 heads per kv head 45/48 and 39/41; 5 chunks of up to 300 rows in fp32 156/204 (D = 128
+// 359/469); D = 128, 32 requests with 3 tokens 70/70 and 61/60.  One token at D = 128 took 48 us with
+// two and 45 with one, so it takes one there.
 template <typename T, int RB>
 static cudaError_t launch_keys_d(const KeyArgs& ka, int D, int num_sms, int dev, cudaStream_t s) {
     if (D == 64) return launch_keys<T, 64, RB, 2>(ka, num_sms, dev, s);
