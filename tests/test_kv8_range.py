@@ -495,3 +495,50 @@ def test_calls_at_the_same_time(lib):
         for _, want, _, _, out, _ in cases:
             assert torch.equal(out, want)
     kv8.check(err)
+
+
+# ---- CPU: flags, and the arithmetic of the weights' terms --------------------------------------------------------
+
+def test_attention_flags(lib):
+    """DM_KV8_FILL_ROWS alone is known; an empty call needs no device."""
+    import ctypes as C
+    cache = _lib.DmKv8Cache(1 << 20, 1 << 21, 4, 2, 128, 0)
+    for flags, want in ((0, _lib.DM_OK), (kv8.FILL_ROWS, _lib.DM_OK), (4, _lib.DM_ERR_INVALID_ARG), (3, _lib.DM_ERR_INVALID_ARG)):
+        a = _lib.DmKv8AttnArgs(dtype=0, n=0, num_q_heads=8, max_q_len=1, rows=0, table_width=1, sm_scale=1.0, flags=flags)
+        buf = C.create_string_buffer(512)
+        assert lib.dm_kv8_attention(C.addressof(cache), C.addressof(a), None, buf, 512) == want
+
+
+def test_three_e5m2_terms_hold_nine_bits():
+    """Upper bytes of fp16 values: the value's, of what is left, of what is left then (rounded)."""
+    x = np.exp2(np.random.default_rng(0).uniform(-30, 15, 200000))
+    h = x.astype(np.float16)
+    total = np.zeros_like(x)
+    for i in range(3):
+        bits = h.view(np.uint16)
+        top = ((bits + 0x80) if i == 2 else bits) & 0xff00
+        part = top.astype(np.uint16).view(np.float16)
+        total += part.astype(np.float64)
+        h = (h - part).astype(np.float16)
+    off = np.abs(total - x)
+    # the rounding to fp16 (2^-11, or half of its smallest step 2^-24) comes on top of what the terms
+    # leave (2^-9, or half of e5m2's smallest step 2^-16)
+    assert (off <= x * F16_STEP + 2.0 ** -25 + np.maximum(x * 2.0 ** -9, 2.0 ** -17)).all()
+    assert total[x < 2.0 ** -26].max() == 0  # where a page's scores go that only count in the sum
+
+
+def test_e4m3_terms_in_two_groups():
+    """64 w, or 2^20 w below 2^-12, as three e4m3 terms of scales 1, 1/16, 1/256."""
+    from test_kv8 import to_e4m3
+    w = np.exp2(np.random.default_rng(1).uniform(-40, 2, 20000))
+    scale = np.where(w < 2.0 ** -12, 2.0 ** 20, 64.0)
+    rest = (w * scale).astype(np.float16).astype(np.float64)
+    total = np.zeros_like(w)
+    for i in range(3):
+        part = E4M3[to_e4m3(rest)]
+        total += part / 16.0 ** i
+        rest = (rest - part) * 16
+    off = np.abs(total / scale - w)
+    # fp16 (2^-11, or half of 2^-24), then the terms (2^-12, or half of 2^-9 / 256), of 2^20 w where
+    # the smallest steps count
+    assert (off <= w * (2.0 ** -12 + F16_STEP) + (2.0 ** -25 + 2.0 ** -18) / 2.0 ** 20).all()
