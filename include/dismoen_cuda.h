@@ -593,7 +593,8 @@ int32_t dm_kv8_append(const dm_kv8_cache* cache_host, int32_t dtype, int32_t n, 
  * (DM_DEVERR_CAPACITY).  NaN codes of keys that a query does not see do not reach it; one in
  * V that it sees makes that element NaN, one in K its whole row.
  * dtype (q and out) bf16 or fp32.  Scores, maxima, sums and O are fp32 (bf16 q exact to 2^-17
- * of the row's largest element, fp32 q to 2^-20).  The weights in front of V are rounded, the
+ * of the row's largest element, fp32 q to 2^-20; a score carries log2 of its page's V scale,
+ * whose size in units of 2^-24 it is rounded by: 2^-20 for scales of 2^-16, 2^-17 for 2^-100).  The weights in front of V are rounded, the
  * sums that divide are not: fp32 to 2^-20 of themselves down to 2^-26 of the row's largest
  * (times V's page scale) and by 2^-46 of it below; bf16 to 2^-10 and 2^-37, or, from 40 to
  * 192 query rows per request and kv head on (by the number of requests), to 2^-8 down to
